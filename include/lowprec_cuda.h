@@ -356,6 +356,98 @@ int lp_dequantize_nvfp4(const uint8_t *codes, int64_t codes_len, const uint8_t *
                         int64_t scales_len, float global_decode_scale, float *dst,
                         int64_t dst_len, lp_stream_t stream);
 
+/* ======================= paged key/value cache and its attention ======= */
+/* What stands between the projections of a decoder layer and its output
+ * projection (no counterpart in the reference, which ends at the products).
+ * Keys and values live in pages of page_size tokens; slot s is token
+ * s mod page_size of page s div page_size.  Device pointers, stream-ordered,
+ * nothing allocated. */
+
+/* element types of the cache and of the rows that go in and out */
+#define LP_F32 0
+#define LP_F16 1
+#define LP_BF16 2
+#define LP_I8 3 /* cache only: int8 codes, one fp32 scale per (token, head) */
+
+/* The cache: element (page, token, head, i) of k is at
+ * k[page*k_strides[0] + token*k_strides[1] + head*k_strides[2] + i], strides
+ * in elements, so pages may hold tokens x heads or heads x tokens.  Rows
+ * start on 16-byte boundaries (pointers and strides).  LP_I8: the value is
+ * code * scale, the scale of (page, token, head) found by its own strides. */
+typedef struct lp_kv_cache {
+  void *k, *v;
+  float *k_scales, *v_scales; /* LP_I8 only */
+  int64_t pages, page_size, kv_heads;
+  int64_t k_strides[3], v_strides[3];
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  int32_t dtype;    /* LP_F16, LP_BF16, LP_I8 */
+  int32_t head_dim; /* a multiple of 16, at most 256; attention: 64, 96, 128 */
+} lp_kv_cache;
+
+/* Rows of head_dim elements: row (token, head) at
+ * data[token*token_stride + head*head_stride]; any strides and alignment. */
+typedef struct lp_rows {
+  void *data;
+  int64_t tokens, heads, token_stride, head_stride;
+  int32_t dtype; /* LP_F32, LP_F16, LP_BF16 */
+  int32_t reserved;
+} lp_rows;
+
+/* Page tables and slot maps from request lengths, in one launch.  Request b
+ * has ctx_lens[b] tokens in the cache and gets new_lens[b] more.  The pages
+ * it lacks are taken in request order from free_pages[free_head[0]..] and
+ * written behind its last one in block_tables (row b, table_width entries,
+ * rows table_stride apart); -1 where the list has run out.  Out: q_start
+ * (requests + 1: first flat token of each request), seq_lens (ctx + new),
+ * and for each flat token its slot and position, -1 past the last token and
+ * (the slot) where there is no page; free_head_out = the next free entry.
+ * positions may be null.  free_head_out must not be free_head: the two
+ * alternate from step to step.  Negative lengths count as 0. */
+int lp_assign_pages(const int32_t *ctx_lens, int64_t ctx_lens_len, const int32_t *new_lens,
+                    int64_t new_lens_len, int64_t page_size, const int32_t *free_pages,
+                    int64_t free_pages_len, const int32_t *free_head, int32_t *block_tables,
+                    int64_t table_width, int64_t table_stride, int32_t *q_start,
+                    int64_t q_start_len, int32_t *seq_lens, int64_t seq_lens_len, int64_t *slots,
+                    int64_t slots_len, int32_t *positions, int64_t positions_len,
+                    int32_t *free_head_out, lp_stream_t stream);
+
+/* Write the key and value rows of new tokens to their slots; a token whose
+ * slot is outside the cache is skipped.  LP_I8: scale = absmax / 127 over the
+ * row (1 for a zero row) and code = round(x / scale), the bytes that
+ * lp_calibrate_symmetric and lp_quantize_batch give with group_size =
+ * head_dim.  Two tokens must not share a slot. */
+int lp_store_kv(const lp_kv_cache *cache, const lp_rows *k, const lp_rows *v,
+                const int64_t *slots, int64_t slots_len, lp_stream_t stream);
+
+/* Read rows back from their slots; zeros where a slot is outside the cache. */
+int lp_load_kv(const lp_kv_cache *cache, const int64_t *slots, int64_t slots_len,
+               const lp_rows *k, const lp_rows *v, lp_stream_t stream);
+
+/* Bytes of workspace that lp_paged_attention takes on the current device.
+ * The workspace is zeroed once, when it is allocated; every call leaves it
+ * ready for the next one on the same stream.  Calls that may run at the same
+ * time need one each. */
+int lp_paged_attention_workspace(int64_t *bytes);
+
+/* Attention of each request's new tokens over its cached keys (the new ones
+ * among them, stored before).  Request b's rows of q are q_start[b] ..
+ * q_start[b+1]; the last of them is at position seq_lens[b] - 1.  A token at
+ * position p sees key j of its request if j <= p, j's page is in the table
+ * (an entry in [0, pages)), and, with window > 0, j > p - window or
+ * j < sinks.  Query head h reads key head h div (heads / kv_heads).
+ *   out = sum_j exp(s_j) v_j / sum_j exp(s_j),  s_j = scale * (q . k_j)
+ * in fp32 inside, rounded once to out's type (= q's); lse (may be null;
+ * tokens x heads) = log sum_j exp(s_j).  A row that sees no key gives zeros
+ * and -inf.  Keys that a row does not see do not touch it, whatever they
+ * hold.  Rows of q outside every request are left alone in out.  out must
+ * not overlap q. */
+int lp_paged_attention(const lp_kv_cache *cache, const int32_t *block_tables, int64_t table_width,
+                       int64_t table_stride, const int32_t *q_start, int64_t q_start_len,
+                       const int32_t *seq_lens, int64_t seq_lens_len, const lp_rows *q,
+                       const lp_rows *out, float scale, int64_t window, int64_t sinks, float *lse,
+                       int64_t lse_len, void *workspace, int64_t workspace_len,
+                       lp_stream_t stream);
+
 /* ======================= host-pointer drop-in forms ==================== */
 /* Same arguments and meaning as the lp_* forms above, HOST pointers, no
  * stream; blocking.  Each replaces the same reference proc as its lp_* form

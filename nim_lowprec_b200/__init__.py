@@ -17,6 +17,8 @@ from .dequant import (  # noqa: F401
     quantizeDequantGemvQ8,
     quantizeQ4_0Batch, quantizeQ8_0, quantizeQ8_0Batch, quantizeQ8_0Split, fp32_mode,
     fp32Mode, gemmNVFP4, setFp32Mode)
+from .attention import (  # noqa: F401
+    KVCache, assignPages, attentionWorkspace, loadKV, pagedAttention, storeKV)
 from .ggml import QK, QK_K, BlockQ4_0, BlockQ4_K, BlockQ6_K, BlockQ8_0  # noqa: F401
 from . import parallel  # noqa: F401  (LpPool's row-sharded forms)
 

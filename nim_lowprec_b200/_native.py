@@ -21,6 +21,11 @@ LP_ERR_TIMEOUT = 5
 LP_ERR_UNSUPPORTED = 6
 LP_ERR_NO_DEVICE = 7
 
+LP_F32 = 0  # element types of the paged cache and its rows
+LP_F16 = 1
+LP_BF16 = 2
+LP_I8 = 3
+
 LP_FP32_FAST = 0
 LP_FP32_EXACT = 1
 
@@ -109,6 +114,11 @@ SIGNATURES = {
     "lp_dequant_gemv_q4_k": "pnnpnpnp",
     "lp_dequant_gemv_q6_k": "pnnpnpnp",
     "lp_gemm_nvfp4": "pnpnppnpnpnpnp",
+    "lp_assign_pages": "pnpnnpnppnnpnpnpnpnpp",
+    "lp_store_kv": "ppppnp",
+    "lp_load_kv": "ppnppp",
+    "lp_paged_attention_workspace": "p",
+    "lp_paged_attention": "ppnnpnpnppfnnpnpnp",
     "lph_pool_init": "pi",
     "lph_pool_shutdown": "p",
     "lph_pool_thread_count": "p",

@@ -1,0 +1,358 @@
+// attn.cuh -- what the paged-attention kernels share: their arguments, the
+// split of the work over the grid, the visible keys of a row, and the exact
+// recomputation of a row whose sum is not finite.
+//
+// Work split.  The query rows of request b and key head h are the pairs (new
+// token t, query head g of the group), r = t * G + g, in blocks of RB rows.
+// A block sees a contiguous run of keys (with a window: the sinks' run and the
+// window's run), cut into units of KU keys.  All units of all (b, h, block)
+// items are laid end to end and every CTA takes one contiguous, equal share,
+// so ragged lengths, few long requests and many short ones all fill the grid.
+// An item cut by a CTA boundary leaves partial results (running maximum, sum
+// and unnormalised output, fp32) in the workspace; the CTA that arrives last
+// adds them in CTA order, so results do not depend on the timing.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "lp_device.cuh"
+#include "lp_internal.h"
+
+namespace lp {
+namespace attn {
+
+struct Pool {  // one of the cache's two tensors; strides in elements
+  const uint8_t* data;
+  const float* scales;
+  int64_t page, token, head;     // strides of data
+  int64_t spage, stoken, shead;  // strides of scales
+};
+
+struct Args {
+  const void* q;
+  void* out;
+  float* lse;  // [tokens, heads] or null
+  int q_type;  // LP_F32 / LP_F16 / LP_BF16, out's too
+  int q_vec;   // rows of q and out start on 16-byte boundaries
+  int64_t q_token, q_head, o_token, o_head;
+  Pool k, v;
+  const int32_t* table;
+  const int32_t* qstart;
+  const int32_t* seqlens;
+  int64_t table_stride;
+  int table_width, pages, page_size;
+  int requests, tokens, heads, kv_heads, group;
+  int window, sinks;  // window 0: none
+  float scale_log2;   // softmax scale * log2(e)
+  uint32_t* counters;
+  float* partials;
+};
+
+// ------------------------------------------------------- requests, rows
+
+struct Request {
+  int start, n;  // first row of q, new tokens
+  int base;      // position of the first new token (may be negative)
+  int limit;     // keys the table can hold, at most the request's length
+};
+
+__device__ __forceinline__ Request request(const Args& a, int b) {
+  Request r;
+  r.start = min(max(__ldg(a.qstart + b), 0), a.tokens);
+  r.n = min(max(__ldg(a.qstart + b + 1), r.start), a.tokens) - r.start;
+  const int seq = max(__ldg(a.seqlens + b), 0);
+  r.base = seq - r.n;
+  r.limit = static_cast<int>(
+      min(static_cast<int64_t>(seq), static_cast<int64_t>(a.table_width) * a.page_size));
+  return r;
+}
+
+// Units that rows [row0, row0 + RB) of a request see: the first `sink` units
+// of the cache, then the units from `first` on.
+struct Units {
+  int sink, first, n;
+  int lo, hi;  // the window's run of keys, [lo, hi]
+};
+
+template <int KU, int RB>
+__device__ __forceinline__ Units units(const Args& a, const Request& r, int block) {
+  Units u;
+  const int rows = r.n * a.group;
+  const int p0 = r.base + block * RB / a.group;
+  const int p1 = r.base + (min(block * RB + RB, rows) - 1) / a.group;
+  u.hi = min(p1, r.limit - 1);
+  u.lo = a.window > 0 ? max(p0 - a.window + 1, 0) : 0;
+  const int sinks = a.window > 0 ? min(a.sinks, u.hi + 1) : 0;
+  u.sink = sinks > 0 ? (sinks + KU - 1) / KU : 0;
+  u.first = max(u.lo / KU, u.sink);
+  u.n = u.hi < 0 ? 0 : u.sink + max(u.hi / KU - u.first + 1, 0);
+  // a block that sees nothing still writes its zeros: one unit, all masked
+  if (u.n <= 0) {
+    u.n = 1;
+    u.sink = 0;
+    u.first = 0;
+  }
+  return u;
+}
+
+template <int KU, int RB>
+__device__ __forceinline__ int64_t request_units(const Args& a, int b) {
+  const Request r = request(a, b);
+  const int blocks = (r.n * a.group + RB - 1) / RB;
+  int64_t s = 0;
+  for (int i = 0; i < blocks; ++i) s += units<KU, RB>(a, r, i).n;
+  return s;
+}
+
+// ------------------------------------------------------- the CTA's share
+
+struct Cursor {
+  int64_t begin, end;  // the CTA's units
+  int64_t per_cta;     // units per CTA (the last ones may have fewer)
+  int64_t item0;       // number of the current item's first unit
+  int b, head, block;  // the current item
+  int pad;
+};
+
+// Total units and the item that holds unit `begin` of this CTA.  Each thread
+// sums a run of requests, the sums are scanned in shared memory, and the
+// thread whose run holds `begin` walks it.  All threads of the block call it.
+template <int KU, int RB, int THREADS>
+__device__ void find_share(const Args& a, int64_t min_units, Cursor* cur, int64_t* sums) {
+  const int t = threadIdx.x;
+  const int run = (a.requests + THREADS - 1) / THREADS;
+  const int b0 = min(t * run, a.requests), b1 = min(b0 + run, a.requests);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += request_units<KU, RB>(a, b);
+  mine *= a.kv_heads;
+  // inclusive scan: within the warp, then over the warps' totals
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if ((t & 31) >= o) inc += y;
+  }
+  if ((t & 31) == 31) sums[t >> 5] = inc;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < (t >> 5)) before += sums[w];
+    total += sums[w];
+  }
+  const int64_t excl = before + inc - mine;
+  const int64_t per = max((total + gridDim.x - 1) / static_cast<int64_t>(gridDim.x), min_units);
+  const int64_t begin = min(static_cast<int64_t>(blockIdx.x) * per, total);
+  if (t == 0) {
+    cur->begin = begin;
+    cur->end = min(begin + per, total);
+    cur->per_cta = per;
+  }
+  if (begin >= excl && begin < excl + mine) {
+    int64_t at = excl;
+    int b = b0;
+    int64_t w = request_units<KU, RB>(a, b);
+    while (begin >= at + w * a.kv_heads) {
+      at += w * a.kv_heads;
+      w = request_units<KU, RB>(a, ++b);
+    }
+    const int head = static_cast<int>((begin - at) / w);
+    at += head * w;
+    const Request r = request(a, b);
+    int block = 0;
+    int n = units<KU, RB>(a, r, 0).n;
+    while (begin >= at + n) {
+      at += n;
+      n = units<KU, RB>(a, r, ++block).n;
+    }
+    cur->b = b;
+    cur->head = head;
+    cur->block = block;
+    cur->item0 = at;
+  }
+  __syncthreads();
+}
+
+// The item after (b, head, block); every thread computes the same.
+template <int RB>
+__device__ __forceinline__ void next_item(const Args& a, int& b, int& head, int& block) {
+  Request r = request(a, b);
+  if (++block < (r.n * a.group + RB - 1) / RB) return;
+  block = 0;
+  if (++head < a.kv_heads) return;
+  head = 0;
+  do {
+    if (++b >= a.requests) return;
+    r = request(a, b);
+  } while (r.n == 0);
+}
+
+// CTAs that share an item of units [u0, u0 + n): first..last, and the slot of
+// a CTA's partial (0: its share begins inside the item or at its first unit).
+struct Sharers {
+  int first, last;
+};
+__device__ __forceinline__ Sharers sharers(int64_t u0, int64_t n, int64_t per) {
+  return {static_cast<int>(u0 / per), static_cast<int>((u0 + n - 1) / per)};
+}
+__device__ __forceinline__ int slot_of(int cta, int64_t u0, int64_t per) {
+  return 2 * cta + (u0 > static_cast<int64_t>(cta) * per ? 1 : 0);
+}
+
+// ------------------------------------------------------- element access
+
+__device__ __forceinline__ float load_elem(const void* p, int type, int64_t i) {
+  if (type == LP_F32) return static_cast<const float*>(p)[i];
+  if (type == LP_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+// One rounding, to the output's type.
+__device__ __forceinline__ void store_elem(void* p, int type, int64_t i, float v) {
+  if (type == LP_F32) static_cast<float*>(p)[i] = v;
+  else if (type == LP_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
+
+// Page of key j of request b, or -1 where the table has none.
+__device__ __forceinline__ int page_of(const Args& a, int b, int j) {
+  const int p = __ldg(a.table + b * a.table_stride + j / a.page_size);
+  return static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
+}
+
+template <class C>
+__device__ __forceinline__ float cache_elem(const Pool& p, int64_t row, int64_t srow, int d) {
+  if constexpr (C::kInt8) {
+    return static_cast<float>(reinterpret_cast<const int8_t*>(p.data)[row + d]) * p.scales[srow];
+  } else {
+    return C::to_float(reinterpret_cast<const uint16_t*>(p.data)[row + d]);
+  }
+}
+
+// One query row by one warp, key by key over its visible keys alone, fp32.
+// The tiled kernels give masked keys the weight 0; a 0 times an infinity or a
+// NaN that a masked key's value holds is a NaN.  So a row that ends not
+// finite is computed again here, where masked keys are never read: it is
+// finite if the row's own keys are.
+template <class C, int D>
+__device__ __noinline__ void exact_row(const Args& a, int b, int head, int t, int g) {
+  const int lane = threadIdx.x & 31;
+  const Request r = request(a, b);
+  const int pos = r.base + t;
+  const int qh = head * a.group + g;
+  const int64_t qrow = (r.start + t) * a.q_token + qh * a.q_head;
+  float q[D / 32], o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    q[i] = load_elem(a.q, a.q_type, qrow + lane + 32 * i);
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  const int end = min(pos + 1, r.limit);
+  const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+  for (int j = 0; j < end; ++j) {
+    if (j < lo && j >= a.sinks) j = lo;
+    if (j >= end) break;
+    const int page = page_of(a, b, j);
+    if (page < 0) continue;
+    const int off = j % a.page_size;
+    const int64_t kr = page * a.k.page + off * a.k.token + head * a.k.head;
+    const int64_t ks = page * a.k.spage + off * a.k.stoken + head * a.k.shead;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      s = fmaf(q[i], cache_elem<C>(a.k, kr, ks, lane + 32 * i), s);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    s *= a.scale_log2;
+    const float mn = fmaxf(m, s);
+    const float ref = mn == -INFINITY ? 0.0f : mn;
+    const float c = ex2(m - ref), p = ex2(s - ref);
+    m = mn;
+    l = fmaf(l, c, p);
+    const int64_t vr = page * a.v.page + off * a.v.token + head * a.v.head;
+    const int64_t vs = page * a.v.spage + off * a.v.stoken + head * a.v.shead;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      o[i] = fmaf(o[i], c, p * cache_elem<C>(a.v, vr, vs, lane + 32 * i));
+  }
+  const int64_t orow = (r.start + t) * a.o_token + qh * a.o_head;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+    store_elem(a.out, a.q_type, orow + lane + 32 * i, l == 0.0f ? 0.0f : __fdiv_rn(o[i], l));
+  if (a.lse && lane == 0)
+    a.lse[static_cast<int64_t>(r.start + t) * a.heads + qh] =
+        l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------- cache formats
+
+struct CF16 {
+  static constexpr bool kInt8 = false, kBf16 = false;
+  __device__ static float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+};
+struct CBF16 {
+  static constexpr bool kInt8 = false, kBf16 = true;
+  __device__ static float to_float(uint16_t v) {
+    return __uint_as_float(static_cast<uint32_t>(v) << 16);
+  }
+};
+struct CI8 {  // codes are widened to fp16, which holds them exactly
+  static constexpr bool kInt8 = true, kBf16 = false;
+};
+
+// (a, b) rounded to the 16-bit type of the tensor-core operands, a in the low half
+template <class C>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  uint32_t r;
+  if constexpr (C::kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <class C>
+__device__ __forceinline__ float low16(uint32_t w) {
+  if constexpr (C::kBf16) return __uint_as_float(w << 16);
+  else return h2f(w & 0xffffu);
+}
+template <class C>
+__device__ __forceinline__ float high16(uint32_t w) {
+  if constexpr (C::kBf16) return __uint_as_float(w & 0xffff0000u);
+  else return h2f(w >> 16);
+}
+
+// Bytes u0..u3 of w, each code + 128, to two packed pairs of fp16 codes:
+// 0x64 before a byte is the fp16 number 1024 + byte, and 1152 less is the code.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
+  const uint32_t x = prmt(w, 0x64646464u, sel);
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
+  return r;
+}
+
+// Two signed bytes of w to packed bf16: 0x43 before a byte's low seven bits is
+// 128 + those, before its top bit 128 or 256; the difference is the code.
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t sel) {
+  const uint32_t x = prmt(w, 0x43434343u, sel);
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0x437f437fu), "r"(x & 0x43804380u));
+  return r;
+}
+
+// The power of two that brings |x| <= amax below 1 (1 where amax is 0 or not
+// finite), as an exponent e: 2^-e * amax < 1 (< 4 next to the type's end).
+__device__ __forceinline__ int row_exponent(float amax) {
+  const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 126;
+  return amax == 0.0f || !finite(amax) ? 0 : min(max(e, -100), 126);
+}
+__device__ __forceinline__ float pow2(int e) {  // -126 <= e <= 127
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+}  // namespace attn
+}  // namespace lp

@@ -131,6 +131,22 @@ int launch_gemm_nvf4(const uint8_t* w, const uint8_t* ws, const float* gw, const
                      const uint8_t* xs, const float* gx, int64_t n, float* y, int64_t m, int64_t k,
                      cudaStream_t st);
 
+// paged cache (kvcache.cu) and its attention (attn_rows.cu)
+int launch_assign_pages(const int32_t* ctx, const int32_t* add, int64_t requests,
+                        int64_t page_size, const int32_t* free_pages, int64_t free_len,
+                        const int32_t* free_head, int32_t* table, int64_t table_stride,
+                        int64_t table_width, int32_t* qstart, int32_t* seqlens, int64_t* slots,
+                        int64_t tokens, int32_t* positions, int32_t* free_head_out,
+                        cudaStream_t st);
+int launch_store_kv(const lp_kv_cache& c, const lp_rows& k, const lp_rows& v, const int64_t* slots,
+                    bool vec, cudaStream_t st);
+int launch_load_kv(const lp_kv_cache& c, const int64_t* slots, const lp_rows& k, const lp_rows& v,
+                   bool vec, cudaStream_t st);
+namespace attn {
+struct Args;
+}
+int launch_attn_rows(const attn::Args& a, int cache_type, int dim, cudaStream_t st);
+
 // error words of the translation units whose kernels wait (read + clear)
 unsigned int take_error_gemv();
 unsigned int take_error_gemm_tc();
