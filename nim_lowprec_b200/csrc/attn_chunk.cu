@@ -1,0 +1,921 @@
+// attn_chunk.cu -- attention of a chunk of new tokens over a paged cache, on
+// the 5th-generation tensor cores.
+//
+//   S = Q K^T, P = exp2(c S - m), O += P V, l += sum P      (one pass over the keys)
+//
+// CTA = TILES row tiles of 128 query rows (token, head of the group) of one
+// key head, key tiles of 128 keys; 16 warps, of which
+//   warps 0-3, 4-7  softmax, one thread per row (tensor memory lane).  Two row
+//                   tiles: one warpgroup each.  One row tile: both share it,
+//                   64 keys each, and swap the row maxima in shared memory.
+//   warps 8-11      load keys and values into a ring of swizzled 128-key
+//                   tiles, 16 bytes a lane: pages may have any size and any
+//                   16-byte strides, and keys that no row of the tile sees
+//                   (past the end, before the window, on missing pages) are
+//                   zeros, whatever the cache holds there.  fp16 and bf16
+//                   pages go by cp.async; int8 codes through registers, where
+//                   they are widened (exactly) to the operand type.
+//   warp 12         one lane issues the products: tcgen05.mma kind::f16,
+//                   M = 128, S and O in tensor memory, P from tensor memory
+//                   (it takes the columns of the S it came from).
+// While one tile's softmax runs, the tensor cores work on the other tile, or,
+// with one row tile, on the next key tile's S (two S buffers).
+//
+// 16-bit queries: two row tiles, P in one part of the operand type.  fp32
+// results need more bits than one 16-bit operand has, so queries and weights
+// are split into two fp16 or three bf16 parts whose products add up in the
+// same fp32 accumulator; that is bound by the products, so one row tile and
+// the wider ring serve it.  Which types take which parts: launch_attn_chunk.
+//
+// The running maximum moves only when a row's grows by more than 2^8 (the
+// weights stay below 2^8 times 1, or 2^15 with fp16's extra 2^7): the sums are
+// the same and O is rescaled a few times per row rather than per key tile.
+#include <type_traits>
+
+#include "attn.cuh"
+#include "tc_ptx.cuh"
+
+namespace lp {
+namespace {
+
+using namespace attn;
+using namespace tc;
+
+constexpr int kKeys = 128;             // keys per tile, = one unit
+constexpr int kSoftThreads = 256;
+constexpr int kLoadThreads = 128;
+constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroups: setmaxnreg)
+constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
+constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
+constexpr int kMinUnits = 2;
+
+// C: the cache's format; Q: type of the operands of Q K^T, P: of P V;
+// NQ, NP: parts of queries and weights.
+template <class C_, class Q_, class P_, int NQ_, int NP_, int TILES_, int D_>
+struct Cfg {
+  using C = C_;
+  using Q = Q_;
+  using P = P_;
+  static constexpr int NQ = NQ_, NP = NP_, TILES = TILES_, D = D_;
+  static constexpr int BLOCKS = (D + 63) / 64;
+  static constexpr int TILE = BLOCKS * kBlock;  // bytes of a Q part, K or V tile
+  static constexpr int STAGES = D == 64 ? 8 : NQ == 3 ? 3 : 4;
+  // key tiles whose presence and scales are held: the loaders write a tile's
+  // before its softmax reads them, and, with this many, after the softmax of
+  // the tile that had the place is done (int8 loads run a tile further ahead)
+  static constexpr int META = STAGES <= 4 && !C::kInt8 ? 4 : 8;
+  static constexpr int ROWS = 128 * TILES;
+  static constexpr int SMEM = 1024 + TILES * NQ * TILE + STAGES * TILE;
+  // fp16 weights are held times 2^7, bf16 has the range without
+  static constexpr float kUp = P::kBf16 ? 1.0f : 128.0f;
+};
+
+struct Shared {
+  Cursor cur;
+  int64_t sums[kThreads / 32];
+  uint64_t full[8], empty[8];
+  uint64_t qfull[2], sfull[2], pfull[2], pvdone[2], done;
+  uint32_t tmem;
+  volatile int abort;
+  int last;
+  uint32_t there[8][4];           // keys of a tile that are loaded
+  float xmax[2][128], xsum[2][128];
+  int bad[128];
+  int64_t koff[4][128], voff[4][128];  // rows of a tile in the cache, -1: zeros
+};
+template <int N>
+struct Scales {
+  float k[N][128], v[N][128];
+};
+
+__device__ __forceinline__ void named_bar(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tie(uint32_t* r, int n) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i < n) asm volatile("" : "+r"(r[i]));
+}
+// Bits of keys key0 .. key0 + 31 that are below x.
+__device__ __forceinline__ uint32_t below(int x) {
+  return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
+}
+
+// What every role walks through: the CTA's items, in order.
+struct Walk {
+  int64_t at, end, item0, per;
+  int b, head, block;
+  Request rq;
+  Units un;
+  int u0, n, rows;  // first unit of this CTA's part of the item, units, rows
+};
+template <class F>
+__device__ __forceinline__ bool open_item(const Args& a, Walk& w) {
+  if (w.at >= w.end) return false;
+  w.rq = request(a, w.b);
+  w.un = units<kKeys, F::ROWS>(a, w.rq, w.block);
+  w.u0 = static_cast<int>(w.at - w.item0);
+  w.n = static_cast<int>(min(static_cast<int64_t>(w.un.n), w.end - w.item0)) - w.u0;
+  w.rows = min(F::ROWS, w.rq.n * a.group - w.block * F::ROWS);
+  return true;
+}
+template <class F>
+__device__ __forceinline__ void close_item(const Args& a, Walk& w) {
+  w.at += w.n;
+  if (w.u0 + w.n == w.un.n) {
+    w.item0 += w.un.n;
+    next_item<F::ROWS>(a, w.b, w.head, w.block);
+  }
+}
+__device__ __forceinline__ int key_of(const Walk& w, int i) {
+  const int u = w.u0 + i;
+  return (u < w.un.sink ? u : w.un.first + u - w.un.sink) * kKeys;
+}
+
+// ------------------------------------------------------------- loaders
+
+template <class F>
+__device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
+                                          Scales<F::META>* scales, uint8_t* ring) {
+  using C = typename F::C;
+  constexpr int ES = C::kInt8 ? 1 : 2;
+  constexpr int CH = C::kInt8 ? 16 : 8;       // elements per load
+  constexpr int CPR = F::D / CH;              // loads per row (int8: 4, 6, 8; 16-bit: 8, 12, 16)
+  constexpr int LPR = C::kInt8 ? 8 : 8;       // lanes that share a row
+  constexpr int RPP = kLoadThreads / LPR;     // rows per pass
+  constexpr int RPT = kKeys / RPP;            // rows per thread
+  const int t = threadIdx.x - kSoftThreads;
+  const int sub = t % LPR, row0 = t / LPR;
+  int64_t seq = 0;   // tiles put so far: stage and phase
+  int64_t tile = 0;  // key tiles so far, over all items: meta slot
+
+  // where tile i's rows are; its scales and presence for the softmax
+  auto locate = [&](int i, int64_t slot) {
+    const int j = key_of(w, i) + t;
+    const bool want = j <= w.un.hi && (j >= w.un.lo || j < a.sinks);
+    int page = -1, off = 0;
+    if (want) {
+      page = page_of(a, w.b, j);
+      off = j % a.page_size;
+    }
+    const bool on = page >= 0;
+    const int m = static_cast<int>(slot % 4);
+    sh.koff[m][t] = on ? page * a.k.page + off * a.k.token + w.head * a.k.head : -1;
+    sh.voff[m][t] = on ? page * a.v.page + off * a.v.token + w.head * a.v.head : -1;
+    const int mm = static_cast<int>(slot % F::META);
+    const uint32_t bits = __ballot_sync(0xffffffffu, on);
+    if ((t & 31) == 0) sh.there[mm][t >> 5] = bits;
+    if constexpr (C::kInt8) {
+      scales->k[mm][t] =
+          on ? __ldg(a.k.scales + page * a.k.spage + off * a.k.stoken + w.head * a.k.shead) : 0.0f;
+      scales->v[mm][t] =
+          on ? __ldg(a.v.scales + page * a.v.spage + off * a.v.stoken + w.head * a.v.shead) : 0.0f;
+    }
+    named_bar(3, kLoadThreads);
+  };
+
+  if constexpr (!C::kInt8) {
+    int64_t told = 0;  // tiles whose arrival has been signalled
+    auto tell = [&] {
+      fence_async();
+      mbar_arrive(&sh.full[told % F::STAGES]);
+      ++told;
+    };
+    auto put = [&](const Pool& pool, const int64_t* offs) {
+      const int s = static_cast<int>(seq % F::STAGES);
+      if (seq >= F::STAGES) {
+        const uint32_t ph = static_cast<uint32_t>(seq / F::STAGES - 1) & 1;
+        if (!mbar_try_wait(&sh.empty[s], ph)) {
+          // no room yet: what is on its way must not wait for it
+          if (told < seq) {
+            cp_wait<0>();
+            tell();
+          }
+          mbar_wait(&sh.empty[s], ph, &sh.abort);
+        }
+      }
+      const uint32_t dst = saddr(ring + s * F::TILE);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int r = row0 + i * RPP;
+        const int64_t off = offs[r];
+        const uint8_t* src = pool.data + (off < 0 ? 0 : off * ES);
+#pragma unroll
+        for (int c = 0; c < (CPR + LPR - 1) / LPR; ++c)
+          if (c * LPR + sub < CPR)
+            cp16(dst + c * kBlock + r * 128 + ((sub ^ (r & 7)) << 4), src + (c * LPR + sub) * 16,
+                 off >= 0);
+      }
+      cp_commit();
+      ++seq;
+      if (told + 1 < seq) {
+        cp_wait<1>();
+        tell();
+      }
+    };
+    while (open_item<F>(a, w)) {
+      if (F::TILES == 2) {
+        for (int i = 0; i < w.n; ++i) {
+          locate(i, tile + i);
+          put(a.k, sh.koff[(tile + i) % 4]);
+          put(a.v, sh.voff[(tile + i) % 4]);
+        }
+      } else {
+        locate(0, tile);
+        put(a.k, sh.koff[tile % 4]);
+        for (int i = 0; i < w.n; ++i) {
+          if (i + 1 < w.n) {
+            locate(i + 1, tile + i + 1);
+            put(a.k, sh.koff[(tile + i + 1) % 4]);
+          }
+          put(a.v, sh.voff[(tile + i) % 4]);
+        }
+      }
+      tile += w.n;
+      close_item<F>(a, w);
+    }
+    if (told < seq) {
+      cp_wait<0>();
+      tell();
+    }
+  } else {
+    uint4 bk[RPT], bv[RPT];
+    auto get = [&](uint4* buf, const Pool& pool, const int64_t* offs) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int64_t off = offs[row0 + i * RPP];
+        buf[i] = off >= 0 && sub < CPR
+                     ? __ldg(reinterpret_cast<const uint4*>(pool.data + off) + sub)
+                     : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    auto put = [&](const uint4* buf, auto type) {
+      using T = decltype(type);
+      const int s = static_cast<int>(seq % F::STAGES);
+      if (seq >= F::STAGES)
+        mbar_wait(&sh.empty[s], static_cast<uint32_t>(seq / F::STAGES - 1) & 1, &sh.abort);
+      uint8_t* dst = ring + s * F::TILE + (sub >> 2) * kBlock;
+      if (sub < CPR) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const int r = row0 + i * RPP;
+          const uint32_t w4[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if constexpr (T::kBf16) {
+              o[2 * x] = codes_bf16(w4[x], 0x4140u);
+              o[2 * x + 1] = codes_bf16(w4[x], 0x4342u);
+            } else {
+              o[2 * x] = codes_f16(w4[x] ^ 0x80808080u, 0x4140u);
+              o[2 * x + 1] = codes_f16(w4[x] ^ 0x80808080u, 0x4342u);
+            }
+          }
+          uint8_t* p = dst + r * 128;
+          const int c = (sub & 3) * 2;
+          *reinterpret_cast<uint4*>(p + ((c ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(p + (((c + 1) ^ (r & 7)) << 4)) =
+              make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      fence_async();
+      mbar_arrive(&sh.full[s]);
+      ++seq;
+    };
+    // after a tile is put, the next one of its kind is on its way
+    while (open_item<F>(a, w)) {
+      locate(0, tile);
+      get(bk, a.k, sh.koff[tile % 4]);
+      get(bv, a.v, sh.voff[tile % 4]);
+      auto put_k = [&](int i) {
+        put(bk, typename F::Q{});
+        if (i + 1 < w.n) {
+          locate(i + 1, tile + i + 1);
+          get(bk, a.k, sh.koff[(tile + i + 1) % 4]);
+        }
+      };
+      auto put_v = [&](int i) {
+        put(bv, typename F::P{});
+        if (i + 1 < w.n) get(bv, a.v, sh.voff[(tile + i + 1) % 4]);
+      };
+      if (F::TILES == 2) {
+        for (int i = 0; i < w.n; ++i) {
+          put_k(i);
+          put_v(i);
+        }
+      } else {
+        put_k(0);
+        for (int i = 0; i < w.n; ++i) {
+          if (i + 1 < w.n) put_k(i + 1);
+          put_v(i);
+        }
+      }
+      tile += w.n;
+      close_item<F>(a, w);
+    }
+  }
+}
+
+// ------------------------------------------------------------ products
+
+// Tensor memory columns: S (and P) of tile or buffer x, O of tile x, third
+// parts of the weights of buffer x.
+__device__ __forceinline__ uint32_t s_col(int x) { return 128u * x; }
+__device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
+__device__ __forceinline__ uint32_t p3_col(int x) { return 384u + 64u * x; }
+
+template <class F>
+__device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, const uint8_t* qs,
+                                         const uint8_t* ring) {
+  constexpr uint32_t id_qk = idesc_f16(F::Q::kBf16, false, 128, kKeys);
+  constexpr uint32_t id_pv = idesc_f16(F::P::kBf16, true, 128, F::D);
+  const uint32_t tm = sh.tmem;
+  int64_t seq = 0;
+  uint32_t nq[2] = {0, 0};  // items so far, per tile
+  uint32_t np[2] = {0, 0};  // weights taken so far, per tile or buffer
+  int64_t nb = 0;           // one row tile: key tiles so far
+
+  auto wait_tile = [&]() -> const uint8_t* {
+    const int s = static_cast<int>(seq % F::STAGES);
+    mbar_wait(&sh.full[s], static_cast<uint32_t>(seq / F::STAGES) & 1, &sh.abort);
+    fence_after();
+    return ring + s * F::TILE;
+  };
+  auto free_tile = [&] { mma_commit(&sh.empty[seq++ % F::STAGES]); };
+  // a descriptor's address field counts 16 bytes: an offset is an add
+  auto qk = [&](int tile, int x, const uint8_t* k) {
+    const uint64_t kd = sw128_desc(k);
+    for (int p = 0; p < F::NQ; ++p) {
+      const uint64_t qd = sw128_desc(qs + (tile * F::NQ + p) * F::TILE);
+#pragma unroll
+      for (int s = 0; s < F::D / 16; ++s) {
+        const int o = ((s / 4) * kBlock + (s % 4) * 32) >> 4;
+        mma_f16(tm + s_col(x), qd + o, kd + o, id_qk, p + s > 0);
+      }
+    }
+    mma_commit(&sh.sfull[x]);
+  };
+  auto pv = [&](int tile, int x, const uint8_t* v, bool first) {
+    mbar_wait(&sh.pfull[x], np[x]++ & 1, &sh.abort);
+    fence_after();
+    const uint64_t vd = sw128_mn_desc(v, kBlock);
+    for (int p = 0; p < F::NP; ++p) {
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s) {
+        const uint32_t col = p < 2 ? s_col(x) + 32 * (s / 2) + 8 * (s % 2) + 16 * p
+                                   : p3_col(x) + 8 * s;
+        mma_f16_ta(tm + o_col(tile), tm + col, vd + s * (2048 >> 4), id_pv, !first || p + s > 0);
+      }
+    }
+    mma_commit(&sh.pvdone[x]);
+  };
+
+  while (open_item<F>(a, w)) {
+    const int nt = F::TILES == 2 && w.rows > 128 ? 2 : 1;
+    for (int t = 0; t < nt; ++t) mbar_wait(&sh.qfull[t], nq[t]++ & 1, &sh.abort);
+    if (F::TILES == 2) {
+      const uint8_t* k = wait_tile();
+      for (int t = 0; t < nt; ++t) qk(t, t, k);
+      free_tile();
+      for (int i = 0; i < w.n; ++i) {
+        const uint8_t* v = wait_tile();
+        const int vs = static_cast<int>(seq++ % F::STAGES);
+        const bool more = i + 1 < w.n;
+        for (int t = 0; t < nt; ++t) {
+          pv(t, t, v, i == 0);
+          if (t == nt - 1) mma_commit(&sh.empty[vs]);
+          if (more) {
+            if (t == 0) k = wait_tile();
+            qk(t, t, k);
+            if (t == nt - 1) free_tile();
+          }
+        }
+      }
+    } else {
+      qk(0, static_cast<int>(nb & 1), wait_tile());
+      free_tile();
+      for (int i = 0; i < w.n; ++i, ++nb) {
+        if (i + 1 < w.n) {
+          qk(0, static_cast<int>(nb + 1 & 1), wait_tile());
+          free_tile();
+        }
+        pv(0, static_cast<int>(nb & 1), wait_tile(), i == 0);
+        free_tile();
+      }
+    }
+    close_item<F>(a, w);
+  }
+  mma_commit(&sh.done);  // nothing of ours runs when tensor memory is freed
+  mbar_wait(&sh.done, 0, &sh.abort);
+}
+
+// ------------------------------------------------------------- softmax
+
+// Query row (request, row r of the item) into its parts in shared memory;
+// returns the factor from a score to the exponent of 2.
+template <class F>
+__device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r, bool ok, int row,
+                                            int c0, int c1, uint8_t* q) {
+  const int rr = w.block * F::ROWS + r;
+  const int64_t q0 = ok ? static_cast<int64_t>(w.rq.start + rr / a.group) * a.q_token +
+                              (w.head * a.group + rr % a.group) * a.q_head
+                        : 0;
+  auto eight = [&](int c, float* x) {  // elements 8c .. 8c + 7
+    if (!ok) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    } else if (a.q_vec && a.q_type == LP_F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + q0) + 2 * c;
+      const float4 u = __ldg(p), v = __ldg(p + 1);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+      x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else if (a.q_vec) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + q0) + c);
+      const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = a.q_type == LP_F16 ? low16<CF16>(h[i]) : low16<CBF16>(h[i]);
+        x[2 * i + 1] = a.q_type == LP_F16 ? high16<CF16>(h[i]) : high16<CBF16>(h[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = load_elem(a.q, a.q_type, q0 + 8 * c + i);
+    }
+  };
+  // fp16 operands from other types: a power of two per row (see attn_rows.cu)
+  float f = 1.0f, back = 1.0f;
+  if (!F::Q::kBf16 && a.q_type != LP_F16) {
+    float amax = 0.0f;
+    for (int c = 0; c < F::D / 8; ++c) {
+      float x[8];
+      eight(c, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    }
+    const int e = row_exponent(amax);
+    f = pow2(14 - e);
+    back = pow2(e - 14);
+  }
+  // a negative scale goes into the queries, so that larger scores have larger weights
+  if (a.scale_log2 < 0.0f) f = -f;
+  for (int c = c0; c < c1; ++c) {
+    float x[8];
+    eight(c, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= f;
+    uint8_t* dst = q + (c / 8) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+#pragma unroll
+    for (int p = 0; p < F::NQ; ++p) {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = pack16<typename F::Q>(x[2 * i], x[2 * i + 1]);
+        x[2 * i] -= low16<typename F::Q>(o[i]);
+        x[2 * i + 1] -= high16<typename F::Q>(o[i]);
+      }
+      *reinterpret_cast<uint4*>(dst + p * F::TILE) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  return fabsf(a.scale_log2) * back;
+}
+
+template <class F>
+__device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
+                                          const Scales<F::META>* scales, uint8_t* qs) {
+  using C = typename F::C;
+  using P = typename F::P;
+  constexpr int D = F::D;
+  constexpr bool kTwo = F::TILES == 2;
+  constexpr int COLS = kTwo ? 128 : 64;  // keys of a tile that this thread takes
+  const int wg = threadIdx.x >> 7, row = threadIdx.x & 127;
+  const int warp = threadIdx.x >> 5;
+  const int tile = kTwo ? wg : 0;
+  const int col0 = kTwo ? 0 : wg * 64;
+  const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+  const uint32_t tm = sh.tmem + lanes;
+  // output columns of this thread (D = 96 halves into 64 and 32)
+  const int d0 = kTwo ? 0 : wg * (D == 64 ? 32 : 64);
+  const int d1 = kTwo ? D : (wg ? D : D == 64 ? 32 : 64);
+  int64_t tiles = 0;  // key tiles so far, over all items: meta slot, S buffer
+  uint32_t ns = 0, npv = 0;
+
+  while (open_item<F>(a, w)) {
+    const bool live = !kTwo || tile == 0 || w.rows > 128;  // warpgroup uniform
+    const int r = tile * 128 + row;
+    const bool ok = r < w.rows;
+    float c = 0.0f;
+    if (live) {
+      constexpr int half = (D / 8 + 1) / 2;
+      c = load_query<F>(a, w, r, ok, row, kTwo || wg == 0 ? 0 : half,
+                        kTwo || wg == 1 ? D / 8 : half, qs + tile * F::NQ * F::TILE);
+      fence_async();
+      mbar_arrive(&sh.qfull[tile]);
+    }
+
+    const int rr = w.block * F::ROWS + r;
+    const int pos = ok ? w.rq.base + rr / a.group : -1;
+    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+    // the warp's rows: all of them see keys from lo_w up to pos_w
+    const int r0 = tile * 128 + (warp & 3) * 32;
+    const int pos_w = w.rq.base + (w.block * F::ROWS + r0) / a.group;
+    const int last_w = w.rq.base + (w.block * F::ROWS + min(r0 + 31, w.rows - 1)) / a.group;
+    const int lo_w = a.window > 0 ? last_w - a.window + 1 : 0;
+    const float grow = c > 0.0f ? kLazy / c : INFINITY;
+
+    float m = -INFINITY, l = 0.0f;  // reference (in scores) and sum
+    // The product with the weights of key tile `slot`.  A barrier must not be
+    // waited for two phases early: with one row tile the weights run two
+    // products ahead, so each S buffer has its own barrier.
+    auto wait_pv = [&](int64_t slot) {
+      if (kTwo) mbar_wait(&sh.pvdone[tile], (npv - 1) & 1, &sh.abort);
+      else mbar_wait(&sh.pvdone[slot & 1], static_cast<uint32_t>(slot >> 1) & 1, &sh.abort);
+      fence_after();
+    };
+    if (live) {
+      for (int i = 0; i < w.n; ++i) {
+        const int key0 = key_of(w, i) + col0;
+        const int64_t slot = tiles + i;
+        const int x = kTwo ? tile : static_cast<int>(slot & 1);
+        const int mm = static_cast<int>(slot % F::META);
+        const uint32_t sc = tm + s_col(x) + col0;
+        if (kTwo) mbar_wait(&sh.sfull[x], ns++ & 1, &sh.abort);
+        else mbar_wait(&sh.sfull[x], static_cast<uint32_t>(slot >> 1) & 1, &sh.abort);
+        fence_after();
+        uint32_t see[COLS / 32];
+        bool full = key0 + COLS - 1 <= pos_w && (key0 >= lo_w || key0 + COLS <= a.sinks);
+#pragma unroll
+        for (int h = 0; h < COLS / 32; ++h) {
+          see[h] = sh.there[mm][col0 / 32 + h];
+          full = full && see[h] == 0xffffffffu;
+        }
+        if (!full) {
+#pragma unroll
+          for (int h = 0; h < COLS / 32; ++h) {
+            const int k = key0 + 32 * h;
+            see[h] &= below(pos + 1 - k) & (~below(lo - k) | below(a.sinks - k));
+          }
+        }
+        const float* sk = C::kInt8 ? &scales->k[mm][col0] : nullptr;
+        const float* sv = C::kInt8 ? &scales->v[mm][col0] : nullptr;
+
+        // ---- the row's maximum
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < COLS / 32; ++h) {
+          uint32_t v[32];
+          tmem_ld32(sc + 32 * h, v);
+          tmem_wait_ld();
+          tie(v, 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float s = __uint_as_float(v[e]);
+            if constexpr (C::kInt8) s *= sk[32 * h + e];
+            if (!full) s = see[h] >> e & 1u ? s : -INFINITY;
+            mx = fmaxf(mx, s);
+          }
+        }
+        if constexpr (!kTwo) {
+          sh.xmax[wg][row] = mx;
+          named_bar(2, kSoftThreads);
+          mx = fmaxf(mx, sh.xmax[1 - wg][row]);
+          named_bar(2, kSoftThreads);
+        }
+        // ---- a new reference, and what there is in its units
+        const bool move = mx > m + grow || (m == -INFINITY && mx != -INFINITY);
+        if (i == 0) {
+          m = mx;
+        } else if (__any_sync(0xffffffffu, move)) {
+          const float corr = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - mx) * c);
+          wait_pv(slot - 1);
+          for (int d = d0; d < d1; d += 32) {
+            uint32_t v[32];
+            tmem_ld32(tm + o_col(tile) + d, v);
+            tmem_wait_ld();
+            tie(v, 32);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
+            tmem_st32(tm + o_col(tile) + d, v);
+          }
+          tmem_wait_st();
+          l *= corr;
+          if (move) m = mx;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        // ---- weights
+#pragma unroll
+        for (int h = 0; h < COLS / 32; ++h) {
+          uint32_t v[32];
+          tmem_ld32(sc + 32 * h, v);
+          tmem_wait_ld();
+          tie(v, 32);
+          uint32_t p[F::NP][16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int k = 2 * e + z;
+              float s = __uint_as_float(v[k]);
+              if constexpr (C::kInt8) s *= sk[32 * h + k];
+              float g = ex2(fmaf(s, c, -mc));
+              if (!full) g = see[h] >> k & 1u ? g : 0.0f;
+              l += g;
+              if constexpr (C::kInt8) g = g == 0.0f ? 0.0f : g * sv[32 * h + k];
+              y[z] = g * F::kUp;
+            }
+#pragma unroll
+            for (int q = 0; q < F::NP; ++q) {
+              p[q][e] = pack16<P>(y[0], y[1]);
+              if (q + 1 < F::NP) {
+                y[0] -= low16<P>(p[q][e]);
+                y[1] -= high16<P>(p[q][e]);
+              }
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < F::NP; ++q) {
+            const uint32_t to = q < 2 ? sc + 32 * h + 16 * q : tm + p3_col(x) + (col0 / 2) + 16 * h;
+            tmem_st16(to, p[q]);
+          }
+        }
+        tmem_wait_st();
+        fence_before();
+        mbar_arrive(&sh.pfull[x]);
+        ++npv;
+      }
+      wait_pv(tiles + w.n - 1);
+    }
+    tiles += w.n;
+    if constexpr (!kTwo) {  // both halves' sums
+      sh.xsum[wg][row] = l;
+      named_bar(2, kSoftThreads);
+      l += sh.xsum[1 - wg][row];
+      named_bar(2, kSoftThreads);
+    }
+    // from here on the reference in units of log2; sums carry kUp like O
+    m = m == -INFINITY ? -INFINITY : m * c;
+
+    // ---- an item of several CTAs: leave the partial, the last one joins
+    bool final = true;
+    const Sharers ss = sharers(w.item0, w.un.n, w.per);
+    constexpr int64_t kSlot = static_cast<int64_t>(F::ROWS) * (D + 2);
+    if (ss.last > ss.first) {
+      float* mine = a.partials + slot_of(blockIdx.x, w.item0, w.per) * kSlot;
+      if (live) {
+        for (int d = d0; d < d1; d += 32) {
+          uint32_t v[32];
+          tmem_ld32(tm + o_col(tile) + d, v);
+          tmem_wait_ld();
+          tie(v, 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mine[(d + e) * F::ROWS + r] = __uint_as_float(v[e]);
+        }
+        if (d0 == 0) {
+          mine[D * F::ROWS + r] = m;
+          mine[(D + 1) * F::ROWS + r] = l;
+        }
+      }
+      __threadfence();
+      named_bar(2, kSoftThreads);
+      if (threadIdx.x == 0) {
+        const uint32_t n = static_cast<uint32_t>(ss.last - ss.first);
+        sh.last = atomicInc(a.counters + ss.first, n) == n;
+        __threadfence();
+      }
+      named_bar(2, kSoftThreads);
+      final = sh.last != 0;
+    }
+    if (final) {
+      const bool joined = ss.last > ss.first;
+      float inv = 0.0f, ref = 0.0f;
+      bool good = true;
+      if (live) {
+        if (joined) {
+          m = -INFINITY, l = 0.0f;
+          for (int k = ss.first; k <= ss.last; ++k) {
+            const float* o = a.partials + slot_of(k, w.item0, w.per) * kSlot;
+            m = fmaxf(m, __ldcg(o + D * F::ROWS + r));
+          }
+          ref = m == -INFINITY ? 0.0f : m;
+          for (int k = ss.first; k <= ss.last; ++k) {
+            const float* o = a.partials + slot_of(k, w.item0, w.per) * kSlot;
+            l = fmaf(__ldcg(o + (D + 1) * F::ROWS + r), ex2(__ldcg(o + D * F::ROWS + r) - ref), l);
+          }
+        }
+        good = finite(l);
+      }
+      const int t = rr / a.group, g = rr % a.group;
+      const int qh = w.head * a.group + g;
+      const int64_t orow = static_cast<int64_t>(w.rq.start + t) * a.o_token + qh * a.o_head;
+      // two passes over the columns: is the row finite, then write it
+      auto column_block = [&](int d, float* v) {
+        if (!joined) {
+          uint32_t u[32];
+          tmem_ld32(tm + o_col(tile) + d, u);
+          tmem_wait_ld();
+          tie(u, 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+          for (int k = ss.first; k <= ss.last; ++k) {
+            const float* o = a.partials + slot_of(k, w.item0, w.per) * kSlot;
+            const float f = ex2(__ldcg(o + D * F::ROWS + r) - ref);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = fmaf(__ldcg(o + (d + e) * F::ROWS + r), f, v[e]);
+          }
+        }
+      };
+      if (live) {
+        inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f / F::kUp, l);
+        for (int d = d0; d < d1; d += 32) {
+          float v[32];
+          column_block(d, v);
+          float s = 0.0f;  // not finite if one of them is not
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s = fmaf(v[e], 0.0f, s);
+          good = good && s == 0.0f;
+          if (ok) {
+            if (a.q_vec && a.q_type == LP_F32) {
+              float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + orow + d);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                p[e] = make_float4(v[4 * e] * inv, v[4 * e + 1] * inv, v[4 * e + 2] * inv,
+                                   v[4 * e + 3] * inv);
+            } else if (a.q_vec) {
+              uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + orow + d);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t h[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  const float y0 = v[8 * e + 2 * z] * inv, y1 = v[8 * e + 2 * z + 1] * inv;
+                  h[z] = a.q_type == LP_F16 ? pack16<CF16>(y0, y1) : pack16<CBF16>(y0, y1);
+                }
+                p[e] = make_uint4(h[0], h[1], h[2], h[3]);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) store_elem(a.out, a.q_type, orow + d + e, v[e] * inv);
+            }
+          }
+        }
+        if (ok && d0 == 0 && a.lse)
+          a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
+              l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      }
+      if constexpr (!kTwo) {  // one answer for the row's two halves; its stores are done
+        if (wg == 1) sh.bad[row] = !good;
+        __threadfence_block();
+        named_bar(2, kSoftThreads);
+        if (wg == 0) good = good && !sh.bad[row];
+        else good = true;
+      }
+      __syncwarp();
+      uint32_t again = __ballot_sync(0xffffffffu, live && ok && !good);
+      while (again) {
+        const int x = __ffs(again) - 1;
+        again &= again - 1;
+        const int row_x = w.block * F::ROWS + tile * 128 + (warp & 3) * 32 + x;
+        exact_row<C, D>(a, w.b, w.head, row_x / a.group, row_x % a.group);
+      }
+      __syncwarp();
+    }
+    if constexpr (!kTwo) named_bar(2, kSoftThreads);  // sh.bad, sh.last are free
+    fence_before();
+    close_item<F>(a, w);
+  }
+}
+
+template <class F>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ Shared sh;
+  __shared__ std::conditional_t<F::C::kInt8, Scales<F::META>, int> scale_mem;
+  Scales<F::META>* scales = reinterpret_cast<Scales<F::META>*>(&scale_mem);
+  uint8_t* qs = smem_raw + ((1024u - (saddr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* ring = qs + F::TILES * F::NQ * F::TILE;
+  const int warp = threadIdx.x >> 5;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F::STAGES; ++s) {
+      mbar_init(&sh.full[s], kLoadThreads);
+      mbar_init(&sh.empty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sh.qfull[x], F::TILES == 2 ? 128 : kSoftThreads);
+      mbar_init(&sh.sfull[x], 1);
+      mbar_init(&sh.pfull[x], F::TILES == 2 ? 128 : kSoftThreads);
+      mbar_init(&sh.pvdone[x], 1);
+    }
+    mbar_init(&sh.done, 1);
+    sh.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) tmem_alloc(&sh.tmem, 512);
+  find_share<kKeys, F::ROWS, kThreads>(a, kMinUnits, &sh.cur, sh.sums);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  Walk w;
+  w.at = sh.cur.begin;
+  w.end = sh.cur.end;
+  w.item0 = sh.cur.item0;
+  w.per = sh.cur.per_cta;
+  w.b = sh.cur.b;
+  w.head = sh.cur.head;
+  w.block = sh.cur.block;
+  // a wait that runs out sets sh.abort; the roles then run to their ends
+  // without waiting, so no barrier is left short and tensor memory is freed
+  if (w.at < w.end) {
+    // 128 registers a thread at launch: 2 x 176 + 112 + 48 = 4 x 128
+    if (warp < 8) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+      soft_role<F>(a, w, sh, scales, qs);
+    } else if (warp < 12) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+      load_role<F>(a, w, sh, scales, ring);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      if (threadIdx.x == 384) mma_role<F>(a, w, sh, qs, ring);
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    fence_after();
+    tmem_dealloc(sh.tmem, 512);
+  }
+}
+
+template <class F>
+int launch(const Args& a, cudaStream_t st) {
+  const DeviceInfo& di = device_info();
+  static int attr_set[kMaxDevices];
+  const int slot = di.ordinal % kMaxDevices;
+  if (!attr_set[slot]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_attn_chunk<F>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+    if (e != cudaSuccess) return cuda_status(e);
+    attr_set[slot] = 1;
+  }
+  k_attn_chunk<F><<<di.sm_count, kThreads, F::SMEM, st>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+template <class C, class Q, class P, int NQ, int NP, int TILES>
+int launch_dim(const Args& a, int dim, cudaStream_t st) {
+  switch (dim) {
+    case 64: return launch<Cfg<C, Q, P, NQ, NP, TILES, 64>>(a, st);
+    case 96: return launch<Cfg<C, Q, P, NQ, NP, TILES, 96>>(a, st);
+    case 128: return launch<Cfg<C, Q, P, NQ, NP, TILES, 128>>(a, st);
+    default: return LP_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace
+
+// Parts by what the result's type needs (its rounding is the largest error
+// that is allowed to show): fp32 about 22 bits of queries and weights, fp16
+// 11, bf16 8.  An int8 cache's weights carry the value scales, whose range
+// over a row's keys fp16 does not span: bf16.
+int launch_attn_chunk(const attn::Args& a, int cache_type, int dim, cudaStream_t st) {
+  const bool f32 = a.q_type == LP_F32, f16 = a.q_type == LP_F16;
+  if (cache_type == LP_F16)  // a bf16 query is exact in scaled fp16
+    return f32 ? launch_dim<CF16, CF16, CF16, 2, 2, 1>(a, dim, st)
+               : launch_dim<CF16, CF16, CF16, 1, 1, 2>(a, dim, st);
+  if (cache_type == LP_BF16)
+    return f32   ? launch_dim<CBF16, CBF16, CBF16, 3, 3, 1>(a, dim, st)
+           : f16 ? launch_dim<CBF16, CBF16, CBF16, 2, 2, 1>(a, dim, st)
+                 : launch_dim<CBF16, CBF16, CBF16, 1, 1, 2>(a, dim, st);
+  return f32   ? launch_dim<CI8, CF16, CBF16, 2, 3, 1>(a, dim, st)
+         : f16 ? launch_dim<CI8, CF16, CBF16, 1, 2, 1>(a, dim, st)
+               : launch_dim<CI8, CBF16, CBF16, 1, 1, 2>(a, dim, st);
+}
+
+unsigned int take_error_attn_chunk() {
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v)) != cudaSuccess) return LP_ERR_CUDA;
+  if (v) {
+    const unsigned int z = 0;
+    cudaMemcpyToSymbol(g_device_error, &z, sizeof(z));
+  }
+  return v;
+}
+
+}  // namespace lp

@@ -155,6 +155,8 @@ int lp_device_error(void) {
   if (!e) e = e2;
   if (!e) e = e3;
   if (!e) e = e4;
+  const unsigned int e5 = lp::take_error_attn_chunk();
+  if (!e) e = e5;
   return static_cast<int>(e);
 }
 

@@ -10,8 +10,10 @@ namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
 constexpr int64_t kCounterBytes = 4096;  // one 4-byte counter per CTA of a launch
-constexpr int64_t kSlotRows = 8;         // rows of a partial result
+constexpr int64_t kSlotRows = 256;       // most rows of a partial result
 constexpr int64_t kSlotDim = 128;
+// Mean query rows per request and key head from which the chunk kernel is used.
+constexpr int64_t kChunkRows = 32;
 
 #define LP_REQUIRE(cond)              \
   do {                                \
@@ -178,7 +180,10 @@ int lp_paged_attention(const lp_kv_cache* cache, const int32_t* block_tables, in
   a.scale_log2 = scale * 1.4426950408889634f;
   a.counters = static_cast<uint32_t*>(workspace);
   a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-  return lp::launch_attn_rows(a, cache->dtype, cache->head_dim, S(stream));
+  // mean rows per request and key head; a tile of the chunk kernel has 128 or 256
+  const bool chunk = q->tokens * a.group >= kChunkRows * n;
+  return chunk ? lp::launch_attn_chunk(a, cache->dtype, cache->head_dim, S(stream))
+               : lp::launch_attn_rows(a, cache->dtype, cache->head_dim, S(stream));
 }
 
 }  // extern "C"

@@ -131,7 +131,8 @@ int launch_gemm_nvf4(const uint8_t* w, const uint8_t* ws, const float* gw, const
                      const uint8_t* xs, const float* gx, int64_t n, float* y, int64_t m, int64_t k,
                      cudaStream_t st);
 
-// paged cache (kvcache.cu) and its attention (attn_rows.cu)
+// paged cache (kvcache.cu) and its attention (attn_rows.cu: few rows,
+// attn_chunk.cu: tcgen05)
 int launch_assign_pages(const int32_t* ctx, const int32_t* add, int64_t requests,
                         int64_t page_size, const int32_t* free_pages, int64_t free_len,
                         const int32_t* free_head, int32_t* table, int64_t table_stride,
@@ -146,12 +147,14 @@ namespace attn {
 struct Args;
 }
 int launch_attn_rows(const attn::Args& a, int cache_type, int dim, cudaStream_t st);
+int launch_attn_chunk(const attn::Args& a, int cache_type, int dim, cudaStream_t st);
 
 // error words of the translation units whose kernels wait (read + clear)
 unsigned int take_error_gemv();
 unsigned int take_error_gemm_tc();
 unsigned int take_error_pool();
 unsigned int take_error_gemm_fp4();
+unsigned int take_error_attn_chunk();
 
 // While on (this thread only), the lp_* entry points run their shape and
 // argument checks and return without launching anything (capi.cu).
