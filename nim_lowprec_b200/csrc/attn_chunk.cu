@@ -84,7 +84,7 @@ struct Shared {
   int64_t koff[4][128], voff[4][128];  // rows of a tile in the cache, -1: zeros
 };
 template <int N>
-struct Scales {
+struct __align__(16) Scales {
   float k[N][128], v[N][128];
 };
 
@@ -145,6 +145,15 @@ __device__ __forceinline__ int key_of(const Walk& w, int i) {
   return (u < w.un.sink ? u : w.un.first + u - w.un.sink) * kKeys;
 }
 
+// Where a role is in the ring of key and value tiles.
+template <int STAGES>
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) stage = 0, phase ^= 1;
+  }
+};
+
 // ------------------------------------------------------------- loaders
 
 template <class F>
@@ -159,23 +168,26 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
   constexpr int RPT = kKeys / RPP;            // rows per thread
   const int t = threadIdx.x - kSoftThreads;
   const int sub = t % LPR, row0 = t / LPR;
-  int64_t seq = 0;   // tiles put so far: stage and phase
-  int64_t tile = 0;  // key tiles so far, over all items: meta slot
+  Ring<F::STAGES> at;   // the next tile to put
+  bool lap = false;     // the ring has been filled once
+  uint32_t tile = 0;    // key tiles so far, over all items: meta slot
 
-  // where tile i's rows are; its scales and presence for the softmax
-  auto locate = [&](int i, int64_t slot) {
+  // The page of key t of the item's tile i: looked up a tile ahead.
+  int next_page = -1;
+  auto look = [&](int i) {
     const int j = key_of(w, i) + t;
-    const bool want = j <= w.un.hi && (j >= w.un.lo || j < a.sinks);
-    int page = -1, off = 0;
-    if (want) {
-      page = page_of(a, w.b, j);
-      off = j % a.page_size;
-    }
+    next_page = j <= w.un.hi && (j >= w.un.lo || j < a.sinks) ? page_of(a, w.b, j) : -1;
+  };
+  // where tile i's rows are; its scales and presence for the softmax
+  auto locate = [&](int i, uint32_t slot) {
+    const int page = next_page;
+    if (i + 1 < w.n) look(i + 1);
     const bool on = page >= 0;
-    const int m = static_cast<int>(slot % 4);
+    const int off = on ? (key_of(w, i) + t) % a.page_size : 0;
+    const int m = slot % 4;
     sh.koff[m][t] = on ? page * a.k.page + off * a.k.token + w.head * a.k.head : -1;
     sh.voff[m][t] = on ? page * a.v.page + off * a.v.token + w.head * a.v.head : -1;
-    const int mm = static_cast<int>(slot % F::META);
+    const int mm = slot % F::META;
     const uint32_t bits = __ballot_sync(0xffffffffu, on);
     if ((t & 31) == 0) sh.there[mm][t >> 5] = bits;
     if constexpr (C::kInt8) {
@@ -188,26 +200,22 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
   };
 
   if constexpr (!C::kInt8) {
-    int64_t told = 0;  // tiles whose arrival has been signalled
+    Ring<F::STAGES> told;   // the next tile to signal
+    int untold = 0;
     auto tell = [&] {
       fence_async();
-      mbar_arrive(&sh.full[told % F::STAGES]);
-      ++told;
+      mbar_arrive(&sh.full[told.stage]);
+      told.next();
+      --untold;
     };
     auto put = [&](const Pool& pool, const int64_t* offs) {
-      const int s = static_cast<int>(seq % F::STAGES);
-      if (seq >= F::STAGES) {
-        const uint32_t ph = static_cast<uint32_t>(seq / F::STAGES - 1) & 1;
-        if (!mbar_try_wait(&sh.empty[s], ph)) {
-          // no room yet: what is on its way must not wait for it
-          if (told < seq) {
-            cp_wait<0>();
-            tell();
-          }
-          mbar_wait(&sh.empty[s], ph, &sh.abort);
-        }
+      if (lap && !mbar_try_wait(&sh.empty[at.stage], at.phase ^ 1)) {
+        // no room yet: what is on its way must not wait for it
+        cp_wait<0>();
+        while (untold) tell();
+        mbar_wait(&sh.empty[at.stage], at.phase ^ 1, &sh.abort);
       }
-      const uint32_t dst = saddr(ring + s * F::TILE);
+      const uint32_t dst = saddr(ring + at.stage * F::TILE);
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         const int r = row0 + i * RPP;
@@ -220,13 +228,15 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
                  off >= 0);
       }
       cp_commit();
-      ++seq;
-      if (told + 1 < seq) {
-        cp_wait<1>();
+      at.next();
+      lap = lap || at.stage == 0;
+      if (++untold > 2) {  // three tiles in flight
+        cp_wait<2>();
         tell();
       }
     };
     while (open_item<F>(a, w)) {
+      look(0);
       if (F::TILES == 2) {
         for (int i = 0; i < w.n; ++i) {
           locate(i, tile + i);
@@ -247,10 +257,8 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
       tile += w.n;
       close_item<F>(a, w);
     }
-    if (told < seq) {
-      cp_wait<0>();
-      tell();
-    }
+    cp_wait<0>();
+    while (untold) tell();
   } else {
     uint4 bk[RPT], bv[RPT];
     auto get = [&](uint4* buf, const Pool& pool, const int64_t* offs) {
@@ -264,10 +272,8 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
     };
     auto put = [&](const uint4* buf, auto type) {
       using T = decltype(type);
-      const int s = static_cast<int>(seq % F::STAGES);
-      if (seq >= F::STAGES)
-        mbar_wait(&sh.empty[s], static_cast<uint32_t>(seq / F::STAGES - 1) & 1, &sh.abort);
-      uint8_t* dst = ring + s * F::TILE + (sub >> 2) * kBlock;
+      if (lap) mbar_wait(&sh.empty[at.stage], at.phase ^ 1, &sh.abort);
+      uint8_t* dst = ring + at.stage * F::TILE + (sub >> 2) * kBlock;
       if (sub < CPR) {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
@@ -292,11 +298,13 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
         }
       }
       fence_async();
-      mbar_arrive(&sh.full[s]);
-      ++seq;
+      mbar_arrive(&sh.full[at.stage]);
+      at.next();
+      lap = lap || at.stage == 0;
     };
     // after a tile is put, the next one of its kind is on its way
     while (open_item<F>(a, w)) {
+      look(0);
       locate(0, tile);
       get(bk, a.k, sh.koff[tile % 4]);
       get(bv, a.v, sh.voff[tile % 4]);
@@ -343,24 +351,26 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
   constexpr uint32_t id_qk = idesc_f16(F::Q::kBf16, false, 128, kKeys);
   constexpr uint32_t id_pv = idesc_f16(F::P::kBf16, true, 128, F::D);
   const uint32_t tm = sh.tmem;
-  int64_t seq = 0;
+  Ring<F::STAGES> at;
   uint32_t nq[2] = {0, 0};  // items so far, per tile
   uint32_t np[2] = {0, 0};  // weights taken so far, per tile or buffer
-  int64_t nb = 0;           // one row tile: key tiles so far
+  uint32_t nb = 0;          // one row tile: key tiles so far
 
   auto wait_tile = [&]() -> const uint8_t* {
-    const int s = static_cast<int>(seq % F::STAGES);
-    mbar_wait(&sh.full[s], static_cast<uint32_t>(seq / F::STAGES) & 1, &sh.abort);
+    mbar_wait(&sh.full[at.stage], at.phase, &sh.abort);
     fence_after();
-    return ring + s * F::TILE;
+    return ring + at.stage * F::TILE;
   };
-  auto free_tile = [&] { mma_commit(&sh.empty[seq++ % F::STAGES]); };
+  auto free_tile = [&] {
+    mma_commit(&sh.empty[at.stage]);
+    at.next();
+  };
   // a descriptor's address field counts 16 bytes: an offset is an add
   auto qk = [&](int tile, int x, const uint8_t* k) {
     const uint64_t kd = sw128_desc(k);
     for (int p = 0; p < F::NQ; ++p) {
       const uint64_t qd = sw128_desc(qs + (tile * F::NQ + p) * F::TILE);
-#pragma unroll
+#pragma unroll 4
       for (int s = 0; s < F::D / 16; ++s) {
         const int o = ((s / 4) * kBlock + (s % 4) * 32) >> 4;
         mma_f16(tm + s_col(x), qd + o, kd + o, id_qk, p + s > 0);
@@ -373,7 +383,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
     fence_after();
     const uint64_t vd = sw128_mn_desc(v, kBlock);
     for (int p = 0; p < F::NP; ++p) {
-#pragma unroll
+#pragma unroll 4
       for (int s = 0; s < kKeys / 16; ++s) {
         const uint32_t col = p < 2 ? s_col(x) + 32 * (s / 2) + 8 * (s % 2) + 16 * p
                                    : p3_col(x) + 8 * s;
@@ -392,7 +402,8 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
       free_tile();
       for (int i = 0; i < w.n; ++i) {
         const uint8_t* v = wait_tile();
-        const int vs = static_cast<int>(seq++ % F::STAGES);
+        const uint32_t vs = at.stage;
+        at.next();
         const bool more = i + 1 < w.n;
         for (int t = 0; t < nt; ++t) {
           pv(t, t, v, i == 0);
@@ -489,7 +500,8 @@ __device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r,
       *reinterpret_cast<uint4*>(dst + p * F::TILE) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
-  return fabsf(a.scale_log2) * back;
+  // (never 0: a masked score of -inf stays one)
+  return fmaxf(fabsf(a.scale_log2) * back, 1e-36f);
 }
 
 template <class F>
@@ -509,7 +521,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
   // output columns of this thread (D = 96 halves into 64 and 32)
   const int d0 = kTwo ? 0 : wg * (D == 64 ? 32 : 64);
   const int d1 = kTwo ? D : (wg ? D : D == 64 ? 32 : 64);
-  int64_t tiles = 0;  // key tiles so far, over all items: meta slot, S buffer
+  uint32_t tiles = 0;  // key tiles so far, over all items: meta slot, S buffer
   uint32_t ns = 0, npv = 0;
 
   while (open_item<F>(a, w)) {
@@ -533,26 +545,26 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
     const int pos_w = w.rq.base + (w.block * F::ROWS + r0) / a.group;
     const int last_w = w.rq.base + (w.block * F::ROWS + min(r0 + 31, w.rows - 1)) / a.group;
     const int lo_w = a.window > 0 ? last_w - a.window + 1 : 0;
-    const float grow = c > 0.0f ? kLazy / c : INFINITY;
+    const float grow = kLazy / c;
 
     float m = -INFINITY, l = 0.0f;  // reference (in scores) and sum
     // The product with the weights of key tile `slot`.  A barrier must not be
     // waited for two phases early: with one row tile the weights run two
     // products ahead, so each S buffer has its own barrier.
-    auto wait_pv = [&](int64_t slot) {
+    auto wait_pv = [&](uint32_t slot) {
       if (kTwo) mbar_wait(&sh.pvdone[tile], (npv - 1) & 1, &sh.abort);
-      else mbar_wait(&sh.pvdone[slot & 1], static_cast<uint32_t>(slot >> 1) & 1, &sh.abort);
+      else mbar_wait(&sh.pvdone[slot & 1], slot >> 1 & 1, &sh.abort);
       fence_after();
     };
     if (live) {
       for (int i = 0; i < w.n; ++i) {
         const int key0 = key_of(w, i) + col0;
-        const int64_t slot = tiles + i;
-        const int x = kTwo ? tile : static_cast<int>(slot & 1);
-        const int mm = static_cast<int>(slot % F::META);
+        const uint32_t slot = tiles + i;
+        const int x = kTwo ? tile : slot & 1;
+        const int mm = slot % F::META;
         const uint32_t sc = tm + s_col(x) + col0;
         if (kTwo) mbar_wait(&sh.sfull[x], ns++ & 1, &sh.abort);
-        else mbar_wait(&sh.sfull[x], static_cast<uint32_t>(slot >> 1) & 1, &sh.abort);
+        else mbar_wait(&sh.sfull[x], slot >> 1 & 1, &sh.abort);
         fence_after();
         uint32_t see[COLS / 32];
         bool full = key0 + COLS - 1 <= pos_w && (key0 >= lo_w || key0 + COLS <= a.sinks);
@@ -571,22 +583,44 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
         const float* sk = C::kInt8 ? &scales->k[mm][col0] : nullptr;
         const float* sv = C::kInt8 ? &scales->v[mm][col0] : nullptr;
 
-        // ---- the row's maximum
-        float mx = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t v[32];
-          tmem_ld32(sc + 32 * h, v);
+        // Scores 32 .. of this thread's columns: int8 keys' scales and the mask
+        // are applied on each of the two reads (registers hold 64 of 128).
+        auto ready = [&](uint32_t* v, int h) {
           tmem_wait_ld();
           tie(v, 32);
+          if constexpr (C::kInt8) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float s = __uint_as_float(v[e]);
-            if constexpr (C::kInt8) s *= sk[32 * h + e];
-            if (!full) s = see[h] >> e & 1u ? s : -INFINITY;
-            mx = fmaxf(mx, s);
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(sk + 32 * h + e);
+              v[e] = __float_as_uint(__uint_as_float(v[e]) * k4.x);
+              v[e + 1] = __float_as_uint(__uint_as_float(v[e + 1]) * k4.y);
+              v[e + 2] = __float_as_uint(__uint_as_float(v[e + 2]) * k4.z);
+              v[e + 3] = __float_as_uint(__uint_as_float(v[e + 3]) * k4.w);
+            }
+          }
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = see[h] >> e & 1u ? v[e] : 0xff800000u;
+          }
+        };
+        uint32_t va[32], vb[32];
+        // ---- the row's maximum; a chunk's read runs while the one before is used
+        float mx = -INFINITY, my = -INFINITY;
+        tmem_ld32(sc, va);
+#pragma unroll
+        for (int h = 0; h < COLS / 32; ++h) {
+          uint32_t* v = h & 1 ? vb : va;
+          ready(v, h);
+          tmem_ld32(sc + 32 * ((h + 1) % (COLS / 32)), h & 1 ? va : vb);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            mx = fmaxf(mx, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+            my = fmaxf(my, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
           }
         }
+        mx = fmaxf(mx, my);
+        tmem_wait_ld();  // the next pass's first chunk, which waits in registers
+        tie(va, 32);
         if constexpr (!kTwo) {
           sh.xmax[wg][row] = mx;
           named_bar(2, kSoftThreads);
@@ -614,34 +648,34 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
           if (move) m = mx;
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;
-        // ---- weights
+        // ---- weights (the first chunk is on its way since the last pass)
+        const uint64_t c2 = pk(c, c), mc2 = pk(-mc, -mc);
+        uint64_t la = 0, lb = 0;
 #pragma unroll
         for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t v[32];
-          tmem_ld32(sc + 32 * h, v);
-          tmem_wait_ld();
-          tie(v, 32);
+          uint32_t* v = h & 1 ? vb : va;
+          ready(v, h);
+          if (h + 1 < COLS / 32) tmem_ld32(sc + 32 * (h + 1), h & 1 ? va : vb);
           uint32_t p[F::NP][16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float y[2];
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const int k = 2 * e + z;
-              float s = __uint_as_float(v[k]);
-              if constexpr (C::kInt8) s *= sk[32 * h + k];
-              float g = ex2(fmaf(s, c, -mc));
-              if (!full) g = see[h] >> k & 1u ? g : 0.0f;
-              l += g;
-              if constexpr (C::kInt8) g = g == 0.0f ? 0.0f : g * sv[32 * h + k];
-              y[z] = g * F::kUp;
+            float y0, y1;
+            upk(fma2(pk(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, mc2), y0, y1);
+            y0 = ex2(y0), y1 = ex2(y1);
+            uint64_t& sum = e & 1 ? lb : la;
+            sum = add2(sum, pk(y0, y1));
+            if constexpr (C::kInt8) {
+              const float2 s2 = *reinterpret_cast<const float2*>(sv + 32 * h + 2 * e);
+              y0 = y0 == 0.0f ? 0.0f : y0 * s2.x;
+              y1 = y1 == 0.0f ? 0.0f : y1 * s2.y;
             }
+            if constexpr (F::kUp != 1.0f) y0 *= F::kUp, y1 *= F::kUp;
 #pragma unroll
             for (int q = 0; q < F::NP; ++q) {
-              p[q][e] = pack16<P>(y[0], y[1]);
+              p[q][e] = pack16<P>(y0, y1);
               if (q + 1 < F::NP) {
-                y[0] -= low16<P>(p[q][e]);
-                y[1] -= high16<P>(p[q][e]);
+                y0 -= low16<P>(p[q][e]);
+                y1 -= high16<P>(p[q][e]);
               }
             }
           }
@@ -650,6 +684,12 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
             const uint32_t to = q < 2 ? sc + 32 * h + 16 * q : tm + p3_col(x) + (col0 / 2) + 16 * h;
             tmem_st16(to, p[q]);
           }
+        }
+        {
+          float y[4];
+          upk(la, y[0], y[1]);
+          upk(lb, y[2], y[3]);
+          l += (y[0] + y[1]) + (y[2] + y[3]);
         }
         tmem_wait_st();
         fence_before();
@@ -805,7 +845,7 @@ template <class F>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ Shared sh;
-  __shared__ std::conditional_t<F::C::kInt8, Scales<F::META>, int> scale_mem;
+  __shared__ __align__(16) std::conditional_t<F::C::kInt8, Scales<F::META>, int> scale_mem;
   Scales<F::META>* scales = reinterpret_cast<Scales<F::META>*>(&scale_mem);
   uint8_t* qs = smem_raw + ((1024u - (saddr(smem_raw) & 1023u)) & 1023u);
   uint8_t* ring = qs + F::TILES * F::NQ * F::TILE;
@@ -842,15 +882,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
   // a wait that runs out sets sh.abort; the roles then run to their ends
   // without waiting, so no barrier is left short and tensor memory is freed
   if (w.at < w.end) {
-    // 128 registers a thread at launch: 2 x 176 + 112 + 48 = 4 x 128
+    // 128 registers a thread at launch: 2 x 176 + 104 + 56 = 4 x 128
     if (warp < 8) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
       soft_role<F>(a, w, sh, scales, qs);
     } else if (warp < 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
       load_role<F>(a, w, sh, scales, ring);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (threadIdx.x == 384) mma_role<F>(a, w, sh, qs, ring);
     }
   }
