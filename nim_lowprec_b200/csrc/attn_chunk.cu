@@ -15,7 +15,7 @@
 //                   zeros, whatever the cache holds there.  fp16 and bf16
 //                   pages go by cp.async; int8 codes through registers, where
 //                   they are widened (exactly) to the operand type.
-//   warp 12         one lane issues the products: tcgen05.mma kind::f16,
+//   warp 12         issues the products: tcgen05.mma kind::f16,
 //                   M = 128, S and O in tensor memory, P from tensor memory
 //                   (it takes the columns of the S it came from).
 // While one tile's softmax runs, the tensor cores work on the other tile, or,
@@ -79,7 +79,7 @@ struct Shared {
   volatile int abort;
   int last;
   uint32_t there[8][4];           // keys of a tile that are loaded
-  float xmax[2][128], xsum[2][128];
+  float xmax[2][2][128], xsum[2][128];
   int bad[128];
   int64_t koff[4][128], voff[4][128];  // rows of a tile in the cache, -1: zeros
 };
@@ -345,91 +345,117 @@ __device__ __forceinline__ uint32_t s_col(int x) { return 128u * x; }
 __device__ __forceinline__ uint32_t o_col(int x) { return 256u + 128u * x; }
 __device__ __forceinline__ uint32_t p3_col(int x) { return 384u + 64u * x; }
 
+// One lane of a converged warp, the same one every time.  The warp stays
+// together around it, so descriptors and addresses live in uniform registers:
+// a lone thread's products each waited about 120 cycles for theirs to be moved
+// there, twice what the product takes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred P; elect.sync _|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 template <class F>
 __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, const uint8_t* qs,
                                          const uint8_t* ring) {
   constexpr uint32_t id_qk = idesc_f16(F::Q::kBf16, false, 128, kKeys);
   constexpr uint32_t id_pv = idesc_f16(F::P::kBf16, true, 128, F::D);
-  const uint32_t tm = sh.tmem;
+  const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(sh.tmem)));
+  const uint64_t q_desc = sw128_desc(qs), k_desc = sw128_desc(ring);
+  const uint64_t v_desc = sw128_mn_desc(ring, kBlock);
   Ring<F::STAGES> at;
   uint32_t nq[2] = {0, 0};  // items so far, per tile
   uint32_t np[2] = {0, 0};  // weights taken so far, per tile or buffer
   uint32_t nb = 0;          // one row tile: key tiles so far
 
-  auto wait_tile = [&]() -> const uint8_t* {
+  auto wait_tile = [&] {
     mbar_wait(&sh.full[at.stage], at.phase, &sh.abort);
+    __syncwarp();
     fence_after();
-    return ring + at.stage * F::TILE;
-  };
-  auto free_tile = [&] {
-    mma_commit(&sh.empty[at.stage]);
-    at.next();
   };
   // a descriptor's address field counts 16 bytes: an offset is an add
-  auto qk = [&](int tile, int x, const uint8_t* k) {
-    const uint64_t kd = sw128_desc(k);
-    for (int p = 0; p < F::NQ; ++p) {
-      const uint64_t qd = sw128_desc(qs + (tile * F::NQ + p) * F::TILE);
-#pragma unroll 4
-      for (int s = 0; s < F::D / 16; ++s) {
-        const int o = ((s / 4) * kBlock + (s % 4) * 32) >> 4;
-        mma_f16(tm + s_col(x), qd + o, kd + o, id_qk, p + s > 0);
+  auto qk = [&](int tile, int x, uint32_t stage, bool last) {
+    if (elect_one()) {
+      const uint64_t kd = k_desc + stage * (F::TILE >> 4);
+#pragma unroll
+      for (int p = 0; p < F::NQ; ++p) {
+        const uint64_t qd = q_desc + (tile * F::NQ + p) * (F::TILE >> 4);
+#pragma unroll
+        for (int s = 0; s < F::D / 16; ++s) {
+          const int o = ((s / 4) * kBlock + (s % 4) * 32) >> 4;
+          mma_f16(tm + s_col(x), qd + o, kd + o, id_qk, p + s > 0);
+        }
       }
+      mma_commit(&sh.sfull[x]);
+      if (last) mma_commit(&sh.empty[stage]);
     }
-    mma_commit(&sh.sfull[x]);
+    __syncwarp();
   };
-  auto pv = [&](int tile, int x, const uint8_t* v, bool first) {
+  auto pv = [&](int tile, int x, uint32_t stage, bool first, bool last) {
     mbar_wait(&sh.pfull[x], np[x]++ & 1, &sh.abort);
+    __syncwarp();
     fence_after();
-    const uint64_t vd = sw128_mn_desc(v, kBlock);
-    for (int p = 0; p < F::NP; ++p) {
-#pragma unroll 4
-      for (int s = 0; s < kKeys / 16; ++s) {
-        const uint32_t col = p < 2 ? s_col(x) + 32 * (s / 2) + 8 * (s % 2) + 16 * p
-                                   : p3_col(x) + 8 * s;
-        mma_f16_ta(tm + o_col(tile), tm + col, vd + s * (2048 >> 4), id_pv, !first || p + s > 0);
-      }
+    if (elect_one()) {
+      const uint64_t vd = v_desc + stage * (F::TILE >> 4);
+#pragma unroll
+      for (int p = 0; p < F::NP; ++p)
+#pragma unroll
+        for (int s = 0; s < kKeys / 16; ++s) {
+          const uint32_t col = p < 2 ? s_col(x) + 32 * (s / 2) + 8 * (s % 2) + 16 * p
+                                     : p3_col(x) + 8 * s;
+          mma_f16_ta(tm + o_col(tile), tm + col, vd + s * (2048 >> 4), id_pv, !first || p + s > 0);
+        }
+      mma_commit(&sh.pvdone[x]);
+      if (last) mma_commit(&sh.empty[stage]);
     }
-    mma_commit(&sh.pvdone[x]);
+    __syncwarp();
   };
 
-  while (open_item<F>(a, w)) {
-    const int nt = F::TILES == 2 && w.rows > 128 ? 2 : 1;
+  while (uniform(open_item<F>(a, w))) {
+    const int n = uniform(w.n);
+    const int nt = F::TILES == 2 && uniform(w.rows) > 128 ? 2 : 1;
     for (int t = 0; t < nt; ++t) mbar_wait(&sh.qfull[t], nq[t]++ & 1, &sh.abort);
-    if (F::TILES == 2) {
-      const uint8_t* k = wait_tile();
-      for (int t = 0; t < nt; ++t) qk(t, t, k);
-      free_tile();
-      for (int i = 0; i < w.n; ++i) {
-        const uint8_t* v = wait_tile();
+    __syncwarp();
+    if constexpr (F::TILES == 2) {
+      wait_tile();
+      qk(0, 0, at.stage, nt == 1);
+      if (nt == 2) qk(1, 1, at.stage, true);
+      at.next();
+      for (int i = 0; i < n; ++i) {
+        wait_tile();
         const uint32_t vs = at.stage;
         at.next();
-        const bool more = i + 1 < w.n;
-        for (int t = 0; t < nt; ++t) {
-          pv(t, t, v, i == 0);
-          if (t == nt - 1) mma_commit(&sh.empty[vs]);
-          if (more) {
-            if (t == 0) k = wait_tile();
-            qk(t, t, k);
-            if (t == nt - 1) free_tile();
-          }
+        const bool more = i + 1 < n;
+        pv(0, 0, vs, i == 0, nt == 1);
+        if (more) {
+          wait_tile();
+          qk(0, 0, at.stage, nt == 1);
         }
+        if (nt == 2) {
+          pv(1, 1, vs, i == 0, true);
+          if (more) qk(1, 1, at.stage, true);
+        }
+        if (more) at.next();
       }
     } else {
-      qk(0, static_cast<int>(nb & 1), wait_tile());
-      free_tile();
-      for (int i = 0; i < w.n; ++i, ++nb) {
-        if (i + 1 < w.n) {
-          qk(0, static_cast<int>(nb + 1 & 1), wait_tile());
-          free_tile();
+      wait_tile();
+      qk(0, nb & 1, at.stage, true);
+      at.next();
+      for (int i = 0; i < n; ++i, ++nb) {
+        if (i + 1 < n) {
+          wait_tile();
+          qk(0, nb + 1 & 1, at.stage, true);
+          at.next();
         }
-        pv(0, static_cast<int>(nb & 1), wait_tile(), i == 0);
-        free_tile();
+        wait_tile();
+        pv(0, nb & 1, at.stage, i == 0, true);
+        at.next();
       }
     }
     close_item<F>(a, w);
   }
-  mma_commit(&sh.done);  // nothing of ours runs when tensor memory is freed
+  if (elect_one()) mma_commit(&sh.done);  // nothing of ours runs when tensor memory is freed
   mbar_wait(&sh.done, 0, &sh.abort);
 }
 
@@ -466,15 +492,23 @@ __device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r,
       for (int i = 0; i < 8; ++i) x[i] = load_elem(a.q, a.q_type, q0 + 8 * c + i);
     }
   };
+  // Loads of 64 elements are in flight together: a row is far from the next
+  // one, so each costs a trip to L2.
+  constexpr int B = 8;
   // fp16 operands from other types: a power of two per row (see attn_rows.cu)
   float f = 1.0f, back = 1.0f;
   if (!F::Q::kBf16 && a.q_type != LP_F16) {
     float amax = 0.0f;
-    for (int c = 0; c < F::D / 8; ++c) {
-      float x[8];
-      eight(c, x);
+    for (int c = 0; c < F::D / 8; c += B) {
+      float x[B][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+      for (int b = 0; b < B; ++b)
+        if (c + b < F::D / 8) eight(c + b, x[b]);
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + b < F::D / 8) amax = fmaxf(amax, fabsf(x[b][i]));
     }
     const int e = row_exponent(amax);
     f = pow2(14 - e);
@@ -482,22 +516,29 @@ __device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r,
   }
   // a negative scale goes into the queries, so that larger scores have larger weights
   if (a.scale_log2 < 0.0f) f = -f;
-  for (int c = c0; c < c1; ++c) {
-    float x[8];
-    eight(c, x);
+  for (int c = c0; c < c1; c += B) {
+    float xs[B][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= f;
-    uint8_t* dst = q + (c / 8) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+    for (int b = 0; b < B; ++b)
+      if (c + b < c1) eight(c + b, xs[b]);
 #pragma unroll
-    for (int p = 0; p < F::NQ; ++p) {
-      uint32_t o[4];
+    for (int b = 0; b < B; ++b) {
+      if (c + b >= c1) break;
+      float* x = xs[b];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i] = pack16<typename F::Q>(x[2 * i], x[2 * i + 1]);
-        x[2 * i] -= low16<typename F::Q>(o[i]);
-        x[2 * i + 1] -= high16<typename F::Q>(o[i]);
+      for (int i = 0; i < 8; ++i) x[i] *= f;
+      uint8_t* dst = q + ((c + b) / 8) * kBlock + row * 128 + ((((c + b) & 7) ^ (row & 7)) << 4);
+#pragma unroll
+      for (int p = 0; p < F::NQ; ++p) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = pack16<typename F::Q>(x[2 * i], x[2 * i + 1]);
+          x[2 * i] -= low16<typename F::Q>(o[i]);
+          x[2 * i + 1] -= high16<typename F::Q>(o[i]);
+        }
+        *reinterpret_cast<uint4*>(dst + p * F::TILE) = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      *reinterpret_cast<uint4*>(dst + p * F::TILE) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
   // (never 0: a masked score of -inf stays one)
@@ -622,10 +663,9 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
         tmem_wait_ld();  // the next pass's first chunk, which waits in registers
         tie(va, 32);
         if constexpr (!kTwo) {
-          sh.xmax[wg][row] = mx;
+          sh.xmax[x][wg][row] = mx;  // (the buffer's last readers are two barriers back)
           named_bar(2, kSoftThreads);
-          mx = fmaxf(mx, sh.xmax[1 - wg][row]);
-          named_bar(2, kSoftThreads);
+          mx = fmaxf(mx, sh.xmax[x][1 - wg][row]);
         }
         // ---- a new reference, and what there is in its units
         const bool move = mx > m + grow || (m == -INFINITY && mx != -INFINITY);
@@ -891,7 +931,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
       load_role<F>(a, w, sh, scales, ring);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      if (threadIdx.x == 384) mma_role<F>(a, w, sh, qs, ring);
+      if (warp == 12) mma_role<F>(a, w, sh, qs, ring);
     }
   }
   __syncwarp();
