@@ -13,8 +13,9 @@
 //                   16-byte strides, and keys that no row of the tile sees
 //                   (past the end, before the window, on missing pages) are
 //                   zeros, whatever the cache holds there.  fp16 and bf16
-//                   pages go by cp.async; int8 codes through registers, where
-//                   they are widened (exactly) to the operand type.
+//                   pages go by cp.async into the ring; int8 codes by cp.async
+//                   into a small ring of their own, from where the thread that
+//                   fetched them widens them (exactly) to the operand type.
 //   warp 12         issues the products: tcgen05.mma kind::f16,
 //                   M = 128, S and O in tensor memory, P from tensor memory
 //                   (it takes the columns of the S it came from).
@@ -59,15 +60,20 @@ struct Cfg {
   static constexpr int NQ = NQ_, NP = NP_, TILES = TILES_, D = D_;
   static constexpr int BLOCKS = (D + 63) / 64;
   static constexpr int TILE = BLOCKS * kBlock;  // bytes of a Q part, K or V tile
-  static constexpr int STAGES = D == 64 ? 8 : NQ == 3 ? 3 : 4;
+  static constexpr int STAGES = C::kInt8 ? (D == 64 ? 4 : 3) : D == 64 ? 8 : NQ == 3 ? 3 : 4;
+  // int8: tiles of codes on their way, 16 bytes a lane
+  static constexpr int RAW = C::kInt8 ? 3 : 0;
+  static constexpr int LPR = C::kInt8 && D == 64 ? 4 : 8;  // loading lanes that share a row
+  static constexpr int RAW_TILE = kKeys * LPR * 16;
   // key tiles whose presence and scales are held: the loaders write a tile's
   // before its softmax reads them, and, with this many, after the softmax of
   // the tile that had the place is done (int8 loads run a tile further ahead)
-  static constexpr int META = STAGES <= 4 && !C::kInt8 ? 4 : 8;
+  static constexpr int META = C::kInt8 ? 6 : STAGES <= 4 ? 4 : 8;
   static constexpr int ROWS = 128 * TILES;
-  static constexpr int SMEM = 1024 + TILES * NQ * TILE + STAGES * TILE;
+  static constexpr int SMEM = 1024 + TILES * NQ * TILE + STAGES * TILE + RAW * RAW_TILE;
   // fp16 weights are held times 2^7, bf16 has the range without
   static constexpr float kUp = P::kBf16 ? 1.0f : 128.0f;
+  static constexpr float kUpLog = P::kBf16 ? 0.0f : 7.0f;
 };
 
 struct Shared {
@@ -81,7 +87,7 @@ struct Shared {
   uint32_t there[8][4];           // keys of a tile that are loaded
   float xmax[2][2][128], xsum[2][128];
   int bad[128];
-  int64_t koff[4][128], voff[4][128];  // rows of a tile in the cache, -1: zeros
+  int64_t koff[3][128], voff[3][128];  // rows of a tile in the cache, -1: zeros
 };
 template <int N>
 struct __align__(16) Scales {
@@ -99,10 +105,32 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
                "r"(on ? 16 : 0)
                : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0)
+               : "memory");
+}
+// Whether the phase is over, without the suspension of try_wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(saddr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint64_t pku(uint32_t a, uint32_t b) {
+  return pk(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ void upku(uint64_t r, uint32_t& a, uint32_t& b) {
+  float x, y;
+  upk(r, x, y);
+  a = __float_as_uint(x), b = __float_as_uint(y);
 }
 __device__ __forceinline__ void tie(uint32_t* r, int n) {
 #pragma unroll
@@ -158,12 +186,12 @@ struct Ring {
 
 template <class F>
 __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
-                                          Scales<F::META>* scales, uint8_t* ring) {
+                                          Scales<F::META>* scales, uint8_t* ring, uint8_t* raw) {
   using C = typename F::C;
   constexpr int ES = C::kInt8 ? 1 : 2;
   constexpr int CH = C::kInt8 ? 16 : 8;       // elements per load
   constexpr int CPR = F::D / CH;              // loads per row (int8: 4, 6, 8; 16-bit: 8, 12, 16)
-  constexpr int LPR = C::kInt8 ? 8 : 8;       // lanes that share a row
+  constexpr int LPR = F::LPR;                 // lanes that share a row
   constexpr int RPP = kLoadThreads / LPR;     // rows per pass
   constexpr int RPT = kKeys / RPP;            // rows per thread
   const int t = threadIdx.x - kSoftThreads;
@@ -184,17 +212,18 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
     if (i + 1 < w.n) look(i + 1);
     const bool on = page >= 0;
     const int off = on ? (key_of(w, i) + t) % a.page_size : 0;
-    const int m = slot % 4;
+    const int m = slot % 3;
     sh.koff[m][t] = on ? page * a.k.page + off * a.k.token + w.head * a.k.head : -1;
     sh.voff[m][t] = on ? page * a.v.page + off * a.v.token + w.head * a.v.head : -1;
     const int mm = slot % F::META;
     const uint32_t bits = __ballot_sync(0xffffffffu, on);
     if ((t & 31) == 0) sh.there[mm][t >> 5] = bits;
     if constexpr (C::kInt8) {
-      scales->k[mm][t] =
-          on ? __ldg(a.k.scales + page * a.k.spage + off * a.k.stoken + w.head * a.k.shead) : 0.0f;
-      scales->v[mm][t] =
-          on ? __ldg(a.v.scales + page * a.v.spage + off * a.v.stoken + w.head * a.v.shead) : 0.0f;
+      const int64_t p = on ? page : 0;
+      cp4(saddr(&scales->k[mm][t]),
+          a.k.scales + p * a.k.spage + off * a.k.stoken + w.head * a.k.shead, on);
+      cp4(saddr(&scales->v[mm][t]),
+          a.v.scales + p * a.v.spage + off * a.v.stoken + w.head * a.v.shead, on);
     }
     named_bar(3, kLoadThreads);
   };
@@ -209,7 +238,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
       --untold;
     };
     auto put = [&](const Pool& pool, const int64_t* offs) {
-      if (lap && !mbar_try_wait(&sh.empty[at.stage], at.phase ^ 1)) {
+      if (lap && !mbar_test(&sh.empty[at.stage], at.phase ^ 1)) {
         // no room yet: what is on its way must not wait for it
         cp_wait<0>();
         while (untold) tell();
@@ -240,18 +269,18 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
       if (F::TILES == 2) {
         for (int i = 0; i < w.n; ++i) {
           locate(i, tile + i);
-          put(a.k, sh.koff[(tile + i) % 4]);
-          put(a.v, sh.voff[(tile + i) % 4]);
+          put(a.k, sh.koff[(tile + i) % 3]);
+          put(a.v, sh.voff[(tile + i) % 3]);
         }
       } else {
         locate(0, tile);
-        put(a.k, sh.koff[tile % 4]);
+        put(a.k, sh.koff[tile % 3]);
         for (int i = 0; i < w.n; ++i) {
           if (i + 1 < w.n) {
             locate(i + 1, tile + i + 1);
-            put(a.k, sh.koff[(tile + i + 1) % 4]);
+            put(a.k, sh.koff[(tile + i + 1) % 3]);
           }
-          put(a.v, sh.voff[(tile + i) % 4]);
+          put(a.v, sh.voff[(tile + i) % 3]);
         }
       }
       tile += w.n;
@@ -260,34 +289,55 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
     cp_wait<0>();
     while (untold) tell();
   } else {
-    uint4 bk[RPT], bv[RPT];
-    auto get = [&](uint4* buf, const Pool& pool, const int64_t* offs) {
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const int64_t off = offs[row0 + i * RPP];
-        buf[i] = off >= 0 && sub < CPR
-                     ? __ldg(reinterpret_cast<const uint4*>(pool.data + off) + sub)
-                     : make_uint4(0u, 0u, 0u, 0u);
+    // The item's tiles in the order of their use, RAW of them on their way.  A
+    // thread widens the pieces that it fetched itself, so only its own copies
+    // have to have landed.
+    uint8_t* mine = raw + t * 16;
+    auto kind = [&](int q, int& i) {  // of the q-th tile: key tile i's values?
+      if (F::TILES == 2) {
+        i = q >> 1;
+        return (q & 1) != 0;
       }
+      const bool v = q == 2 * w.n - 1 || (q > 0 && (q & 1) == 0);
+      i = q == 2 * w.n - 1 ? w.n - 1 : v ? (q >> 1) - 1 : (q + 1) >> 1;
+      return v;
     };
-    auto put = [&](const uint4* buf, auto type) {
+    auto issue = [&](int q, int slot) {
+      if (q < 2 * w.n) {
+        int i;
+        const bool v = kind(q, i);
+        if (!v) locate(i, tile + i);
+        const int m = (tile + i) % 3;
+        const Pool& pool = v ? a.v : a.k;
+        const int64_t* offs = v ? sh.voff[m] : sh.koff[m];
+        const uint32_t dst = saddr(mine + slot * F::RAW_TILE);
+#pragma unroll
+        for (int x = 0; x < RPT; ++x) {
+          const int64_t off = offs[row0 + x * RPP];
+          if (sub < CPR) cp16(dst + x * (kLoadThreads * 16), pool.data + (off < 0 ? 0 : off) + sub * 16, off >= 0);
+        }
+      }
+      cp_commit();
+    };
+    auto widen = [&](auto type, int slot) {
       using T = decltype(type);
-      if (lap) mbar_wait(&sh.empty[at.stage], at.phase ^ 1, &sh.abort);
       uint8_t* dst = ring + at.stage * F::TILE + (sub >> 2) * kBlock;
       if (sub < CPR) {
 #pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const int r = row0 + i * RPP;
-          const uint32_t w4[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+        for (int x = 0; x < RPT; ++x) {
+          const int r = row0 + x * RPP;
+          const uint4 u = *reinterpret_cast<const uint4*>(mine + slot * F::RAW_TILE +
+                                                          x * (kLoadThreads * 16));
+          const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
           uint32_t o[8];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int y = 0; y < 4; ++y) {
             if constexpr (T::kBf16) {
-              o[2 * x] = codes_bf16(w4[x], 0x4140u);
-              o[2 * x + 1] = codes_bf16(w4[x], 0x4342u);
+              o[2 * y] = codes_bf16(w4[y], 0x4140u);
+              o[2 * y + 1] = codes_bf16(w4[y], 0x4342u);
             } else {
-              o[2 * x] = codes_f16(w4[x] ^ 0x80808080u, 0x4140u);
-              o[2 * x + 1] = codes_f16(w4[x] ^ 0x80808080u, 0x4342u);
+              o[2 * y] = codes_f16(w4[y] ^ 0x80808080u, 0x4140u);
+              o[2 * y + 1] = codes_f16(w4[y] ^ 0x80808080u, 0x4342u);
             }
           }
           uint8_t* p = dst + r * 128;
@@ -297,43 +347,28 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
               make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
-      fence_async();
-      mbar_arrive(&sh.full[at.stage]);
-      at.next();
-      lap = lap || at.stage == 0;
     };
-    // after a tile is put, the next one of its kind is on its way
     while (open_item<F>(a, w)) {
       look(0);
-      locate(0, tile);
-      get(bk, a.k, sh.koff[tile % 4]);
-      get(bv, a.v, sh.voff[tile % 4]);
-      auto put_k = [&](int i) {
-        put(bk, typename F::Q{});
-        if (i + 1 < w.n) {
-          locate(i + 1, tile + i + 1);
-          get(bk, a.k, sh.koff[(tile + i + 1) % 4]);
-        }
-      };
-      auto put_v = [&](int i) {
-        put(bv, typename F::P{});
-        if (i + 1 < w.n) get(bv, a.v, sh.voff[(tile + i + 1) % 4]);
-      };
-      if (F::TILES == 2) {
-        for (int i = 0; i < w.n; ++i) {
-          put_k(i);
-          put_v(i);
-        }
-      } else {
-        put_k(0);
-        for (int i = 0; i < w.n; ++i) {
-          if (i + 1 < w.n) put_k(i + 1);
-          put_v(i);
-        }
+      for (int q = 0; q < F::RAW; ++q) issue(q, q);
+      int slot = 0;
+      for (int q = 0; q < 2 * w.n; ++q) {
+        cp_wait<F::RAW - 1>();
+        if (lap) mbar_wait(&sh.empty[at.stage], at.phase ^ 1, &sh.abort);
+        int i;
+        if (kind(q, i)) widen(typename F::P{}, slot);
+        else widen(typename F::Q{}, slot);
+        fence_async();
+        mbar_arrive(&sh.full[at.stage]);
+        at.next();
+        lap = lap || at.stage == 0;
+        issue(q + F::RAW, slot);
+        slot = slot + 1 == F::RAW ? 0 : slot + 1;
       }
       tile += w.n;
       close_item<F>(a, w);
     }
+    cp_wait<0>();
   }
 }
 
@@ -632,11 +667,11 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
           if constexpr (C::kInt8) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 k4 = *reinterpret_cast<const float4*>(sk + 32 * h + e);
-              v[e] = __float_as_uint(__uint_as_float(v[e]) * k4.x);
-              v[e + 1] = __float_as_uint(__uint_as_float(v[e + 1]) * k4.y);
-              v[e + 2] = __float_as_uint(__uint_as_float(v[e + 2]) * k4.z);
-              v[e + 3] = __float_as_uint(__uint_as_float(v[e + 3]) * k4.w);
+              const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(sk + 32 * h + e);
+              const uint64_t x = mul2(pku(v[e], v[e + 1]), k4.x);
+              const uint64_t y = mul2(pku(v[e + 2], v[e + 3]), k4.y);
+              upku(x, v[e], v[e + 1]);
+              upku(y, v[e + 2], v[e + 3]);
             }
           }
           if (!full) {
@@ -688,8 +723,9 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
           if (move) m = mx;
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;
-        // ---- weights (the first chunk is on its way since the last pass)
-        const uint64_t c2 = pk(c, c), mc2 = pk(-mc, -mc);
+        // ---- weights, times kUp (the first chunk is on its way since the last pass)
+        const float up = F::NP == 1 ? F::kUpLog : 0.0f;
+        const uint64_t c2 = pk(c, c), mc2 = pk(up - mc, up - mc);
         uint64_t la = 0, lb = 0;
 #pragma unroll
         for (int h = 0; h < COLS / 32; ++h) {
@@ -700,22 +736,27 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y0, y1;
-            upk(fma2(pk(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, mc2), y0, y1);
-            y0 = ex2(y0), y1 = ex2(y1);
+            upk(fma2(pku(v[2 * e], v[2 * e + 1]), c2, mc2), y0, y1);
+            uint64_t y = pk(ex2(y0), ex2(y1));
+            // more than one part: 2^7 as a product, which rounds nothing
+            if constexpr (F::NP > 1 && F::kUp != 1.0f) y = mul2(y, pk(F::kUp, F::kUp));
             uint64_t& sum = e & 1 ? lb : la;
-            sum = add2(sum, pk(y0, y1));
-            if constexpr (C::kInt8) {
-              const float2 s2 = *reinterpret_cast<const float2*>(sv + 32 * h + 2 * e);
-              y0 = y0 == 0.0f ? 0.0f : y0 * s2.x;
-              y1 = y1 == 0.0f ? 0.0f : y1 * s2.y;
-            }
-            if constexpr (F::kUp != 1.0f) y0 *= F::kUp, y1 *= F::kUp;
+            sum = add2(sum, y);
+            if constexpr (C::kInt8)
+              y = mul2(y, *reinterpret_cast<const uint64_t*>(sv + 32 * h + 2 * e));
 #pragma unroll
             for (int q = 0; q < F::NP; ++q) {
-              p[q][e] = pack16<P>(y0, y1);
-              if (q + 1 < F::NP) {
-                y0 -= low16<P>(p[q][e]);
-                y1 -= high16<P>(p[q][e]);
+              upk(y, y0, y1);
+              if (q + 1 == F::NP) {
+                p[q][e] = pack16<P>(y0, y1);
+              } else if constexpr (P::kBf16) {
+                // a part is the upper half of what is left, which the difference keeps exactly
+                const uint32_t h0 = __float_as_uint(y0), h1 = __float_as_uint(y1);
+                p[q][e] = prmt(h0, h1, 0x7632u);
+                y = fma2(pku(h0 & 0xffff0000u, h1 & 0xffff0000u), pk(-1.0f, -1.0f), y);
+              } else {
+                p[q][e] = pack16<P>(y0, y1);
+                y = fma2(pk(low16<P>(p[q][e]), high16<P>(p[q][e])), pk(-1.0f, -1.0f), y);
               }
             }
           }
@@ -745,7 +786,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
       l += sh.xsum[1 - wg][row];
       named_bar(2, kSoftThreads);
     }
-    // from here on the reference in units of log2; sums carry kUp like O
+    // from here on the reference in units of log2 (sums carry kUp, like O)
     m = m == -INFINITY ? -INFINITY : m * c;
 
     // ---- an item of several CTAs: leave the partial, the last one joins
@@ -821,7 +862,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
         }
       };
       if (live) {
-        inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f / F::kUp, l);
+        inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         for (int d = d0; d < d1; d += 32) {
           float v[32];
           column_block(d, v);
@@ -856,7 +897,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
         }
         if (ok && d0 == 0 && a.lse)
           a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
-              l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+              l == 0.0f ? -INFINITY : (m + (log2f(l) - F::kUpLog)) * kLn2;
       }
       if constexpr (!kTwo) {  // one answer for the row's two halves; its stores are done
         if (wg == 1) sh.bad[row] = !good;
@@ -928,7 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
       soft_role<F>(a, w, sh, scales, qs);
     } else if (warp < 12) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-      load_role<F>(a, w, sh, scales, ring);
+      load_role<F>(a, w, sh, scales, ring, ring + F::STAGES * F::TILE);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (warp == 12) mma_role<F>(a, w, sh, qs, ring);
