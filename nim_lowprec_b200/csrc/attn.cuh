@@ -6,8 +6,10 @@
 // token t, query head g of the group), r = t * G + g, in blocks of RB rows.
 // A block sees a contiguous run of keys (with a window: the sinks' run and the
 // window's run), cut into units of KU keys.  All units of all (b, h, block)
-// items are laid end to end and every CTA takes one contiguous, equal share,
-// so ragged lengths, few long requests and many short ones all fill the grid.
+// items are laid end to end, behind each item XU more for what an item costs
+// beside its keys (its queries, the join of its parts, its outputs), and every
+// CTA takes one contiguous, equal share, so ragged lengths, few long requests
+// and many short ones all fill the grid.
 // An item cut by a CTA boundary leaves partial results (running maximum, sum
 // and unnormalised output, fp32) in the workspace; the CTA that arrives last
 // adds them in CTA order, so results do not depend on the timing.
@@ -94,12 +96,12 @@ __device__ __forceinline__ Units units(const Args& a, const Request& r, int bloc
   return u;
 }
 
-template <int KU, int RB>
+template <int KU, int RB, int XU>
 __device__ __forceinline__ int64_t request_units(const Args& a, int b) {
   const Request r = request(a, b);
   const int blocks = (r.n * a.group + RB - 1) / RB;
   int64_t s = 0;
-  for (int i = 0; i < blocks; ++i) s += units<KU, RB>(a, r, i).n;
+  for (int i = 0; i < blocks; ++i) s += units<KU, RB>(a, r, i).n + XU;
   return s;
 }
 
@@ -116,13 +118,13 @@ struct Cursor {
 // Total units and the item that holds unit `begin` of this CTA.  Each thread
 // sums a run of requests, the sums are scanned in shared memory, and the
 // thread whose run holds `begin` walks it.  All threads of the block call it.
-template <int KU, int RB, int THREADS>
+template <int KU, int RB, int XU, int THREADS>
 __device__ void find_share(const Args& a, int64_t min_units, Cursor* cur, int64_t* sums) {
   const int t = threadIdx.x;
   const int run = (a.requests + THREADS - 1) / THREADS;
   const int b0 = min(t * run, a.requests), b1 = min(b0 + run, a.requests);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += request_units<KU, RB>(a, b);
+  for (int b = b0; b < b1; ++b) mine += request_units<KU, RB, XU>(a, b);
   mine *= a.kv_heads;
   // inclusive scan: within the warp, then over the warps' totals
   int64_t inc = mine;
@@ -149,19 +151,19 @@ __device__ void find_share(const Args& a, int64_t min_units, Cursor* cur, int64_
   if (begin >= excl && begin < excl + mine) {
     int64_t at = excl;
     int b = b0;
-    int64_t w = request_units<KU, RB>(a, b);
+    int64_t w = request_units<KU, RB, XU>(a, b);
     while (begin >= at + w * a.kv_heads) {
       at += w * a.kv_heads;
-      w = request_units<KU, RB>(a, ++b);
+      w = request_units<KU, RB, XU>(a, ++b);
     }
     const int head = static_cast<int>((begin - at) / w);
     at += head * w;
     const Request r = request(a, b);
     int block = 0;
-    int n = units<KU, RB>(a, r, 0).n;
+    int n = units<KU, RB>(a, r, 0).n + XU;
     while (begin >= at + n) {
       at += n;
-      n = units<KU, RB>(a, r, ++block).n;
+      n = units<KU, RB>(a, r, ++block).n + XU;
     }
     cur->b = b;
     cur->head = head;
@@ -184,6 +186,48 @@ __device__ __forceinline__ void next_item(const Args& a, int& b, int& head, int&
     r = request(a, b);
   } while (r.n == 0);
 }
+
+// A role's walk through the CTA's items, in order.  open() finds the next part
+// of an item that has units of its own; close() steps behind it.
+template <int KU, int RB, int XU>
+struct Walk {
+  int64_t at, end, item0, per;
+  int b, head, block;
+  Request rq;
+  Units un;
+  int u0, n, rows;  // the part: first unit of the item's, units; rows of the item
+
+  __device__ __forceinline__ void start(const Cursor& c) {
+    at = c.begin, end = c.end, item0 = c.item0, per = c.per_cta;
+    b = c.b, head = c.head, block = c.block;
+  }
+  __device__ __forceinline__ bool open(const Args& a) {
+    while (at < end) {
+      rq = request(a, b);
+      un = units<KU, RB>(a, rq, block);
+      u0 = static_cast<int>(at - item0);
+      n = static_cast<int>(min(static_cast<int64_t>(un.n), end - item0)) - u0;
+      rows = min(RB, rq.n * a.group - block * RB);
+      if (n > 0) return true;
+      skip(a);  // the share begins behind the item's units
+    }
+    return false;
+  }
+  __device__ __forceinline__ void close(const Args& a) {
+    if (u0 + n == un.n) skip(a);
+    else at += n;
+  }
+  __device__ __forceinline__ void skip(const Args& a) {
+    item0 += un.n + XU;
+    at = item0;
+    next_item<RB>(a, b, head, block);
+  }
+  // first key of the part's i-th unit
+  __device__ __forceinline__ int key(int i) const {
+    const int u = u0 + i;
+    return (u < un.sink ? u : un.first + u - un.sink) * KU;
+  }
+};
 
 // CTAs that share an item of units [u0, u0 + n): first..last, and the slot of
 // a CTA's partial (0: its share begins inside the item or at its first unit).

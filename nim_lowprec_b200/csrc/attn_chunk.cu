@@ -49,6 +49,9 @@ constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroup
 constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
 constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
 constexpr int kMinUnits = 2;
+// What an item costs beside its keys, in key tiles: 8 us of queries, start and
+// outputs against 2 to 3 us per tile.
+constexpr int kItemUnits = 4;
 
 // C: the cache's format; Q: type of the operands of Q K^T, P: of P V;
 // NQ, NP: parts of queries and weights.
@@ -75,6 +78,9 @@ struct Cfg {
   static constexpr float kUp = P::kBf16 ? 1.0f : 128.0f;
   static constexpr float kUpLog = P::kBf16 ? 0.0f : 7.0f;
 };
+
+template <class F>
+using WalkOf = Walk<kKeys, F::ROWS, kItemUnits>;
 
 struct Shared {
   Cursor cur;
@@ -142,37 +148,6 @@ __device__ __forceinline__ uint32_t below(int x) {
   return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
 }
 
-// What every role walks through: the CTA's items, in order.
-struct Walk {
-  int64_t at, end, item0, per;
-  int b, head, block;
-  Request rq;
-  Units un;
-  int u0, n, rows;  // first unit of this CTA's part of the item, units, rows
-};
-template <class F>
-__device__ __forceinline__ bool open_item(const Args& a, Walk& w) {
-  if (w.at >= w.end) return false;
-  w.rq = request(a, w.b);
-  w.un = units<kKeys, F::ROWS>(a, w.rq, w.block);
-  w.u0 = static_cast<int>(w.at - w.item0);
-  w.n = static_cast<int>(min(static_cast<int64_t>(w.un.n), w.end - w.item0)) - w.u0;
-  w.rows = min(F::ROWS, w.rq.n * a.group - w.block * F::ROWS);
-  return true;
-}
-template <class F>
-__device__ __forceinline__ void close_item(const Args& a, Walk& w) {
-  w.at += w.n;
-  if (w.u0 + w.n == w.un.n) {
-    w.item0 += w.un.n;
-    next_item<F::ROWS>(a, w.b, w.head, w.block);
-  }
-}
-__device__ __forceinline__ int key_of(const Walk& w, int i) {
-  const int u = w.u0 + i;
-  return (u < w.un.sink ? u : w.un.first + u - w.un.sink) * kKeys;
-}
-
 // Where a role is in the ring of key and value tiles.
 template <int STAGES>
 struct Ring {
@@ -185,7 +160,7 @@ struct Ring {
 // ------------------------------------------------------------- loaders
 
 template <class F>
-__device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
+__device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh,
                                           Scales<F::META>* scales, uint8_t* ring, uint8_t* raw) {
   using C = typename F::C;
   constexpr int ES = C::kInt8 ? 1 : 2;
@@ -203,7 +178,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
   // The page of key t of the item's tile i: looked up a tile ahead.
   int next_page = -1;
   auto look = [&](int i) {
-    const int j = key_of(w, i) + t;
+    const int j = w.key(i) + t;
     next_page = j <= w.un.hi && (j >= w.un.lo || j < a.sinks) ? page_of(a, w.b, j) : -1;
   };
   // where tile i's rows are; its scales and presence for the softmax
@@ -211,7 +186,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
     const int page = next_page;
     if (i + 1 < w.n) look(i + 1);
     const bool on = page >= 0;
-    const int off = on ? (key_of(w, i) + t) % a.page_size : 0;
+    const int off = on ? (w.key(i) + t) % a.page_size : 0;
     const int m = slot % 3;
     sh.koff[m][t] = on ? page * a.k.page + off * a.k.token + w.head * a.k.head : -1;
     sh.voff[m][t] = on ? page * a.v.page + off * a.v.token + w.head * a.v.head : -1;
@@ -264,7 +239,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
         tell();
       }
     };
-    while (open_item<F>(a, w)) {
+    while (w.open(a)) {
       look(0);
       if (F::TILES == 2) {
         for (int i = 0; i < w.n; ++i) {
@@ -284,7 +259,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
         }
       }
       tile += w.n;
-      close_item<F>(a, w);
+      w.close(a);
     }
     cp_wait<0>();
     while (untold) tell();
@@ -341,14 +316,17 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
             }
           }
           uint8_t* p = dst + r * 128;
-          const int c = (sub & 3) * 2;
-          *reinterpret_cast<uint4*>(p + ((c ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(p + (((c + 1) ^ (r & 7)) << 4)) =
-              make_uint4(o[4], o[5], o[6], o[7]);
+          // lanes of the two column blocks write their halves in opposite order:
+          // eight lanes then meet in no bank
+          const bool odd = sub >> 2 & 1;
+          const int c = ((sub & 3) * 2 + odd) ^ (r & 7);
+          const uint4 h0 = make_uint4(o[0], o[1], o[2], o[3]), h1 = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(p + (c << 4)) = odd ? h1 : h0;
+          *reinterpret_cast<uint4*>(p + ((c ^ 1) << 4)) = odd ? h0 : h1;
         }
       }
     };
-    while (open_item<F>(a, w)) {
+    while (w.open(a)) {
       look(0);
       for (int q = 0; q < F::RAW; ++q) issue(q, q);
       int slot = 0;
@@ -366,7 +344,7 @@ __device__ __forceinline__ void load_role(const Args& a, Walk w, Shared& sh,
         slot = slot + 1 == F::RAW ? 0 : slot + 1;
       }
       tile += w.n;
-      close_item<F>(a, w);
+      w.close(a);
     }
     cp_wait<0>();
   }
@@ -392,7 +370,7 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 template <class F>
-__device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, const uint8_t* qs,
+__device__ __forceinline__ void mma_role(const Args& a, WalkOf<F> w, Shared& sh, const uint8_t* qs,
                                          const uint8_t* ring) {
   constexpr uint32_t id_qk = idesc_f16(F::Q::kBf16, false, 128, kKeys);
   constexpr uint32_t id_pv = idesc_f16(F::P::kBf16, true, 128, F::D);
@@ -447,7 +425,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
     __syncwarp();
   };
 
-  while (uniform(open_item<F>(a, w))) {
+  while (uniform(w.open(a))) {
     const int n = uniform(w.n);
     const int nt = F::TILES == 2 && uniform(w.rows) > 128 ? 2 : 1;
     for (int t = 0; t < nt; ++t) mbar_wait(&sh.qfull[t], nq[t]++ & 1, &sh.abort);
@@ -488,7 +466,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
         at.next();
       }
     }
-    close_item<F>(a, w);
+    w.close(a);
   }
   if (elect_one()) mma_commit(&sh.done);  // nothing of ours runs when tensor memory is freed
   mbar_wait(&sh.done, 0, &sh.abort);
@@ -499,7 +477,7 @@ __device__ __forceinline__ void mma_role(const Args& a, Walk w, Shared& sh, cons
 // Query row (request, row r of the item) into its parts in shared memory;
 // returns the factor from a score to the exponent of 2.
 template <class F>
-__device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r, bool ok, int row,
+__device__ __forceinline__ float load_query(const Args& a, const WalkOf<F>& w, int r, bool ok, int row,
                                             int c0, int c1, uint8_t* q) {
   const int rr = w.block * F::ROWS + r;
   const int64_t q0 = ok ? static_cast<int64_t>(w.rq.start + rr / a.group) * a.q_token +
@@ -581,7 +559,7 @@ __device__ __forceinline__ float load_query(const Args& a, const Walk& w, int r,
 }
 
 template <class F>
-__device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
+__device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh,
                                           const Scales<F::META>* scales, uint8_t* qs) {
   using C = typename F::C;
   using P = typename F::P;
@@ -600,7 +578,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
   uint32_t tiles = 0;  // key tiles so far, over all items: meta slot, S buffer
   uint32_t ns = 0, npv = 0;
 
-  while (open_item<F>(a, w)) {
+  while (w.open(a)) {
     const bool live = !kTwo || tile == 0 || w.rows > 128;  // warpgroup uniform
     const int r = tile * 128 + row;
     const bool ok = r < w.rows;
@@ -634,7 +612,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
     };
     if (live) {
       for (int i = 0; i < w.n; ++i) {
-        const int key0 = key_of(w, i) + col0;
+        const int key0 = w.key(i) + col0;
         const uint32_t slot = tiles + i;
         const int x = kTwo ? tile : slot & 1;
         const int mm = slot % F::META;
@@ -918,7 +896,7 @@ __device__ __forceinline__ void soft_role(const Args& a, Walk w, Shared& sh,
     }
     if constexpr (!kTwo) named_bar(2, kSoftThreads);  // sh.bad, sh.last are free
     fence_before();
-    close_item<F>(a, w);
+    w.close(a);
   }
 }
 
@@ -948,18 +926,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
     mbar_fence_init();
   }
   if (warp == 12) tmem_alloc(&sh.tmem, 512);
-  find_share<kKeys, F::ROWS, kThreads>(a, kMinUnits, &sh.cur, sh.sums);
+  find_share<kKeys, F::ROWS, kItemUnits, kThreads>(a, kMinUnits, &sh.cur, sh.sums);
   fence_before();
   __syncthreads();
   fence_after();
-  Walk w;
-  w.at = sh.cur.begin;
-  w.end = sh.cur.end;
-  w.item0 = sh.cur.item0;
-  w.per = sh.cur.per_cta;
-  w.b = sh.cur.b;
-  w.head = sh.cur.head;
-  w.block = sh.cur.block;
+  WalkOf<F> w;
+  w.start(sh.cur);
   // a wait that runs out sets sh.abort; the roles then run to their ends
   // without waiting, so no barrier is left short and tensor memory is freed
   if (w.at < w.end) {

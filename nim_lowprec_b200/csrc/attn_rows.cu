@@ -1,29 +1,27 @@
 // attn_rows.cu -- attention of a few query rows over a paged cache: single
-// new tokens (decode), and every case that the chunk kernel does not take.
+// new tokens (decode), and chunks too short for a tile of the chunk kernel.
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max),  j visible
 //
 // One pass over the keys with a running maximum and sum per row.  What bounds
-// it is the cache's bytes, so the whole design serves the loads:
+// it is the cache's bytes, so the design serves the loads:
 //   * A CTA takes up to 8 query rows of one key head (all query heads of the
-//     group), so keys and values are read once for the group.
-//   * Each of its 8 warps takes steps of 16 keys (32 of an int8 cache) and
-//     holds keys and values in registers only: a lane's 16-byte loads are
-//     already the B fragments of m16n8k16 products, for keys with the head
-//     dimension permuted (the queries are permuted alike), for values after
-//     byte permutes that pair two keys.  No shared memory, no barrier and no
-//     shuffle stands between a load and its use; the next step's keys are in
-//     flight while this step's products run.
-//   * The products use 16 rows where there are 8 queries; the other 8 rows
-//     carry what 16 bits drop: row i the query's high part, row i + 8 the
-//     rest (hi + lo is 22 bits of fp16, 16 of bf16), and likewise for the
-//     weights p.  Both parts of a row meet in the same thread.  fp32 results
-//     with bf16 operands take a second product for a third part (24 bits).
-//     fp16 parts are scaled: queries by a power of two per row, queries and
-//     weights to at most 2^14, second parts by 2^12 more (which the row's
-//     other accumulator takes back).  So they neither overflow nor fall under
-//     the type's smallest numbers: weights of 2^-29 of the row's largest keep
-//     22 bits.
+//     group), so keys and values are read once for the group.  Two CTAs of
+//     four warps share an SM: one joins its rows while the other streams.
+//   * Each warp streams for itself: steps of 16 to 32 keys (keys and values,
+//     8 KB) go by cp.async into its own ring of 24 KB, two to five steps ahead
+//     of their use, across item boundaries.  No barrier stands between a load
+//     and its use, and a step's pages may lie anywhere.
+//   * The products are m16n8k16 with 16 rows where there are 8 queries; the
+//     other 8 rows carry what 16 bits drop: row i the query's high part, row
+//     i + 8 the rest (hi + lo is 22 bits of fp16, 16 of bf16), and likewise
+//     for the weights p.  Both parts of a row meet in the same thread.  fp32
+//     results with bf16 operands take a second product for a third part (24
+//     bits).  fp16 parts are scaled: queries by a power of two per row,
+//     queries and weights to at most 2^14, second parts by 2^12 more (which
+//     the row's other accumulator takes back).  So they neither overflow nor
+//     fall under the type's smallest numbers: weights of 2^-29 of the row's
+//     largest keep 22 bits.
 //   * An int8 cache's scales are per (token, head): a key's multiplies its
 //     score, a value's its weight, so the codes go into the products exactly.
 //   * The tensor cores serve here to keep the arithmetic (8 rows: 16 fma per
@@ -36,14 +34,15 @@ namespace {
 
 using namespace attn;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;
 constexpr int kUnit = 32;  // keys per unit: a warp's share of a round
 // A CTA takes at least this many units: fewer would cost more in the join of
 // the partial results than the spread over more SMs gives back.
 constexpr int kMinUnits = 4;
-constexpr int kTop = 14;  // queries and weights are below 2^kTop in 16 bits
+constexpr int kItemUnits = 8;  // what an item costs beside its keys, in units
+constexpr int kTop = 14;       // queries and weights are below 2^kTop in 16 bits
 // fp16: second parts, at most 2^(kTop - 11), are held times 2^kLow
 constexpr int kLow = 12;
 
@@ -58,73 +57,109 @@ struct ValueType<CI8> { using T = CBF16; };
 
 template <class C, int D>
 struct Shape {
-  static constexpr int KS = C::kInt8 ? 32 : 16;           // keys per step
-  static constexpr int NG = KS / 8;                       // n8 groups of keys
-  static constexpr int E = C::kInt8 && D % 64 == 0 ? 16 : 8;  // elements per key load and lane
-  static constexpr int LW = E * (C::kInt8 ? 1 : 2) / 4;   // words per key load
-  static constexpr int KL = D / (4 * E);                  // key loads
-  static constexpr int KW = KL * LW;                      // words per key and lane
-  static constexpr int KV = KS / 4;                       // values per lane and step
-  static constexpr int VE = D / 8;                        // elements per value and lane
-  static constexpr int VW = VE * (C::kInt8 ? 1 : 2) / 4;
-  static constexpr int STEPS = D / 16;                    // k16 steps of a score
-  // first piece of a value row: VP elements per lane, then the rest
-  static constexpr int VP = C::kInt8 ? (D == 128 ? 16 : 8) : 8;
+  static constexpr int ES = C::kInt8 ? 1 : 2;
+  static constexpr int KS = C::kInt8 || D == 64 ? 32 : 16;  // keys per step
+  static constexpr int NG = KS / 8;                          // n8 groups of keys
+  static constexpr int STEPS = D / 16;                       // k16 steps of a score
+  static constexpr int TILES = D / 8;                        // n8 tiles of an output
+  static constexpr int CHUNKS = D * ES / 16;                 // 16-byte pieces of a row
+  // bytes of a row in the ring, and lanes that fetch one
+  static constexpr int RS = CHUNKS <= 4 ? 64 : CHUNKS <= 8 ? 128 : 256;
+  static constexpr int LPR = RS / 16;
+  static constexpr int HALF = KS * RS;                       // keys, then values
+  static constexpr int SCALES = C::kInt8 ? KS * 8 : 0;       // key scales, value scales
+  static constexpr int STAGE = 2 * HALF + SCALES + 16;       // and presence, first key
+  static constexpr int STAGES = 24576 / (2 * HALF);
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int SMEM = kWarps * RING + kWarps * kWarps * D * 4;
+  [[maybe_unused]] static constexpr int E = D % 64 == 0 ? 16 : 8;  // int8: elements per key read
 };
 
-template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t* r, const uint8_t* p) {
-  if constexpr (WORDS == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
-  } else if constexpr (WORDS == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    r[0] = v.x, r[1] = v.y;
-  } else {
-    r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+// Where piece `c` of row `r` is.  16-bit rows: so that the eight rows of a
+// matrix read meet in no bank.  int8 rows of 128 bytes: so that neither reads
+// of two rows of four pieces (keys) nor of four rows of two (values) do.
+template <class C, int D>
+__device__ __forceinline__ int place(int r, int c) {
+  using S = Shape<C, D>;
+  const int x = !C::kInt8     ? r & 7
+                : S::RS == 64 ? r >> 1 & 3
+                              : ((r >> 1 & 3) * 2) ^ ((r & 1) * 4);
+  return r * S::RS + ((c ^ x) << 4);
 }
 
 template <class C>
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (C::kBf16)
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Head dimension that element e (0 <= e < D/8) of lane group n's value words is.
-template <class C, int D>
-__device__ __forceinline__ int value_dim(int n, int e) {
-  using S = Shape<C, D>;
-  if (S::VE <= S::VP) return n * S::VE + e;
-  if (e < S::VP) return n * S::VP + e;
-  if (!C::kInt8 && D == 128) return 64 + n * 8 + (e - 8);
-  return 8 * S::VP + n * (S::VE - S::VP) + (e - S::VP);
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0)
+               : "memory");
 }
 
-// A step's keys (scales and presence with them), as this lane holds them.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t* r, const uint8_t* p) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x, r[1] = v.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// Head dimension of column n of output tile i.  16-bit values are read as
+// matrices, in order.  A lane reads int8 values as one piece of 16 or 8 codes
+// (D = 96: 8, then 4), and takes tile i's from its code i.
 template <class C, int D>
-struct Keys {
-  uint32_t w[Shape<C, D>::NG][Shape<C, D>::KW];
-  float ks, vs;   // int8: scales of key (key0 + lane)
-  int key0;
-  int page;       // the step's page, or -2: looked up key by key
-  uint32_t there; // bit i: key0 + i is loaded
-};
+__device__ __forceinline__ int value_dim(int n, int i) {
+  if constexpr (!C::kInt8) return i * 8 + n;
+  else if constexpr (D == 96) return i < 8 ? n * 8 + i : 64 + n * 4 + (i - 8);
+  else return n * (D / 8) + i;
+}
+// Head dimension of the first of a lane's four elements in k16 step k: of the
+// queries, and of the keys that meet them (16-bit keys: the second pair is 8 on).
+template <class C, int D>
+__device__ __forceinline__ int key_dim(int k, int c4, int i) {
+  if constexpr (!C::kInt8) return k * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8;
+  else {
+    constexpr int E = Shape<C, D>::E;
+    return (k / (E / 4)) * 4 * E + c4 * E + (k % (E / 4)) * 4 + i;
+  }
+}
+
+using Part = Walk<kUnit, kRows, kItemUnits>;
 
 template <class C, int D, bool T3>
-__global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant__ Args a) {
   using S = Shape<C, D>;
-  constexpr int ES = C::kInt8 ? 1 : 2;
   using V = typename ValueType<C>::T;
   constexpr bool kQ3 = T3 && C::kBf16;
   constexpr float kUp = C::kBf16 ? 1.0f : static_cast<float>(1 << kLow);
@@ -135,53 +170,142 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
   __shared__ int64_t sums[kWarps];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ int s_last;
-  extern __shared__ __align__(16) float s_o[];  // [warp][row][D]
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem + kWarps * S::RING);  // [warp][row of a pass][D]
 
-  find_share<kUnit, kRows, kThreads>(a, kMinUnits, &cur, sums);
-  if (cur.begin >= cur.end) return;
-  const int64_t end = cur.end, per = cur.per_cta;
-  int64_t at = cur.begin, item0 = cur.item0;
-  int b = cur.b, head = cur.head, block = cur.block;
+  find_share<kUnit, kRows, kItemUnits, kThreads>(a, kMinUnits, &cur, sums);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g8 = lane >> 2, c4 = lane & 3;
+  uint8_t* ring = smem + warp * S::RING;
+  const uint32_t ring_s = saddr(ring);
+  constexpr int SPU = kUnit / S::KS;  // steps per unit
+
+  // ---- the loads: this warp's steps of all the CTA's items, in order.  Unit
+  // warp, warp + kWarps, ... of each part, SPU steps each.
+  Part ld;
+  ld.start(cur);
+  bool more = ld.open(a);
+  int ld_u = warp, ld_s = 0;  // unit of the part, step of the unit
+  int page = -1;              // of key0 + lane of the next step
   const bool whole_pages = a.page_size % S::KS == 0;
+  auto settle = [&] {  // to the next step that exists
+    while (more && ld_u >= ld.n) {
+      ld.close(a);
+      more = ld.open(a);
+      ld_u = warp;
+    }
+  };
+  auto look = [&] {  // its pages, one step before they are needed
+    page = -1;
+    if (!more) return;
+    const int j = ld.key(ld_u) + ld_s * S::KS + lane;
+    if ((S::KS == 32 || lane < S::KS) && j <= ld.un.hi && (j >= ld.un.lo || j < a.sinks))
+      page = page_of(a, ld.b, j);
+  };
+  auto issue = [&](int stage) {
+    if (more) {
+      const int key0 = ld.key(ld_u) + ld_s * S::KS, head = ld.head;
+      const int pg = page;
+      const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0);
+      uint8_t* st = ring + stage * S::STAGE;
+      const uint32_t dst = ring_s + stage * S::STAGE;
+      if (lane == 0)
+        *reinterpret_cast<uint2*>(st + 2 * S::HALF + S::SCALES) =
+            make_uint2(there, static_cast<uint32_t>(key0));
+      const int r0 = lane / S::LPR, c = lane % S::LPR;
+      constexpr int RPI = 32 / S::LPR, N = S::KS / RPI;  // rows per instruction, instructions
+      const bool in = S::LPR == S::CHUNKS || c < S::CHUNKS;
+      if (whole_pages && there == (S::KS == 32 ? 0xffffffffu : (1u << (S::KS & 31)) - 1u)) {
+        // one page holds the step: addresses advance by constants
+        const int p0 = __shfl_sync(0xffffffffu, pg, 0);
+        const int off = key0 % a.page_size + r0;
+        const uint8_t* pk = a.k.data + (p0 * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16;
+        const uint8_t* pv = a.v.data + (p0 * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16;
+        const int64_t dk = a.k.token * (RPI * S::ES), dv = a.v.token * (RPI * S::ES);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (in) cp16(dst + place<C, D>(r0 + i * RPI, c), pk, true);
+          pk += dk;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (in) cp16(dst + S::HALF + place<C, D>(r0 + i * RPI, c), pv, true);
+          pv += dv;
+        }
+      } else {
+        const int my_off = pg >= 0 ? (key0 + lane) % a.page_size : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = r0 + i * RPI;
+          const int pr = __shfl_sync(0xffffffffu, pg, r);
+          const int off = __shfl_sync(0xffffffffu, my_off, r);
+          const bool on = pr >= 0;
+          const int64_t p = on ? pr : 0;
+          if (in) {
+            cp16(dst + place<C, D>(r, c),
+                 a.k.data + (p * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16, on);
+            cp16(dst + S::HALF + place<C, D>(r, c),
+                 a.v.data + (p * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16, on);
+          }
+        }
+      }
+      if constexpr (C::kInt8) {
+        const bool on = pg >= 0;
+        const int64_t p = on ? pg : 0;
+        const int off = on ? (key0 + lane) % a.page_size : 0;
+        cp4(dst + 2 * S::HALF + lane * 4,
+            a.k.scales + p * a.k.spage + off * a.k.stoken + head * a.k.shead, on);
+        cp4(dst + 2 * S::HALF + S::KS * 4 + lane * 4,
+            a.v.scales + p * a.v.spage + off * a.v.stoken + head * a.v.shead, on);
+      }
+      if (++ld_s == SPU) {
+        ld_s = 0;
+        ld_u += kWarps;
+        settle();
+      }
+      look();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  settle();
+  look();
+#pragma unroll 1
+  for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
+  int stage = 0;
 
-  while (at < end) {
-    const Request rq = request(a, b);
-    const Units un = units<kUnit, kRows>(a, rq, block);
-    const int u_begin = static_cast<int>(at - item0);
-    const int u_end = static_cast<int>(min(static_cast<int64_t>(un.n), end - item0));
-    const int rows = min(kRows, rq.n * a.group - block * kRows);
-
+  Part w;
+  w.start(cur);
+  while (w.open(a)) {
+    const int rows = w.rows;
     // ---- this lane's row: query parts, position, window
-    const int r = block * kRows + g8;
+    const int r = w.block * kRows + g8;
     const bool row_ok = g8 < rows;
-    const int pos = row_ok ? rq.base + r / a.group : -1;
+    const int pos = row_ok ? w.rq.base + r / a.group : -1;
     const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
-    // the block's rows: keys up to p_first that are at or past lo_last are seen by all of them
-    const int p_first = rq.base + block * kRows / a.group;
+    // keys up to p_first that are at or past lo_last are seen by all of the block's rows
+    const int p_first = w.rq.base + w.block * kRows / a.group;
     const int lo_last =
-        a.window > 0 ? rq.base + (block * kRows + rows - 1) / a.group - a.window + 1 : 0;
+        a.window > 0 ? w.rq.base + (w.block * kRows + rows - 1) / a.group - a.window + 1 : 0;
 
-    uint32_t qa[S::STEPS][4];                 // hi, lo, hi, lo of 4 elements
-    uint32_t qc[kQ3 ? S::STEPS : 1][2];        // third parts
+    uint32_t qa[S::STEPS][4];           // hi, lo, hi, lo of 4 elements
+    uint32_t qc[kQ3 ? S::STEPS : 1][2];  // third parts
     float cscale;
     {
-      const int64_t q0 = row_ok ? (rq.start + r / a.group) * a.q_token +
-                                      (head * a.group + r % a.group) * a.q_head
+      const int64_t q0 = row_ok ? (w.rq.start + r / a.group) * a.q_token +
+                                      (w.head * a.group + r % a.group) * a.q_head
                                 : 0;
       float x[S::STEPS][4];
       float amax = 0.0f;
 #pragma unroll
-      for (int k = 0; k < S::STEPS; ++k) {
-        const int d = (k / (S::E / 4)) * 4 * S::E + c4 * S::E + (k % (S::E / 4)) * 4;
+      for (int k = 0; k < S::STEPS; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[k][i] = row_ok ? load_elem(a.q, a.q_type, q0 + d + i) : 0.0f;
-          amax = fmaxf(amax, fabsf(x[k][i]));
-        }
-      }
+        for (int i = 0; i < 4; ++i)
+          x[k][i] = row_ok ? load_elem(a.q, a.q_type, q0 + key_dim<C, D>(k, c4, i)) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < S::STEPS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const int e = row_exponent(amax);
@@ -201,168 +325,111 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
         }
     }
 
-    float o[S::VE][4];
+    float o[S::TILES][4];
 #pragma unroll
-    for (int i = 0; i < S::VE; ++i)
+    for (int i = 0; i < S::TILES; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    // ---- steps: units u_begin + warp, + 8, ..., each of 32 / KS steps
-    constexpr int SPU = kUnit / S::KS;
-    const int steps = u_begin + warp < u_end ? ((u_end - u_begin - warp + kWarps - 1) / kWarps) * SPU : 0;
-    auto key_of = [&](int s) {
-      const int u = u_begin + warp + (s / SPU) * kWarps;
-      return (u < un.sink ? u : un.first + u - un.sink) * kUnit + (s % SPU) * S::KS;
-    };
-    // whether some row of the block sees key j (the page aside)
-    auto wanted = [&](int j) {
-      return j <= un.hi && (j >= un.lo || j < a.sinks);
-    };
-    auto load_keys = [&](Keys<C, D>& K, int s) {
-      K.key0 = key_of(s);
-      int mypage = -1;  // of key0 + lane
-      const int jl = K.key0 + lane;
-      const bool mine = (S::KS == 32 || lane < S::KS) && wanted(jl);
-      if (whole_pages) {
-        int p = -1;
-        if (K.key0 < rq.limit) p = page_of(a, b, K.key0);
-        K.page = p;
-        mypage = p;
-      } else {
-        K.page = -2;
-        if (mine) mypage = page_of(a, b, jl);
-      }
-      K.there = __ballot_sync(0xffffffffu, mine && mypage >= 0);
-      const int off0 = K.key0 % a.page_size;
-#pragma unroll
-      for (int n = 0; n < S::NG; ++n) {
-        const int i = n * 8 + g8;
-        int page = K.page, off = off0 + i;
-        if (!whole_pages) {
-          page = __shfl_sync(0xffffffffu, mypage, i);
-          off = (K.key0 + i) % a.page_size;
-        }
-        if (K.there >> i & 1u) {
-          const uint8_t* p = a.k.data + (page * a.k.page + off * a.k.token + head * a.k.head) * ES +
-                             c4 * S::E * ES;
-#pragma unroll
-          for (int x = 0; x < S::KL; ++x) load_words<S::LW>(K.w[n] + x * S::LW, p + x * 4 * S::E * ES);
-        } else {
-#pragma unroll
-          for (int x = 0; x < S::KW; ++x) K.w[n][x] = 0u;
-        }
-      }
-      if constexpr (C::kInt8) {
-        K.ks = 0.0f, K.vs = 0.0f;
-        if (K.there >> lane & 1u) {
-          const int off = whole_pages ? off0 + lane : jl % a.page_size;
-          K.ks = __ldg(a.k.scales + mypage * a.k.spage + off * a.k.stoken + head * a.k.shead);
-          K.vs = __ldg(a.v.scales + mypage * a.v.spage + off * a.v.stoken + head * a.v.shead);
-        }
-      }
-      if (!whole_pages) K.page = mypage;  // per lane from here on
-    };
-
-    Keys<C, D> K;
-    if (steps > 0) load_keys(K, 0);
+    const int steps = warp < w.n ? (w.n - warp + kWarps - 1) / kWarps * SPU : 0;
+#pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-      const int key0 = K.key0;
-      const uint32_t there = K.there;
-      // ---- this step's values go out
-      uint32_t vw[S::KV][S::VW];
-      const int off0 = key0 % a.page_size;
-#pragma unroll
-      for (int x = 0; x < S::KV; ++x) {
-        const int i = (x >> 2) * 16 + ((x >> 1) & 1) * 8 + 2 * c4 + (x & 1);
-        int page = K.page, off = off0 + i;
-        if (!whole_pages) {
-          page = __shfl_sync(0xffffffffu, K.page, i);
-          off = (key0 + i) % a.page_size;
-        }
-        if (there >> i & 1u) {
-          const uint8_t* p = a.v.data + (page * a.v.page + off * a.v.token + head * a.v.head) * ES;
-          if constexpr (!C::kInt8 && D == 128) {
-            load_words<4>(vw[x], p + g8 * 16);
-            load_words<4>(vw[x] + 4, p + 128 + g8 * 16);
-          } else if constexpr (S::VE > S::VP) {  // D = 96
-            load_words<S::VP * ES / 4>(vw[x], p + g8 * S::VP * ES);
-            load_words<(S::VE - S::VP) * ES / 4>(vw[x] + S::VP * ES / 4,
-                                                 p + 8 * S::VP * ES + g8 * (S::VE - S::VP) * ES);
-          } else {
-            load_words<S::VW>(vw[x], p + g8 * S::VE * ES);
-          }
-        } else {
-#pragma unroll
-          for (int y = 0; y < S::VW; ++y) vw[x][y] = 0u;
-        }
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+      __syncwarp();  // this step has landed for all lanes, and all are done with the one before
+      issue(stage == 0 ? S::STAGES - 1 : stage - 1);
+      const uint8_t* st = ring + stage * S::STAGE;
+      const uint32_t st_s = ring_s + stage * S::STAGE;
+      if (++stage == S::STAGES) stage = 0;
+      const uint2 info = *reinterpret_cast<const uint2*>(st + 2 * S::HALF + S::SCALES);
+      const uint32_t there = info.x;
+      const int key0 = static_cast<int>(info.y);
+
       // ---- scores
       float sc[S::NG][4];
 #pragma unroll
-      for (int n = 0; n < S::NG; ++n) {
-        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+      for (int n = 0; n < S::NG; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+      if constexpr (!C::kInt8) {
 #pragma unroll
-        for (int k = 0; k < S::STEPS; ++k) {
-          uint32_t b0, b1;
-          if constexpr (C::kInt8) {
-            const uint32_t w = K.w[n][k] ^ 0x80808080u;
-            b0 = codes_f16(w, 0x4140u);
-            b1 = codes_f16(w, 0x4342u);
-          } else {
-            b0 = K.w[n][2 * k];
-            b1 = K.w[n][2 * k + 1];
+        for (int k = 0; k < S::STEPS; k += 2)
+#pragma unroll
+          for (int n = 0; n < S::NG; ++n) {
+            uint32_t kb[4];  // eight keys x 32 dimensions
+            ldmatrix4(kb, st_s + place<C, D>(n * 8 + (lane & 7), k * 2 + (lane >> 3)));
+            mma<C>(sc[n], qa[k], kb[0], kb[1]);
+            mma<C>(sc[n], qa[k + 1], kb[2], kb[3]);
+            if constexpr (kQ3) {
+              const uint32_t q3[4] = {qc[k][0], 0u, qc[k][1], 0u};
+              const uint32_t q4[4] = {qc[k + 1][0], 0u, qc[k + 1][1], 0u};
+              mma<C>(sc[n], q3, kb[0], kb[1]);
+              mma<C>(sc[n], q4, kb[2], kb[3]);
+            }
           }
-          mma<C>(sc[n], qa[k], b0, b1);
-          if constexpr (kQ3) {
-            const uint32_t q3[4] = {qc[k][0], 0u, qc[k][1], 0u};
-            mma<C>(sc[n], q3, b0, b1);
+      } else {
+        constexpr int LW = S::E / 4;
+#pragma unroll
+        for (int x = 0; x < D / (4 * S::E); ++x)
+#pragma unroll
+          for (int n = 0; n < S::NG; ++n) {
+            uint32_t kw[LW];
+            const int byte = x * 4 * S::E + c4 * S::E;
+            lds_words<LW>(kw, st + place<C, D>(n * 8 + g8, byte >> 4) + (byte & 15));
+#pragma unroll
+            for (int y = 0; y < LW; ++y) {
+              const uint32_t u = kw[y] ^ 0x80808080u;
+              mma<C>(sc[n], qa[x * LW + y], codes_f16(u, 0x4140u), codes_f16(u, 0x4342u));
+            }
           }
-        }
       }
-      const float ks = K.ks, vs = K.vs;
-      // ---- the next step's keys go out
-      if (s + 1 < steps) load_keys(K, s + 1);
-
       // ---- weights: log2-domain scores, masks, running maximum
       const bool all = there == (S::KS == 32 ? 0xffffffffu : 0xffffu) &&
                        key0 + S::KS - 1 <= p_first && (key0 >= lo_last || key0 + S::KS <= a.sinks);
+      const float* sks = reinterpret_cast<const float*>(st + 2 * S::HALF);
       float t[S::NG][2];
       float mx = -INFINITY, lnew = 0.0f;
 #pragma unroll
-      for (int n = 0; n < S::NG; ++n)
+      for (int n = 0; n < S::NG; ++n) {
+        float2 ks = make_float2(1.0f, 1.0f);
+        if constexpr (C::kInt8) ks = *reinterpret_cast<const float2*>(sks + n * 8 + 2 * c4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float v = fmaf(sc[n][i + 2], kDown, sc[n][i]) * cscale;
-          if constexpr (C::kInt8) v *= __shfl_sync(0xffffffffu, ks, n * 8 + 2 * c4 + i);
-          if (!all) {
-            const int x = n * 8 + 2 * c4 + i, j = key0 + x;
-            if (!(there >> x & 1u) || j > pos || (j < row_lo && j >= a.sinks)) v = -INFINITY;
-          }
+          if constexpr (C::kInt8) v *= i ? ks.y : ks.x;
           t[n][i] = v;
-          mx = fmaxf(mx, v);
         }
+      }
+      if (!all) {
+#pragma unroll
+        for (int n = 0; n < S::NG; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int x = n * 8 + 2 * c4 + i, j = key0 + x;
+            if (!(there >> x & 1u) || j > pos || (j < row_lo && j >= a.sinks)) t[n][i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < S::NG; ++n) mx = fmaxf(mx, fmaxf(t[n][0], t[n][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float mn = fmaxf(m, mx);
       const float ref = mn == -INFINITY ? 0.0f : mn;
-      float w[S::NG][2];  // weights times 2^kTop
+      float p[S::NG][2];  // weights times 2^kTop
 #pragma unroll
-      for (int n = 0; n < S::NG; ++n)
+      for (int n = 0; n < S::NG; ++n) {
+        float2 vs = make_float2(1.0f, 1.0f);
+        if constexpr (C::kInt8) vs = *reinterpret_cast<const float2*>(sks + S::KS + n * 8 + 2 * c4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          w[n][i] = ex2(t[n][i] - ref) * static_cast<float>(1 << kTop);
-          lnew += w[n][i];
-          if constexpr (C::kInt8) {
-            const float v = __shfl_sync(0xffffffffu, vs, n * 8 + 2 * c4 + i);
-            w[n][i] = w[n][i] == 0.0f ? 0.0f : w[n][i] * v;
-          }
+          p[n][i] = ex2(t[n][i] - ref) * static_cast<float>(1 << kTop);
+          lnew += p[n][i];
+          if constexpr (C::kInt8) p[n][i] *= i ? vs.y : vs.x;
         }
+      }
       if (__any_sync(0xffffffffu, mn != m)) {
         const float corr = ex2(m - ref);
         l *= corr;
 #pragma unroll
-        for (int i = 0; i < S::VE; ++i)
+        for (int i = 0; i < S::TILES; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[i][j] *= corr;
         m = mn;
@@ -374,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
         uint32_t pa[4], pc[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = w[2 * kk + h][0], p1 = w[2 * kk + h][1];
+          const float p0 = p[2 * kk + h][0], p1 = p[2 * kk + h][1];
           const uint32_t hi = pack16<V>(p0, p1);
           const float r0 = (p0 - low16<V>(hi)) * kUpV, r1 = (p1 - high16<V>(hi)) * kUpV;
           pa[2 * h] = hi;
@@ -382,15 +449,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
           if constexpr (T3)
             pc[2 * h] = pack16<V>(r0 - low16<V>(pa[2 * h + 1]), r1 - high16<V>(pa[2 * h + 1]));
         }
-        const uint32_t* v0 = vw[4 * kk];
-        const uint32_t* v1 = vw[4 * kk + 1];
-        const uint32_t* v2 = vw[4 * kk + 2];
-        const uint32_t* v3 = vw[4 * kk + 3];
-        if constexpr (C::kInt8) {
+        if constexpr (!C::kInt8) {
 #pragma unroll
-          for (int x = 0; x < S::VW; ++x) {
-            const uint32_t x0 = prmt(v0[x], v1[x], 0x5140u), x1 = prmt(v0[x], v1[x], 0x7362u);
-            const uint32_t y0 = prmt(v2[x], v3[x], 0x5140u), y1 = prmt(v2[x], v3[x], 0x7362u);
+          for (int i = 0; i < S::TILES; i += 2) {
+            uint32_t vb[4];  // 16 keys x 16 dimensions, transposed
+            ldmatrix4_t(vb, st_s + S::HALF + place<C, D>(kk * 16 + (lane & 15), i + (lane >> 4)));
+            mma<V>(o[i], pa, vb[0], vb[1]);
+            mma<V>(o[i + 1], pa, vb[2], vb[3]);
+            if constexpr (T3) {
+              mma<V>(o[i], pc, vb[0], vb[1]);
+              mma<V>(o[i + 1], pc, vb[2], vb[3]);
+            }
+          }
+        } else {
+          constexpr int VE = D / 8, VP = D == 128 ? 16 : 8, VW = VE / 4;
+          uint32_t vw[4][VW];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = kk * 16 + (x >> 1) * 8 + 2 * c4 + (x & 1);
+            const uint8_t* row = st + S::HALF;
+            const int byte = g8 * VP;
+            lds_words<VP / 4>(vw[x], row + place<C, D>(key, byte >> 4) + (byte & 15));
+            if constexpr (VE > VP) {
+              const int rest = 64 + g8 * 4;
+              lds_words<1>(vw[x] + VP / 4, row + place<C, D>(key, rest >> 4) + (rest & 15));
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < VW; ++x) {
+            const uint32_t x0 = prmt(vw[0][x], vw[1][x], 0x5140u), x1 = prmt(vw[0][x], vw[1][x], 0x7362u);
+            const uint32_t y0 = prmt(vw[2][x], vw[3][x], 0x5140u), y1 = prmt(vw[2][x], vw[3][x], 0x7362u);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t sel = e & 1 ? 0x4342u : 0x4140u;
@@ -400,63 +488,82 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
               if constexpr (T3) mma<V>(o[4 * x + e], pc, b0, b1);
             }
           }
-        } else {
-#pragma unroll
-          for (int x = 0; x < S::VW; ++x) {
-            const uint32_t b0 = prmt(v0[x], v1[x], 0x5410u), b1 = prmt(v2[x], v3[x], 0x5410u);
-            const uint32_t d0 = prmt(v0[x], v1[x], 0x7632u), d1 = prmt(v2[x], v3[x], 0x7632u);
-            mma<V>(o[2 * x], pa, b0, b1);
-            mma<V>(o[2 * x + 1], pa, d0, d1);
-            if constexpr (T3) {
-              mma<V>(o[2 * x], pc, b0, b1);
-              mma<V>(o[2 * x + 1], pc, d0, d1);
-            }
-          }
         }
       }
     }
 
-    // ---- join the warps: row w of the block by warp w
+    // ---- join the warps that had steps: a row of the block by one warp
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    float* so = s_o + (warp * kRows + g8) * D;
-#pragma unroll
-    for (int i = 0; i < S::VE; ++i) {
-      so[value_dim<C, D>(2 * c4, i)] = fmaf(o[i][2], kDownV, o[i][0]);
-      so[value_dim<C, D>(2 * c4 + 1, i)] = fmaf(o[i][3], kDownV, o[i][1]);
-    }
-    if (c4 == 0) {
+    if (warp < w.n && c4 == 0) {
       s_m[warp][g8] = m;
       s_l[warp][g8] = l;
     }
-    __syncthreads();
+    const int nw = min(kWarps, w.n);
     constexpr int DL = D / 32;
-    float ro[DL], rm = -INFINITY, rl = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DL; ++i) ro[i] = 0.0f;
-    for (int w = 0; w < kWarps; ++w) rm = fmaxf(rm, s_m[w][warp]);
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = s_m[w][warp];
-      if (mw == -INFINITY && s_l[w][warp] == 0.0f) continue;  // a warp that saw nothing
-      const float f = ex2(mw - (rm == -INFINITY ? 0.0f : rm));
-      rl = fmaf(s_l[w][warp], f, rl);
-#pragma unroll
-      for (int i = 0; i < DL; ++i)
-        ro[i] = fmaf(s_o[(w * kRows + warp) * D + lane + 32 * i], f, ro[i]);
-    }
+    const Sharers sh = sharers(w.item0, w.un.n, w.per);
+    const bool alone = sh.last == sh.first;
+    constexpr int kSlot = kRows * (D + 2);
 
-    // ---- an item of several CTAs: leave the partial, the last one joins
-    bool final = true;
-    const Sharers sh = sharers(item0, un.n, per);
-    if (sh.last > sh.first) {
-      constexpr int kSlot = kRows * (D + 2);
-      float* mine = a.partials + static_cast<int64_t>(slot_of(blockIdx.x, item0, per)) * kSlot;
+    auto finish = [&](int row, const float* ro, float rm, float rl) {
+      const int rr = w.block * kRows + row;
+      const int t = rr / a.group, g = rr % a.group;
+      bool good = finite(rl);
 #pragma unroll
-      for (int i = 0; i < DL; ++i) mine[warp * D + lane + 32 * i] = ro[i];
-      if (lane == 0) {
-        mine[kRows * D + warp] = rm;
-        mine[kRows * D + kRows + warp] = rl;
+      for (int i = 0; i < DL; ++i) good = good && finite(ro[i]);
+      if (__all_sync(0xffffffffu, good)) {
+        const int qh = w.head * a.group + g;
+        const int64_t orow = (w.rq.start + t) * a.o_token + qh * a.o_head;
+#pragma unroll
+        for (int i = 0; i < DL; ++i)
+          store_elem(a.out, a.q_type, orow + lane + 32 * i, rl == 0.0f ? 0.0f : __fdiv_rn(ro[i], rl));
+        if (a.lse && lane == 0)
+          a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
+              rl == 0.0f ? -INFINITY : (rm + (log2f(rl) - kTop)) * kLn2;
+      } else {
+        exact_row<C, D>(a, w.b, w.head, t, g);
       }
+    };
+
+    for (int row0 = 0; row0 < rows; row0 += kWarps) {
+      if (row0) __syncthreads();
+      if (warp < w.n && row_ok && g8 >= row0 && g8 < row0 + kWarps) {
+        float* so = s_o + (warp * kWarps + g8 - row0) * D;
+#pragma unroll
+        for (int i = 0; i < S::TILES; ++i) {
+          so[value_dim<C, D>(2 * c4, i)] = fmaf(o[i][2], kDownV, o[i][0]);
+          so[value_dim<C, D>(2 * c4 + 1, i)] = fmaf(o[i][3], kDownV, o[i][1]);
+        }
+      }
+      __syncthreads();
+      const int row = row0 + warp;
+      if (row >= rows) continue;
+      float ro[DL], rm = -INFINITY, rl = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DL; ++i) ro[i] = 0.0f;
+      for (int x = 0; x < nw; ++x) rm = fmaxf(rm, s_m[x][row]);
+      const float ref = rm == -INFINITY ? 0.0f : rm;
+      for (int x = 0; x < nw; ++x) {
+        const float f = ex2(s_m[x][row] - ref);
+        rl = fmaf(s_l[x][row], f, rl);
+#pragma unroll
+        for (int i = 0; i < DL; ++i)
+          ro[i] = fmaf(s_o[(x * kWarps + warp) * D + lane + 32 * i], f, ro[i]);
+      }
+      if (alone) {
+        finish(row, ro, rm, rl);
+      } else {
+        float* mine = a.partials + static_cast<int64_t>(slot_of(blockIdx.x, w.item0, w.per)) * kSlot;
+#pragma unroll
+        for (int i = 0; i < DL; ++i) mine[row * D + lane + 32 * i] = ro[i];
+        if (lane == 0) {
+          mine[kRows * D + row] = rm;
+          mine[kRows * D + kRows + row] = rl;
+        }
+      }
+    }
+    // ---- an item of several CTAs: the one that arrives last joins the parts
+    if (!alone) {
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -465,59 +572,51 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_rows(const __grid_constant
         __threadfence();
       }
       __syncthreads();
-      final = s_last != 0;
-      if (final) {
-        rm = -INFINITY, rl = 0.0f;
+      if (s_last) {
+        for (int row = warp; row < rows; row += kWarps) {
+          // the parts' maxima and sums by lanes, then the outputs in CTA order
+          float ro[DL], rm = -INFINITY, rl = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DL; ++i) ro[i] = 0.0f;
-        for (int c = sh.first; c <= sh.last; ++c) {
-          const float* other = a.partials + static_cast<int64_t>(slot_of(c, item0, per)) * kSlot;
-          rm = fmaxf(rm, __ldcg(other + kRows * D + warp));
-        }
-        const float ref = rm == -INFINITY ? 0.0f : rm;
-        for (int c = sh.first; c <= sh.last; ++c) {
-          const float* other = a.partials + static_cast<int64_t>(slot_of(c, item0, per)) * kSlot;
-          const float f = ex2(__ldcg(other + kRows * D + warp) - ref);
-          rl = fmaf(__ldcg(other + kRows * D + kRows + warp), f, rl);
+          for (int i = 0; i < DL; ++i) ro[i] = 0.0f;
+          for (int x = sh.first + lane; x <= sh.last; x += 32)
+            rm = fmaxf(rm, __ldcg(a.partials + slot_of(x, w.item0, w.per) * static_cast<int64_t>(kSlot) +
+                                  kRows * D + row));
 #pragma unroll
-          for (int i = 0; i < DL; ++i)
-            ro[i] = fmaf(__ldcg(other + warp * D + lane + 32 * i), f, ro[i]);
+          for (int x = 16; x > 0; x >>= 1) rm = fmaxf(rm, __shfl_xor_sync(0xffffffffu, rm, x));
+          const float ref = rm == -INFINITY ? 0.0f : rm;
+#pragma unroll 4
+          for (int x = sh.first; x <= sh.last; ++x) {
+            const float* other =
+                a.partials + slot_of(x, w.item0, w.per) * static_cast<int64_t>(kSlot);
+            const float f = ex2(__ldcg(other + kRows * D + row) - ref);
+            rl = fmaf(__ldcg(other + kRows * D + kRows + row), f, rl);
+#pragma unroll
+            for (int i = 0; i < DL; ++i)
+              ro[i] = fmaf(__ldcg(other + row * D + lane + 32 * i), f, ro[i]);
+          }
+          finish(row, ro, rm, rl);
         }
       }
     }
-    if (final && warp < rows) {
-      const int rr = block * kRows + warp;
-      const int t = rr / a.group, g = rr % a.group;
-      bool good = finite(rl);
-#pragma unroll
-      for (int i = 0; i < DL; ++i) good = good && finite(ro[i]);
-      if (__all_sync(0xffffffffu, good)) {
-        const int qh = head * a.group + g;
-        const int64_t orow = (rq.start + t) * a.o_token + qh * a.o_head;
-#pragma unroll
-        for (int i = 0; i < DL; ++i)
-          store_elem(a.out, a.q_type, orow + lane + 32 * i, rl == 0.0f ? 0.0f : __fdiv_rn(ro[i], rl));
-        if (a.lse && lane == 0)
-          a.lse[static_cast<int64_t>(rq.start + t) * a.heads + qh] =
-              rl == 0.0f ? -INFINITY : (rm + (log2f(rl) - kTop)) * kLn2;
-      } else {
-        exact_row<C, D>(a, b, head, t, g);
-      }
-    }
-    __syncthreads();  // s_o, s_m, s_l are free for the next item
-    at = item0 + u_end;
-    if (u_end == un.n) {
-      item0 += un.n;
-      next_item<kRows>(a, b, head, block);
-    }
+    __syncthreads();  // s_o, s_m, s_l, s_last are free for the next item
+    w.close(a);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <class C, int D, bool T3>
 int launch(const Args& a, cudaStream_t st) {
+  using S = Shape<C, D>;
   const DeviceInfo& di = device_info();
-  constexpr int smem = kWarps * kRows * D * 4;
-  k_attn_rows<C, D, T3><<<di.sm_count, kThreads, smem, st>>>(a);
+  static int attr_set[kMaxDevices];
+  const int slot = di.ordinal % kMaxDevices;
+  if (!attr_set[slot]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_attn_rows<C, D, T3>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return cuda_status(e);
+    attr_set[slot] = 1;
+  }
+  k_attn_rows<C, D, T3><<<2 * di.sm_count, kThreads, S::SMEM, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
