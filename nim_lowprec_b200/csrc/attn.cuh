@@ -42,6 +42,7 @@ struct Args {
   const int32_t* seqlens;
   int64_t table_stride;
   int table_width, pages, page_size;
+  int page_shift;  // log2 of page_size, -1 where it is no power of two
   int requests, tokens, heads, kv_heads, group;
   int window, sinks;  // window 0: none
   float scale_log2;   // softmax scale * log2(e)
@@ -264,10 +265,27 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
 
+// A key's page of its request and its place in the page.  Page sizes are
+// nearly always powers of two, and a division is a long chain of instructions.
+__device__ __forceinline__ int page_index(const Args& a, int j) {
+  return a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+}
+__device__ __forceinline__ int page_offset(const Args& a, int j) {
+  return a.page_shift >= 0 ? j & (a.page_size - 1) : j % a.page_size;
+}
+
+// The table's entry for key j of request b, for use later: valid_page() looks
+// at it first, so the load is not waited for where it is made.
+__device__ __forceinline__ int entry_of(const Args& a, int b, int j) {
+  return __ldg(a.table + b * a.table_stride + page_index(a, j));
+}
+__device__ __forceinline__ int valid_page(const Args& a, int entry) {
+  return static_cast<unsigned>(entry) < static_cast<unsigned>(a.pages) ? entry : -1;
+}
+
 // Page of key j of request b, or -1 where the table has none.
 __device__ __forceinline__ int page_of(const Args& a, int b, int j) {
-  const int p = __ldg(a.table + b * a.table_stride + j / a.page_size);
-  return static_cast<unsigned>(p) < static_cast<unsigned>(a.pages) ? p : -1;
+  return valid_page(a, entry_of(a, b, j));
 }
 
 template <class C>
@@ -305,7 +323,7 @@ __device__ __noinline__ void exact_row(const Args& a, int b, int head, int t, in
     if (j >= end) break;
     const int page = page_of(a, b, j);
     if (page < 0) continue;
-    const int off = j % a.page_size;
+    const int off = page_offset(a, j);
     const int64_t kr = page * a.k.page + off * a.k.token + head * a.k.head;
     const int64_t ks = page * a.k.spage + off * a.k.stoken + head * a.k.shead;
     float s = 0.0f;

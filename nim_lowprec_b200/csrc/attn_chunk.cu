@@ -175,18 +175,19 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
   bool lap = false;     // the ring has been filled once
   uint32_t tile = 0;    // key tiles so far, over all items: meta slot
 
-  // The page of key t of the item's tile i: looked up a tile ahead.
-  int next_page = -1;
+  // The table's entry for key t of the item's tile i: looked up a tile ahead.
+  int next_entry = -1;
   auto look = [&](int i) {
     const int j = w.key(i) + t;
-    next_page = j <= w.un.hi && (j >= w.un.lo || j < a.sinks) ? page_of(a, w.b, j) : -1;
+    next_entry = -1;
+    if (j <= w.un.hi && (j >= w.un.lo || j < a.sinks)) next_entry = entry_of(a, w.b, j);
   };
   // where tile i's rows are; its scales and presence for the softmax
   auto locate = [&](int i, uint32_t slot) {
-    const int page = next_page;
+    const int page = valid_page(a, next_entry);
     if (i + 1 < w.n) look(i + 1);
     const bool on = page >= 0;
-    const int off = on ? (w.key(i) + t) % a.page_size : 0;
+    const int off = on ? page_offset(a, w.key(i) + t) : 0;
     const int m = slot % 3;
     sh.koff[m][t] = on ? page * a.k.page + off * a.k.token + w.head * a.k.head : -1;
     sh.voff[m][t] = on ? page * a.v.page + off * a.v.token + w.head * a.v.head : -1;

@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
   ld.start(cur);
   bool more = ld.open(a);
   int ld_u = warp, ld_s = 0;  // unit of the part, step of the unit
-  int page = -1;              // of key0 + lane of the next step
-  const bool whole_pages = a.page_size % S::KS == 0;
+  int entry = -1;             // the table's, for key0 + lane of the next step
+  const bool halves = a.page_size % 16 == 0;  // a page holds each 16 keys of a step
   auto settle = [&] {  // to the next step that exists
     while (more && ld_u >= ld.n) {
       ld.close(a);
@@ -197,16 +197,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
     }
   };
   auto look = [&] {  // its pages, one step before they are needed
-    page = -1;
+    entry = -1;
     if (!more) return;
     const int j = ld.key(ld_u) + ld_s * S::KS + lane;
     if ((S::KS == 32 || lane < S::KS) && j <= ld.un.hi && (j >= ld.un.lo || j < a.sinks))
-      page = page_of(a, ld.b, j);
+      entry = entry_of(a, ld.b, j);
   };
   auto issue = [&](int stage) {
     if (more) {
       const int key0 = ld.key(ld_u) + ld_s * S::KS, head = ld.head;
-      const int pg = page;
+      const int pg = valid_page(a, entry);
       const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0);
       uint8_t* st = ring + stage * S::STAGE;
       const uint32_t dst = ring_s + stage * S::STAGE;
@@ -214,27 +214,33 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
         *reinterpret_cast<uint2*>(st + 2 * S::HALF + S::SCALES) =
             make_uint2(there, static_cast<uint32_t>(key0));
       const int r0 = lane / S::LPR, c = lane % S::LPR;
-      constexpr int RPI = 32 / S::LPR, N = S::KS / RPI;  // rows per instruction, instructions
+      constexpr int RPI = 32 / S::LPR, N = S::KS / RPI;  // rows per load, loads
       const bool in = S::LPR == S::CHUNKS || c < S::CHUNKS;
-      if (whole_pages && there == (S::KS == 32 ? 0xffffffffu : (1u << (S::KS & 31)) - 1u)) {
-        // one page holds the step: addresses advance by constants
-        const int p0 = __shfl_sync(0xffffffffu, pg, 0);
-        const int off = key0 % a.page_size + r0;
-        const uint8_t* pk = a.k.data + (p0 * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16;
-        const uint8_t* pv = a.v.data + (p0 * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16;
+      if (halves) {
+        // addresses advance by constants within a page
         const int64_t dk = a.k.token * (RPI * S::ES), dv = a.v.token * (RPI * S::ES);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (in) cp16(dst + place<C, D>(r0 + i * RPI, c), pk, true);
-          pk += dk;
-        }
+        for (int h = 0; h < S::KS / 16; ++h) {
+          const uint32_t bits = there >> (16 * h) & 0xffffu;
+          const int p0 = __shfl_sync(0xffffffffu, pg, 16 * h + max(__ffs(bits) - 1, 0));
+          const int64_t pp = bits ? p0 : 0;
+          const int off = page_offset(a, key0 + 16 * h) + r0;
+          const uint8_t* pk = a.k.data + (pp * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16;
+          const uint8_t* pv = a.v.data + (pp * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (in) cp16(dst + S::HALF + place<C, D>(r0 + i * RPI, c), pv, true);
-          pv += dv;
+          for (int i = 0; i < N * 16 / S::KS; ++i) {
+            const int r = 16 * h + r0 + i * RPI;
+            const bool on = there >> r & 1u;
+            if (in) {
+              cp16(dst + place<C, D>(r, c), on ? pk : a.k.data, on);
+              cp16(dst + S::HALF + place<C, D>(r, c), on ? pv : a.v.data, on);
+            }
+            pk += dk;
+            pv += dv;
+          }
         }
       } else {
-        const int my_off = pg >= 0 ? (key0 + lane) % a.page_size : 0;
+        const int my_off = pg >= 0 ? page_offset(a, key0 + lane) : 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int r = r0 + i * RPI;
@@ -253,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
       if constexpr (C::kInt8) {
         const bool on = pg >= 0;
         const int64_t p = on ? pg : 0;
-        const int off = on ? (key0 + lane) % a.page_size : 0;
+        const int off = on ? page_offset(a, key0 + lane) : 0;
         cp4(dst + 2 * S::HALF + lane * 4,
             a.k.scales + p * a.k.spage + off * a.k.stoken + head * a.k.shead, on);
         cp4(dst + 2 * S::HALF + S::KS * 4 + lane * 4,

@@ -170,6 +170,9 @@ int lp_paged_attention(const lp_kv_cache* cache, const int32_t* block_tables, in
   a.table_width = static_cast<int>(table_width);
   a.pages = static_cast<int>(cache->pages);
   a.page_size = static_cast<int>(cache->page_size);
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (cache->page_size == int64_t{1} << i) a.page_shift = i;
   a.requests = static_cast<int>(n);
   a.tokens = static_cast<int>(q->tokens);
   a.heads = static_cast<int>(q->heads);
