@@ -41,7 +41,7 @@ constexpr int kUnit = 32;  // keys per unit: a warp's share of a round
 // A CTA takes at least this many units: fewer would cost more in the join of
 // the partial results than the spread over more SMs gives back.
 constexpr int kMinUnits = 4;
-constexpr int kItemUnits = 8;  // what an item costs beside its keys, in units
+constexpr int kItemUnits = 16;  // what an item costs beside its keys, in units
 constexpr int kTop = 14;       // queries and weights are below 2^kTop in 16 bits
 // fp16: second parts, at most 2^(kTop - 11), are held times 2^kLow
 constexpr int kLow = 12;
@@ -116,6 +116,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(on ? 16 : 0)
                : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0)
@@ -203,40 +206,62 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
     if ((S::KS == 32 || lane < S::KS) && j <= ld.un.hi && (j >= ld.un.lo || j < a.sinks))
       entry = entry_of(a, ld.b, j);
   };
+  // Strides in pieces of 16 bytes (scales: elements) fit 32 bits, so a row's
+  // address is two 32 x 32 -> 64 bit products.
+  const int r0 = lane / S::LPR, c = lane % S::LPR;  // row and piece of this lane's loads
+  constexpr int RPI = 32 / S::LPR, N = S::KS / RPI;  // rows per load, loads
+  const bool in = S::LPR == S::CHUNKS || c < S::CHUNKS;
+  const uint32_t kp16 = static_cast<uint32_t>(a.k.page * S::ES >> 4);
+  const uint32_t kt16 = static_cast<uint32_t>(a.k.token * S::ES >> 4);
+  const uint32_t vp16 = static_cast<uint32_t>(a.v.page * S::ES >> 4);
+  const uint32_t vt16 = static_cast<uint32_t>(a.v.token * S::ES >> 4);
+  auto wide = [](uint32_t x, uint32_t y) { return static_cast<uint64_t>(x) * y; };
   auto issue = [&](int stage) {
     if (more) {
       const int key0 = ld.key(ld_u) + ld_s * S::KS, head = ld.head;
       const int pg = valid_page(a, entry);
       const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0);
-      uint8_t* st = ring + stage * S::STAGE;
       const uint32_t dst = ring_s + stage * S::STAGE;
       if (lane == 0)
-        *reinterpret_cast<uint2*>(st + 2 * S::HALF + S::SCALES) =
+        *reinterpret_cast<uint2*>(ring + stage * S::STAGE + 2 * S::HALF + S::SCALES) =
             make_uint2(there, static_cast<uint32_t>(key0));
-      const int r0 = lane / S::LPR, c = lane % S::LPR;
-      constexpr int RPI = 32 / S::LPR, N = S::KS / RPI;  // rows per load, loads
-      const bool in = S::LPR == S::CHUNKS || c < S::CHUNKS;
+      const uint8_t* kh = a.k.data + head * a.k.head * S::ES + c * 16;
+      const uint8_t* vh = a.v.data + head * a.v.head * S::ES + c * 16;
       if (halves) {
         // addresses advance by constants within a page
-        const int64_t dk = a.k.token * (RPI * S::ES), dv = a.v.token * (RPI * S::ES);
+        const uint64_t dk = static_cast<uint64_t>(kt16) * (RPI * 16);
+        const uint64_t dv = static_cast<uint64_t>(vt16) * (RPI * 16);
 #pragma unroll
         for (int h = 0; h < S::KS / 16; ++h) {
           const uint32_t bits = there >> (16 * h) & 0xffffu;
-          const int p0 = __shfl_sync(0xffffffffu, pg, 16 * h + max(__ffs(bits) - 1, 0));
-          const int64_t pp = bits ? p0 : 0;
-          const int off = page_offset(a, key0 + 16 * h) + r0;
-          const uint8_t* pk = a.k.data + (pp * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16;
-          const uint8_t* pv = a.v.data + (pp * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16;
-#pragma unroll
-          for (int i = 0; i < N * 16 / S::KS; ++i) {
-            const int r = 16 * h + r0 + i * RPI;
-            const bool on = there >> r & 1u;
+          const uint32_t p0 = __shfl_sync(0xffffffffu, pg, 16 * h + max(__ffs(bits) - 1, 0));
+          const uint32_t off = page_offset(a, key0 + 16 * h) + r0;
+          const uint32_t d0 = dst + 16 * h * S::RS;  // (place() repeats every eight rows)
+          if (bits == 0xffffu) {
+            const uint8_t* pk = kh + ((wide(p0, kp16) + wide(off, kt16)) << 4);
+            const uint8_t* pv = vh + ((wide(p0, vp16) + wide(off, vt16)) << 4);
             if (in) {
-              cp16(dst + place<C, D>(r, c), on ? pk : a.k.data, on);
-              cp16(dst + S::HALF + place<C, D>(r, c), on ? pv : a.v.data, on);
+#pragma unroll
+              for (int i = 0; i < N * 16 / S::KS; ++i) {
+                const uint32_t to = place<C, D>(r0 + i * RPI, c);
+                cp16(d0 + to, pk + i * dk);
+                cp16(d0 + S::HALF + to, pv + i * dv);
+              }
             }
-            pk += dk;
-            pv += dv;
+          } else {
+            const uint32_t pp = bits ? p0 : 0;
+            const uint8_t* pk = kh + ((wide(pp, kp16) + wide(off, kt16)) << 4);
+            const uint8_t* pv = vh + ((wide(pp, vp16) + wide(off, vt16)) << 4);
+#pragma unroll
+            for (int i = 0; i < N * 16 / S::KS; ++i) {
+              const int r = r0 + i * RPI;
+              const bool on = bits >> r & 1u;
+              const uint32_t to = place<C, D>(r, c);
+              if (in) {
+                cp16(d0 + to, on ? pk + i * dk : a.k.data, on);
+                cp16(d0 + S::HALF + to, on ? pv + i * dv : a.v.data, on);
+              }
+            }
           }
         }
       } else {
@@ -245,25 +270,25 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
         for (int i = 0; i < N; ++i) {
           const int r = r0 + i * RPI;
           const int pr = __shfl_sync(0xffffffffu, pg, r);
-          const int off = __shfl_sync(0xffffffffu, my_off, r);
+          const uint32_t off = __shfl_sync(0xffffffffu, my_off, r);
           const bool on = pr >= 0;
-          const int64_t p = on ? pr : 0;
+          const uint32_t p = on ? pr : 0;
           if (in) {
-            cp16(dst + place<C, D>(r, c),
-                 a.k.data + (p * a.k.page + off * a.k.token + head * a.k.head) * S::ES + c * 16, on);
-            cp16(dst + S::HALF + place<C, D>(r, c),
-                 a.v.data + (p * a.v.page + off * a.v.token + head * a.v.head) * S::ES + c * 16, on);
+            cp16(dst + place<C, D>(r, c), kh + ((wide(p, kp16) + wide(off, kt16)) << 4), on);
+            cp16(dst + S::HALF + place<C, D>(r, c), vh + ((wide(p, vp16) + wide(off, vt16)) << 4), on);
           }
         }
       }
       if constexpr (C::kInt8) {
         const bool on = pg >= 0;
-        const int64_t p = on ? pg : 0;
-        const int off = on ? page_offset(a, key0 + lane) : 0;
+        const uint32_t p = on ? pg : 0;
+        const uint32_t off = on ? page_offset(a, key0 + lane) : 0;
         cp4(dst + 2 * S::HALF + lane * 4,
-            a.k.scales + p * a.k.spage + off * a.k.stoken + head * a.k.shead, on);
+            a.k.scales + head * a.k.shead + wide(p, static_cast<uint32_t>(a.k.spage)) +
+                wide(off, static_cast<uint32_t>(a.k.stoken)), on);
         cp4(dst + 2 * S::HALF + S::KS * 4 + lane * 4,
-            a.v.scales + p * a.v.spage + off * a.v.stoken + head * a.v.shead, on);
+            a.v.scales + head * a.v.shead + wide(p, static_cast<uint32_t>(a.v.spage)) +
+                wide(off, static_cast<uint32_t>(a.v.stoken)), on);
       }
       if (++ld_s == SPU) {
         ld_s = 0;

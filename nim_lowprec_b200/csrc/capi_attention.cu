@@ -41,6 +41,13 @@ int check_cache(const lp_kv_cache* c) {
   if (!c->k || !c->v) return LP_ERR_ARG;
   if (c->dtype == LP_I8 && (!c->k_scales || !c->v_scales)) return LP_ERR_ARG;
   const int64_t es = elem_size(c->dtype);
+  for (int i = 0; i < 3; ++i) {  // not negative, and their kernels' units fit 32 bits
+    LP_REQUIRE(c->k_strides[i] >= 0 && c->k_strides[i] * es / 16 <= kIntMax);
+    LP_REQUIRE(c->v_strides[i] >= 0 && c->v_strides[i] * es / 16 <= kIntMax);
+    if (c->dtype != LP_I8) continue;
+    LP_REQUIRE(c->k_scale_strides[i] >= 0 && c->k_scale_strides[i] <= kIntMax);
+    LP_REQUIRE(c->v_scale_strides[i] >= 0 && c->v_scale_strides[i] <= kIntMax);
+  }
   uint64_t al = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v);
   for (int i = 0; i < 3; ++i)
     al |= static_cast<uint64_t>(c->k_strides[i] * es) | static_cast<uint64_t>(c->v_strides[i] * es);
