@@ -34,10 +34,20 @@ class _CacheStruct(ctypes.Structure):  # lp_kv_cache
                 ("dtype", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
 
 
-class _RowsStruct(ctypes.Structure):  # lp_rows
-    _fields_ = [("data", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("heads", ctypes.c_int64),
-                ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
-                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+_binding = None
+
+
+def _fast():
+    """The compiled argument checks and calls (csrc/torch_binding.cpp)."""
+    global _binding
+    if _binding is None:
+        try:
+            from . import _torch_binding
+        except ImportError as e:
+            raise ImportError("nim_lowprec_b200/_torch_binding.so is missing or was built for another "
+                              "torch: build it with `python nim_lowprec_b200/build.py`") from e
+        _binding = _torch_binding
+    return _binding
 
 
 def _cuda(t, name):
@@ -88,6 +98,8 @@ class KVCache:
         self._index = k.device.index
         self._struct = s
         self._ref = ctypes.addressof(s)
+        self._dim = s.head_dim
+        self._scale = s.head_dim ** -0.5 if s.head_dim else 1.0
 
     @classmethod
     def allocate(cls, pages, pageSize, kvHeads, headDim, dtype, device="cuda"):
@@ -108,54 +120,6 @@ class KVCache:
     headDim = property(lambda s: s._struct.head_dim)
 
 
-def _rows(t, name, dim, device):
-    """lp_rows of a [tokens, heads, dim] tensor; the last dimension contiguous."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise TypeError(f"{name}: expected a tensor on {device}")
-    dt = _ROW_TYPES.get(t.dtype)
-    if dt is None:
-        raise TypeError(f"{name}: expected fp32, fp16 or bf16, got {t.dtype}")
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != dim:
-        raise AssertionError(f"{name}: [tokens, heads, {dim}] expected, got {tuple(shape)}")
-    st = t.stride()
-    if st[2] != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    return _RowsStruct(t.data_ptr(), shape[0], shape[1], st[0], st[1], dt, 0)
-
-
-def _ints(t, name, dtype, device):
-    """Pointer and length of a contiguous vector of whole numbers."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
-        raise TypeError(f"{name}: expected {dtype} on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: tensors must be contiguous")
-    return t.data_ptr(), t.numel()
-
-
-def _table(t, requests, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
-        raise TypeError(f"blockTables: expected int32 on {device}")
-    shape, st = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] != requests:
-        raise AssertionError(f"blockTables: [{requests}, pages] expected, got {tuple(shape)}")
-    if shape[1] > 1 and st[1] != 1:
-        raise ValueError("blockTables: rows must be contiguous")
-    # (torch gives a one-row or empty tensor any stride)
-    return t.data_ptr(), shape[1], st[0] if requests > 1 else shape[1]
-
-
-def _launch(index, name, *args):
-    """The call on the current stream of the tensors' device."""
-    if index == torch.cuda.current_device():
-        st = getattr(N.lib(), name)(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(index):
-            st = getattr(N.lib(), name)(*args, torch.cuda.current_stream().cuda_stream)
-    if st:
-        N.check(st, name[3:])
-
-
 def assignPages(ctxLens, newLens, pageSize, freePages, freeHead, blockTables, qStart, seqLens,
                 slots, positions, freeHeadOut):
     """Page tables and slot maps from request lengths, on the GPU (lp_assign_pages).
@@ -166,37 +130,27 @@ def assignPages(ctxLens, newLens, pageSize, freePages, freeHead, blockTables, qS
     token its slot (int64) and position; -1 past the last token and where there is no page.
     freeHeadOut[0] is the next free entry; it must be another tensor than freeHead.
     positions may be None.  Whole numbers are int32, slots int64."""
-    dev = _cuda(ctxLens, "ctxLens").device
-    i32 = torch.int32
-    ctx, n = _ints(ctxLens, "ctxLens", i32, dev)
-    for t, name in ((freeHead, "freeHead"), (freeHeadOut, "freeHeadOut")):
-        if _ints(t, name, i32, dev)[1] != 1:
-            raise AssertionError(f"{name}: one element expected")
-    pos = (None, 0) if positions is None else _ints(positions, "positions", i32, dev)
-    _launch(dev.index, "lp_assign_pages", ctx, n, *_ints(newLens, "newLens", i32, dev),
-            int(pageSize), *_ints(freePages, "freePages", i32, dev), freeHead.data_ptr(),
-            *_table(blockTables, n, dev), *_ints(qStart, "qStart", i32, dev),
-            *_ints(seqLens, "seqLens", i32, dev), *_ints(slots, "slots", torch.int64, dev),
-            *pos, freeHeadOut.data_ptr())
+    status = _fast().assign_pages(ctxLens, newLens, pageSize, freePages, freeHead, blockTables, qStart,
+                                  seqLens, slots, positions, freeHeadOut)
+    if status:
+        N.check(status, "assignPages")
 
 
 def storeKV(cache, k, v, slots):
     """Write k and v [tokens, kvHeads, headDim] (fp32, fp16, bf16; any strides but the last) to
     their slots (lp_store_kv).  A token whose slot is outside the cache is skipped.  int8 pages
     take the codes and scales of calibrateSymmetric and quantizeBatch over each row."""
-    dev, dim = cache.device, cache._struct.head_dim
-    kr, vr = _rows(k, "k", dim, dev), _rows(v, "v", dim, dev)
-    _launch(cache._index, "lp_store_kv", cache._ref, ctypes.addressof(kr), ctypes.addressof(vr),
-            *_ints(slots, "slots", torch.int64, dev))
+    status = _fast().store_kv(cache._ref, cache._index, cache._dim, k, v, slots)
+    if status:
+        N.check(status, "storeKV")
 
 
 def loadKV(cache, slots, k, v):
     """Read the rows at `slots` back into k and v (lp_load_kv); zeros where a slot is outside
     the cache."""
-    dev, dim = cache.device, cache._struct.head_dim
-    kr, vr = _rows(k, "k", dim, dev), _rows(v, "v", dim, dev)
-    _launch(cache._index, "lp_load_kv", cache._ref,
-            *_ints(slots, "slots", torch.int64, dev), ctypes.addressof(kr), ctypes.addressof(vr))
+    status = _fast().load_kv(cache._ref, cache._index, cache._dim, k, v, slots)
+    if status:
+        N.check(status, "loadKV")
 
 
 def attentionWorkspace(device=None):
@@ -224,26 +178,13 @@ def pagedAttention(cache, blockTables, qStart, seqLens, q, out, scale=None, wind
 
     Without `workspace` one is kept per device and stream; pass your own
     (attentionWorkspace()) to graphs that may be replayed on other streams."""
-    dev, index, dim = cache.device, cache._index, cache._struct.head_dim
-    qr, orr = _rows(q, "q", dim, dev), _rows(out, "out", dim, dev)
-    seq, n = _ints(seqLens, "seqLens", torch.int32, dev)
-    if lse is None:
-        lp, ln = None, 0
-    else:
-        if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.device != dev:
-            raise TypeError(f"lse: expected fp32 on {dev}")
-        if not lse.is_contiguous():
-            raise ValueError("lse: tensors must be contiguous")
-        lp, ln = lse.data_ptr(), lse.numel()
+    fast, index = _fast(), cache._index
     if workspace is None:
-        key = (index, torch.cuda.current_stream(dev).cuda_stream)
+        key = (index, fast.current_stream(index))
         workspace = _workspaces.get(key)
         if workspace is None:
-            workspace = _workspaces[key] = attentionWorkspace(dev)
-    elif not isinstance(workspace, torch.Tensor) or workspace.device != dev or \
-            workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise TypeError(f"workspace: expected attentionWorkspace() of {dev}")
-    _launch(index, "lp_paged_attention", cache._ref, *_table(blockTables, n, dev),
-            *_ints(qStart, "qStart", torch.int32, dev), seq, n, ctypes.addressof(qr),
-            ctypes.addressof(orr), dim ** -0.5 if scale is None else float(scale), int(window),
-            int(sinks), lp, ln, workspace.data_ptr(), workspace.numel())
+            workspace = _workspaces[key] = attentionWorkspace(cache.device)
+    status = fast.paged_attention(cache._ref, index, cache._dim, blockTables, qStart, seqLens, q, out,
+                                  cache._scale if scale is None else scale, window, sinks, lse, workspace)
+    if status:
+        N.check(status, "pagedAttention")

@@ -7,7 +7,9 @@
 Every .cu under csrc/ is compiled for `sm_100a` only (the library uses
 tcgen05/TMA-era PTX: bulk copies, mbarrier waits, f32x2 arithmetic) and
 linked into one shared object next to this file, with the CUDA runtime linked
-statically.  The result travels with the repository snapshot; nothing is
+statically.  Where torch is installed, csrc/torch_binding.cpp becomes the
+CPython module _torch_binding beside it (the paged cache's entry points for
+torch tensors).  The result travels with the repository snapshot; nothing is
 installed into site-packages.
 """
 from __future__ import annotations
@@ -32,6 +34,32 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # reference's -ffp-contract=off (simd/dequant.nim:36).
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
          "--expt-relaxed-constexpr", "-I", CSRC, "-I", INCLUDE]
+
+
+BINDING = os.path.join(HERE, "_torch_binding.so")
+
+
+def build_binding(force: bool = False) -> None:
+    """_torch_binding.so against the installed torch (skipped without torch)."""
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    if not force and not _stale(BINDING, [src, OUT, os.path.join(INCLUDE, "lowprec_cuda.h")]):
+        return
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        return
+    import sysconfig
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = [INCLUDE, os.path.join(cuda, "include"), sysconfig.get_paths()["include"],
+           *cpp_extension.include_paths()]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{i}" for i in inc), src, "-o", BINDING, f"-L{HERE}", f"-L{lib}",
+           "-l:" + os.path.basename(OUT), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True)
 
 
 def sources():
@@ -62,6 +90,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(OUT, objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", OUT, *objs, "-ldl"]
         subprocess.run(cmd, check=True)
+    build_binding(force)
     return OUT
 
 

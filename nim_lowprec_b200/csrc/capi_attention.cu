@@ -58,6 +58,8 @@ int check_rows(const lp_rows* r, int64_t heads) {
   if (!r) return LP_ERR_ARG;
   if (r->dtype != LP_F32 && r->dtype != LP_F16 && r->dtype != LP_BF16) return LP_ERR_ARG;
   LP_REQUIRE(r->tokens >= 0 && r->tokens <= kIntMax && r->heads == heads);
+  LP_REQUIRE(r->token_stride >= 0 && r->token_stride <= kIntMax);
+  LP_REQUIRE(r->head_stride >= 0 && r->head_stride <= kIntMax);
   return bad(r->data, r->tokens) ? LP_ERR_ARG : LP_OK;
 }
 

@@ -159,30 +159,46 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const AssignArg
 
 // --------------------------------------------------- storeKV and loadKV
 //
-// One group of 8, 16 or 32 lanes per (token, head), 8 elements per lane, the
-// key's and the value's row together.  Bytes bound both: each is read and
-// written once, in 16- and 32-byte pieces, two rows in flight per thread.
+// One group of lanes per (token, head), 8 elements per lane (16 into an int8
+// cache, whose arithmetic would otherwise bound it; 4 into fp32), the key's and the value's
+// row together.  Bytes bound both: each is read and written once.
 // int8 rows take calibrateSymmetric's scale over the row (the largest
 // magnitude / 127, 1 for a zero row; quant.nim:95-110) and quantizeBatch's
 // code (divide, round half away from zero; quant.nim:48-60), by the same
 // IEEE operations, so the cache's bytes equal the two calls'.
 constexpr int kRowThreads = 256;
 
+// Numbers of tokens, heads and pages, and the strides (checked at the call),
+// fit 32 bits, so an offset is a sum of 32 x 32 -> 64 bit products.
+__device__ __forceinline__ int64_t wide(uint32_t a, uint32_t b) {
+  return static_cast<int64_t>(static_cast<uint64_t>(a) * b);
+}
 struct RowPtr {
   const uint8_t* p;
-  int64_t token, head;  // in elements
+  uint32_t token, head;  // in elements
+  __device__ __forceinline__ int64_t at(uint32_t t, uint32_t h) const {
+    return wide(t, token) + wide(h, head);
+  }
 };
 struct PoolPtr {
   uint8_t* p;
   float* scales;
-  int64_t page, token, head, spage, stoken, shead;
+  uint32_t page, token, head;     // in pieces of 16 bytes
+  uint32_t spage, stoken, shead;  // in elements
+  template <int T>
+  __device__ __forceinline__ uint8_t* at(uint32_t pg, uint32_t off, uint32_t h) const {
+    return p + ((wide(pg, page) + wide(off, token) + wide(h, head)) << 4);
+  }
+  __device__ __forceinline__ float* scale(uint32_t pg, uint32_t off, uint32_t h) const {
+    return scales + wide(pg, spage) + wide(off, stoken) + wide(h, shead);
+  }
 };
 struct RowsArgs {
   RowPtr k, v;      // storeKV reads, loadKV writes
   PoolPtr kc, vc;
   const int64_t* slots;
   int64_t items;    // tokens * heads
-  int heads, dim, page_size;
+  int heads, dim, page_size, page_shift;
   int64_t slots_end;  // pages * page_size
 };
 
@@ -209,11 +225,6 @@ __device__ __forceinline__ void load8(float* x, const uint8_t* p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = __ldg(reinterpret_cast<const float*>(p) + i);
     }
-  } else if constexpr (T == LP_I8) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = static_cast<float>(static_cast<int8_t>(((i < 4 ? u.x : u.y) >> (8 * (i & 3))) & 255u));
   } else {
     uint32_t w[4];
     if constexpr (VEC) {
@@ -234,6 +245,43 @@ __device__ __forceinline__ void load8(float* x, const uint8_t* p) {
         x[2 * i] = __uint_as_float(w[i] << 16);
         x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
+    }
+  }
+}
+
+__device__ __forceinline__ void load16_i8(float* x, const uint8_t* p) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    x[i] = static_cast<float>(static_cast<int8_t>((w[i >> 2] >> (8 * (i & 3))) & 255u));
+}
+
+// N elements of a cache row, N * size bytes aligned to themselves, 16 at most.
+template <int T, int N>
+__device__ __forceinline__ void load_cache(float* x, const uint8_t* p) {
+  if constexpr (T == LP_I8 && N == 16) {
+    load16_i8(x, p);
+  } else if constexpr (T != LP_I8 && N == 8) {
+    load8<T, true>(x, p);
+  } else {
+    constexpr int B = N * (T == LP_I8 ? 1 : 2);
+    static_assert(B == 4 || B == 8, "");
+    uint32_t w[2];
+    if constexpr (B == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = u.x, w[1] = u.y;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (T == LP_I8)
+        x[i] = static_cast<float>(static_cast<int8_t>((w[i >> 2] >> (8 * (i & 3))) & 255u));
+      else if constexpr (T == LP_F16)
+        x[i] = h2f(w[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+      else
+        x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
     }
   }
 }
@@ -266,94 +314,147 @@ __device__ __forceinline__ void store8(uint8_t* p, const float* x) {
 
 constexpr int size_of(int t) { return t == LP_F32 ? 4 : t == LP_I8 ? 1 : 2; }
 
-template <int L>
+// Codes of x / s, rounded half away from zero, four to a word.  The quotient is exact where it decides something.  x * (1 / s) is off by at most
+// 2^-22 of 127, so a result further than 2^-14 from the middle between two
+// whole numbers rounds as the quotient does; others (and what is not finite)
+// are divided.  (Sixteen divisions a thread took three times the bytes' time.)
+template <int N>
+__device__ __forceinline__ void codes(uint32_t* w, const float* x, float s) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the whole number
+  const float inv = __fdiv_rn(1.0f, s);
+  bool sure = true;
+  uint32_t q[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = fmul(x[i], inv);
+    const float z = fadd(y, kMagic);
+    q[i] = __float_as_uint(z);
+    sure = sure && fabsf(fadd(y, -fadd(z, -kMagic))) < 0.5f - 6.1e-5f;  // (not for a NaN)
+  }
+  if (!sure) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      q[i] = static_cast<uint32_t>(
+          static_cast<int>(fminf(fmaxf(roundf(__fdiv_rn(x[i], s)), -128.0f), 127.0f)));
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    w[i] = prmt(prmt(q[4 * i], q[4 * i + 1], 0x0040u), prmt(q[4 * i + 2], q[4 * i + 3], 0x0040u), 0x5410u);
+}
+
+// A lane's N elements of a row, of which L lanes hold one.
+template <int L, int N>
 __device__ __forceinline__ void store_i8(uint8_t* p, float* scale, const float* x, bool active,
                                          bool write_scale) {
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float s = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
-  uint32_t w[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float r = fminf(fmaxf(roundf(__fdiv_rn(x[i], s)), -128.0f), 127.0f);
-    w[i >> 2] |= (static_cast<uint32_t>(static_cast<int>(r)) & 255u) << (8 * (i & 3));
-  }
-  if (active) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  uint32_t w[N / 4];
+  codes<N>(w, x, s);
+  if (active) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   if (write_scale) *scale = s;
 }
 
-// X: type of the rows, T: type of the cache, L: lanes per row
-template <int X, int T, int L, bool VEC, bool STORE>
+// X: type of the rows, T: type of the cache, L: lanes per row of N elements each
+template <int X, int T, int L, int N, bool VEC, bool STORE>
 __global__ void __launch_bounds__(kRowThreads) k_rows(const RowsArgs a) {
   const int sub = threadIdx.x & (L - 1);
-  const bool lane_in = sub * 8 < a.dim;
+  const bool lane_in = sub * N < a.dim;
   const int64_t groups = static_cast<int64_t>(gridDim.x) * (kRowThreads / L);
   const int64_t g0 = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) / L;
   // whole warps run the same number of rounds: the row's maximum meets by shuffles
   const int64_t w0 = g0 - ((threadIdx.x & 31) / L);
-  for (int64_t r = 0; w0 + r * groups < a.items; ++r) {
-    const int64_t i = g0 + r * groups;
+  for (int64_t r = 0; w0 + r < a.items; r += groups) {
+    const int64_t i = g0 + r;
     const bool in = i < a.items;
-    const int64_t t = in ? i / a.heads : 0;
-    const int h = in ? static_cast<int>(i - t * a.heads) : 0;
+    // (64-bit divisions only where 32 bits do not hold the number)
+    const uint32_t t = !in ? 0
+                       : a.items >> 32 ? static_cast<uint32_t>(i / a.heads)
+                                       : static_cast<uint32_t>(i) / static_cast<uint32_t>(a.heads);
+    const uint32_t h = in ? static_cast<uint32_t>(i - static_cast<int64_t>(t) * a.heads) : 0;
     const int64_t slot = in ? __ldg(a.slots + t) : -1;
+    const int64_t kr = a.k.at(t, h) + sub * N, vr = a.v.at(t, h) + sub * N;
+    float x[N] = {}, y[N] = {};
+    if constexpr (STORE) {  // the rows do not wait for the slots
+      if (in && lane_in) {
+#pragma unroll
+        for (int b = 0; b < N; b += 8) {
+          load8<X, VEC>(x + b, a.k.p + (kr + b) * size_of(X));
+          load8<X, VEC>(y + b, a.v.p + (vr + b) * size_of(X));
+        }
+      }
+    }
     const bool there = slot >= 0 && slot < a.slots_end;
     const bool on = in && lane_in && there;
-    const int64_t page = there ? slot / a.page_size : 0, off = there ? slot - page * a.page_size : 0;
-    const int64_t ko = page * a.kc.page + off * a.kc.token + h * a.kc.head + sub * 8;
-    const int64_t vo = page * a.vc.page + off * a.vc.token + h * a.vc.head + sub * 8;
-    const int64_t ks = page * a.kc.spage + off * a.kc.stoken + h * a.kc.shead;
-    const int64_t vs = page * a.vc.spage + off * a.vc.stoken + h * a.vc.shead;
-    const int64_t kr = t * a.k.token + h * a.k.head + sub * 8;
-    const int64_t vr = t * a.v.token + h * a.v.head + sub * 8;
-    float x[8] = {}, y[8] = {};
+    const int64_t sl = there ? slot : 0;
+    const uint32_t page = static_cast<uint32_t>(a.page_shift >= 0 ? sl >> a.page_shift : sl / a.page_size);
+    const uint32_t off = static_cast<uint32_t>(sl - static_cast<int64_t>(page) * a.page_size);
+    uint8_t* kp = a.kc.template at<T>(page, off, h) + sub * (N * size_of(T));
+    uint8_t* vp = a.vc.template at<T>(page, off, h) + sub * (N * size_of(T));
     if constexpr (STORE) {
-      if (on) {
-        load8<X, VEC>(x, a.k.p + kr * size_of(X));
-        load8<X, VEC>(y, a.v.p + vr * size_of(X));
-      }
       if constexpr (T == LP_I8) {
-        store_i8<L>(a.kc.p + ko, a.kc.scales + ks, x, on, on && sub == 0);
-        store_i8<L>(a.vc.p + vo, a.vc.scales + vs, y, on, on && sub == 0);
+        store_i8<L, N>(kp, a.kc.scale(page, off, h), x, on, on && sub == 0);
+        store_i8<L, N>(vp, a.vc.scale(page, off, h), y, on, on && sub == 0);
       } else if (on) {
-        store8<T, true>(a.kc.p + ko * 2, x);
-        store8<T, true>(a.vc.p + vo * 2, y);
+        store8<T, true>(kp, x);
+        store8<T, true>(vp, y);
       }
     } else {
       if (on) {
-        load8<T, true>(x, a.kc.p + ko * size_of(T));
-        load8<T, true>(y, a.vc.p + vo * size_of(T));
+        load_cache<T, N>(x, kp);
+        load_cache<T, N>(y, vp);
         if constexpr (T == LP_I8) {
-          const float sk = __ldg(a.kc.scales + ks), sv = __ldg(a.vc.scales + vs);
+          const float sk = __ldg(a.kc.scale(page, off, h)), sv = __ldg(a.vc.scale(page, off, h));
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = fmul(x[j], sk), y[j] = fmul(y[j], sv);
+          for (int j = 0; j < N; ++j) x[j] = fmul(x[j], sk), y[j] = fmul(y[j], sv);
         }
       }
       if (in && lane_in) {  // no row at this slot: zeros
-        store8<X, VEC>(const_cast<uint8_t*>(a.k.p) + kr * size_of(X), x);
-        store8<X, VEC>(const_cast<uint8_t*>(a.v.p) + vr * size_of(X), y);
+        uint8_t* ko = const_cast<uint8_t*>(a.k.p) + kr * size_of(X);
+        uint8_t* vo = const_cast<uint8_t*>(a.v.p) + vr * size_of(X);
+        if constexpr (N == 4) {  // (fp32 rows)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if constexpr (VEC) break;
+            reinterpret_cast<float*>(ko)[b] = x[b];
+            reinterpret_cast<float*>(vo)[b] = y[b];
+          }
+          if constexpr (VEC) {
+            *reinterpret_cast<float4*>(ko) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(vo) = make_float4(y[0], y[1], y[2], y[3]);
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < N; b += 8) {
+            store8<X, VEC>(ko + b * size_of(X), x + b);
+            store8<X, VEC>(vo + b * size_of(X), y + b);
+          }
+        }
       }
     }
   }
 }
 
-template <int X, int T, int L, bool STORE>
+template <int X, int T, int L, int N, bool STORE>
 int launch_rows_l(const RowsArgs& a, bool vec, cudaStream_t st) {
   const int64_t blocks = (a.items + kRowThreads / L - 1) / (kRowThreads / L);
   const int grid = static_cast<int>(std::min<int64_t>(blocks, device_info().sm_count * 32ll));
-  if (vec) k_rows<X, T, L, true, STORE><<<grid, kRowThreads, 0, st>>>(a);
-  else k_rows<X, T, L, false, STORE><<<grid, kRowThreads, 0, st>>>(a);
+  if (vec) k_rows<X, T, L, N, true, STORE><<<grid, kRowThreads, 0, st>>>(a);
+  else k_rows<X, T, L, N, false, STORE><<<grid, kRowThreads, 0, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
 template <int X, int T, bool STORE>
 int launch_rows_t(const RowsArgs& a, bool vec, cudaStream_t st) {
-  if (a.dim <= 64) return launch_rows_l<X, T, 8, STORE>(a, vec, st);
-  if (a.dim <= 128) return launch_rows_l<X, T, 16, STORE>(a, vec, st);
-  return launch_rows_l<X, T, 32, STORE>(a, vec, st);
+  // fp32 rows out: 4 elements, so that a warp writes whole lines
+  constexpr int N = STORE ? (T == LP_I8 ? 16 : 8) : X == LP_F32 ? 4 : 8;
+  if (a.dim <= 64) return launch_rows_l<X, T, 64 / N, N, STORE>(a, vec, st);
+  if (a.dim <= 128) return launch_rows_l<X, T, 128 / N, N, STORE>(a, vec, st);
+  constexpr int W = N == 4 ? 8 : N;  // (a row's lanes are in one warp)
+  return launch_rows_l<X, T, 256 / W, W, STORE>(a, vec, st);
 }
 
 template <int X, bool STORE>
@@ -372,17 +473,33 @@ int launch_rows(const RowsArgs& a, int type, int cache_type, bool vec, cudaStrea
 
 RowsArgs rows_args(const lp_kv_cache& c, const lp_rows& k, const lp_rows& v, const int64_t* slots) {
   RowsArgs a;
-  a.k = {static_cast<const uint8_t*>(k.data), k.token_stride, k.head_stride};
-  a.v = {static_cast<const uint8_t*>(v.data), v.token_stride, v.head_stride};
-  a.kc = {static_cast<uint8_t*>(c.k), c.k_scales,          c.k_strides[0],       c.k_strides[1],
-          c.k_strides[2],             c.k_scale_strides[0], c.k_scale_strides[1], c.k_scale_strides[2]};
-  a.vc = {static_cast<uint8_t*>(c.v), c.v_scales,          c.v_strides[0],       c.v_strides[1],
-          c.v_strides[2],             c.v_scale_strides[0], c.v_scale_strides[1], c.v_scale_strides[2]};
+  auto row = [](const lp_rows& r) {
+    return RowPtr{static_cast<const uint8_t*>(r.data), static_cast<uint32_t>(r.token_stride),
+                  static_cast<uint32_t>(r.head_stride)};
+  };
+  auto pool = [&](void* p, float* scales, const int64_t* s, const int64_t* ss) {
+    const int64_t es = c.dtype == LP_I8 ? 1 : 2;
+    PoolPtr o{static_cast<uint8_t*>(p), scales, 0, 0, 0, 0, 0, 0};
+    o.page = static_cast<uint32_t>(s[0] * es / 16);
+    o.token = static_cast<uint32_t>(s[1] * es / 16);
+    o.head = static_cast<uint32_t>(s[2] * es / 16);
+    o.spage = static_cast<uint32_t>(ss[0]);
+    o.stoken = static_cast<uint32_t>(ss[1]);
+    o.shead = static_cast<uint32_t>(ss[2]);
+    return o;
+  };
+  a.k = row(k);
+  a.v = row(v);
+  a.kc = pool(c.k, c.k_scales, c.k_strides, c.k_scale_strides);
+  a.vc = pool(c.v, c.v_scales, c.v_strides, c.v_scale_strides);
   a.slots = slots;
   a.items = k.tokens * c.kv_heads;
   a.heads = static_cast<int>(c.kv_heads);
   a.dim = c.head_dim;
   a.page_size = static_cast<int>(c.page_size);
+  a.page_shift = -1;  // log2 of the page size, where it is a power of two
+  for (int i = 0; i < 31; ++i)
+    if (c.page_size == int64_t{1} << i) a.page_shift = i;
   a.slots_end = c.pages * c.page_size;
   return a;
 }
