@@ -638,44 +638,31 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         const float* sk = C::kInt8 ? &scales->k[mm][col0] : nullptr;
         const float* sv = C::kInt8 ? &scales->v[mm][col0] : nullptr;
 
-        // Scores 32 .. of this thread's columns: int8 keys' scales and the mask
-        // are applied on each of the two reads (registers hold 64 of 128).
-        auto ready = [&](uint32_t* v, int h) {
-          tmem_wait_ld();
-          tie(v, 32);
-          if constexpr (C::kInt8) {
+        // ---- this thread's scores, with int8 keys' scales and the mask
+        uint32_t v[COLS];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(sk + 32 * h + e);
-              const uint64_t x = mul2(pku(v[e], v[e + 1]), k4.x);
-              const uint64_t y = mul2(pku(v[e + 2], v[e + 3]), k4.y);
-              upku(x, v[e], v[e + 1]);
-              upku(y, v[e + 2], v[e + 3]);
-            }
-          }
-          if (!full) {
+        for (int h = 0; h < COLS / 32; ++h) tmem_ld32(sc + 32 * h, v + 32 * h);
+        tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = see[h] >> e & 1u ? v[e] : 0xff800000u;
-          }
-        };
-        uint32_t va[32], vb[32];
-        // ---- the row's maximum; a chunk's read runs while the one before is used
-        float mx = -INFINITY, my = -INFINITY;
-        tmem_ld32(sc, va);
+        for (int h = 0; h < COLS / 32; ++h) tie(v + 32 * h, 32);
+        if constexpr (C::kInt8) {
 #pragma unroll
-        for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t* v = h & 1 ? vb : va;
-          ready(v, h);
-          tmem_ld32(sc + 32 * ((h + 1) % (COLS / 32)), h & 1 ? va : vb);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            mx = fmaxf(mx, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-            my = fmaxf(my, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
+          for (int e = 0; e < COLS; e += 4) {
+            const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(sk + e);
+            upku(mul2(pku(v[e], v[e + 1]), k4.x), v[e], v[e + 1]);
+            upku(mul2(pku(v[e + 2], v[e + 3]), k4.y), v[e + 2], v[e + 3]);
           }
         }
-        mx = fmaxf(mx, my);
-        tmem_wait_ld();  // the next pass's first chunk, which waits in registers
-        tie(va, 32);
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < COLS; ++e) v[e] = see[e / 32] >> (e % 32) & 1u ? v[e] : 0xff800000u;
+        }
+        // ---- the row's maximum
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < COLS; e += 2)
+          top[e / 2 % 4] = fmaxf(top[e / 2 % 4], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+        float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if constexpr (!kTwo) {
           sh.xmax[x][wg][row] = mx;  // (the buffer's last readers are two barriers back)
           named_bar(2, kSoftThreads);
@@ -688,35 +675,32 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         } else if (__any_sync(0xffffffffu, move)) {
           const float corr = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - mx) * c);
           wait_pv(slot - 1);
-          for (int d = d0; d < d1; d += 32) {
-            uint32_t v[32];
-            tmem_ld32(tm + o_col(tile) + d, v);
+          for (int d = d0; d < d1; d += 16) {
+            uint32_t u[16];  // (beside the scores in registers)
+            tmem_ld16(tm + o_col(tile) + d, u);
             tmem_wait_ld();
-            tie(v, 32);
+            tie(u, 16);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
-            tmem_st32(tm + o_col(tile) + d, v);
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * corr);
+            tmem_st16(tm + o_col(tile) + d, u);
           }
-          tmem_wait_st();
           l *= corr;
           if (move) m = mx;
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;
-        // ---- weights, times kUp (the first chunk is on its way since the last pass)
+        // ---- weights, times kUp
         const float up = F::NP == 1 ? F::kUpLog : 0.0f;
         const uint64_t c2 = pk(c, c), mc2 = pk(up - mc, up - mc);
         uint64_t la = 0, lb = 0;
 #pragma unroll
         for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t* v = h & 1 ? vb : va;
-          ready(v, h);
-          if (h + 1 < COLS / 32) tmem_ld32(sc + 32 * (h + 1), h & 1 ? va : vb);
           uint32_t p[F::NP][16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y0, y1;
-            upk(fma2(pku(v[2 * e], v[2 * e + 1]), c2, mc2), y0, y1);
-            uint64_t y = pk(ex2(y0), ex2(y1));
+            uint64_t y = fma2(pku(v[32 * h + 2 * e], v[32 * h + 2 * e + 1]), c2, mc2);
+            upk(y, y0, y1);
+            y = pk(ex2(y0), ex2(y1));
             // more than one part: 2^7 as a product, which rounds nothing
             if constexpr (F::NP > 1 && F::kUp != 1.0f) y = mul2(y, pk(F::kUp, F::kUp));
             uint64_t& sum = e & 1 ? lb : la;
@@ -936,15 +920,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
   // a wait that runs out sets sh.abort; the roles then run to their ends
   // without waiting, so no barrier is left short and tensor memory is freed
   if (w.at < w.end) {
-    // 128 registers a thread at launch: 2 x 176 + 104 + 56 = 4 x 128
+    // 128 registers a thread at launch: 2 x 200 + 64 + 48 = 4 x 128
     if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
       soft_role<F>(a, w, sh, scales, qs);
     } else if (warp < 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
       load_role<F>(a, w, sh, scales, ring, ring + F::STAGES * F::TILE);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
       if (warp == 12) mma_role<F>(a, w, sh, qs, ring);
     }
   }
