@@ -116,6 +116,12 @@ struct Cursor {
   int pad;
 };
 
+// (64-bit divisions are slow, and the numbers nearly always fit 32 bits)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if ((a | b) >> 32) return a / b;
+  return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
+
 // Total units and the item that holds unit `begin` of this CTA.  Each thread
 // sums a run of requests, the sums are scanned in shared memory, and the
 // thread whose run holds `begin` walks it.  All threads of the block call it.
@@ -142,7 +148,7 @@ __device__ void find_share(const Args& a, int64_t min_units, Cursor* cur, int64_
     total += sums[w];
   }
   const int64_t excl = before + inc - mine;
-  const int64_t per = max((total + gridDim.x - 1) / static_cast<int64_t>(gridDim.x), min_units);
+  const int64_t per = max(divide(total + gridDim.x - 1, gridDim.x), min_units);
   const int64_t begin = min(static_cast<int64_t>(blockIdx.x) * per, total);
   if (t == 0) {
     cur->begin = begin;
@@ -157,7 +163,7 @@ __device__ void find_share(const Args& a, int64_t min_units, Cursor* cur, int64_
       at += w * a.kv_heads;
       w = request_units<KU, RB, XU>(a, ++b);
     }
-    const int head = static_cast<int>((begin - at) / w);
+    const int head = static_cast<int>(divide(begin - at, w));
     at += head * w;
     const Request r = request(a, b);
     int block = 0;
@@ -236,7 +242,7 @@ struct Sharers {
   int first, last;
 };
 __device__ __forceinline__ Sharers sharers(int64_t u0, int64_t n, int64_t per) {
-  return {static_cast<int>(u0 / per), static_cast<int>((u0 + n - 1) / per)};
+  return {static_cast<int>(divide(u0, per)), static_cast<int>(divide(u0 + n - 1, per))};
 }
 __device__ __forceinline__ int slot_of(int cta, int64_t u0, int64_t per) {
   return 2 * cta + (u0 > static_cast<int64_t>(cta) * per ? 1 : 0);

@@ -55,9 +55,10 @@ constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroup
 constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
 constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
 constexpr int kMinUnits = 2;
-// What an item costs beside its keys, in key tiles: 8 us of queries, start and
-// outputs against 2 to 3 us per tile.
-constexpr int kItemUnits = 4;
+// What an item costs beside its keys, in key tiles (queries, start, outputs: 7 to
+// 13 us against 1.2 to 2.5 us per tile).  Five fp32 prompts over an int8 cache,
+// some of them short: 406 us with 2, 317 with 4, 311 with 7.
+constexpr int kItemUnits = 6;
 
 // C: the cache's format; Q: type of the operands of Q K^T, P: of P V;
 // NQ, NP: parts of queries and weights.
@@ -80,6 +81,12 @@ struct Cfg {
   static constexpr int META = C::kInt8 ? 6 : STAGES <= 4 ? 4 : 8;
   static constexpr int ROWS = 128 * TILES;
   static constexpr int SMEM = 1024 + TILES * NQ * TILE + STAGES * TILE + RAW * RAW_TILE;
+  // Registers per thread of the roles' warpgroups; 128 each at launch.  One row
+  // tile's softmax holds 64 scores and up to 64 outputs, two tiles' 128 scores.
+  static constexpr int SOFT_REGS = TILES == 2 ? 200 : 216;
+  static constexpr int LOAD_REGS = TILES == 2 ? 64 : 48;
+  static constexpr int MMA_REGS = TILES == 2 ? 48 : 32;
+  static_assert(2 * SOFT_REGS + LOAD_REGS + MMA_REGS == 4 * 128, "");
   // fp16 weights are held times 2^7, bf16 has the range without
   static constexpr float kUp = P::kBf16 ? 1.0f : 128.0f;
   static constexpr float kUpLog = P::kBf16 ? 0.0f : 7.0f;
@@ -723,13 +730,14 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         const float up = F::NP == 1 ? F::kUpLog : 0.0f;
         const uint64_t c2 = pk(c, c), mc2 = pk(up - mc, up - mc);
         uint64_t la = 0, lb = 0;
+        constexpr int PW = kTwo ? 16 : 8;  // pairs per store (registers)
 #pragma unroll
-        for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t p[F::NP][16];
+        for (int h = 0; h < COLS / (2 * PW); ++h) {
+          uint32_t p[F::NP][PW];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < PW; ++e) {
             float y0, y1;
-            uint64_t y = fma2(pku(v[32 * h + 2 * e], v[32 * h + 2 * e + 1]), c2, mc2);
+            uint64_t y = fma2(pku(v[2 * (PW * h + e)], v[2 * (PW * h + e) + 1]), c2, mc2);
             upk(y, y0, y1);
             y = pk(ex2(y0), ex2(y1));
             // more than one part: 2^7 as a product, which rounds nothing
@@ -737,7 +745,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
             uint64_t& sum = e & 1 ? lb : la;
             sum = add2(sum, y);
             if constexpr (C::kInt8)
-              y = mul2(y, *reinterpret_cast<const uint64_t*>(sv + 32 * h + 2 * e));
+              y = mul2(y, *reinterpret_cast<const uint64_t*>(sv + 2 * (PW * h + e)));
 #pragma unroll
             for (int q = 0; q < F::NP; ++q) {
               upk(y, y0, y1);
@@ -756,8 +764,12 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
           }
 #pragma unroll
           for (int q = 0; q < F::NP; ++q) {
-            const uint32_t to = q < 2 ? sc + 32 * h + 16 * q : tm + p3_col(x) + (col0 / 2) + 16 * h;
-            tmem_st16(to, p[q]);
+            // the part's columns begin those of the 32 scores they come from
+            const int at = 2 * PW * h;  // first score
+            const uint32_t to = q < 2 ? sc + at / 32 * 32 + at % 32 / 2 + 16 * q
+                                      : tm + p3_col(x) + (col0 + at) / 2;
+            if constexpr (kTwo) tmem_st16(to, p[q]);
+            else tmem_st8(to, p[q]);
           }
         }
         {
@@ -825,9 +837,9 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
           mine[(D + 1) * F::ROWS + r] = l;
         }
       }
-      __threadfence();
       named_bar(2, kSoftThreads);
       if (threadIdx.x == 0) {
+        __threadfence();  // (for the block's stores: they are before the barrier)
         const uint32_t n = static_cast<uint32_t>(ss.last - ss.first);
         sh.last = atomicInc(a.counters + ss.first, n) == n;
         __threadfence();
@@ -968,15 +980,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
   // a wait that runs out sets sh.abort; the roles then run to their ends
   // without waiting, so no barrier is left short and tensor memory is freed
   if (w.at < w.end) {
-    // 128 registers a thread at launch: 2 x 200 + 64 + 48 = 4 x 128
     if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::SOFT_REGS));
       soft_role<F>(a, w, sh, scales, qs);
     } else if (warp < 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::LOAD_REGS));
       load_role<F>(a, w, sh, scales, ring, ring + F::STAGES * F::TILE);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::MMA_REGS));
       if (warp == 12) mma_role<F>(a, w, sh, qs, ring);
     }
   }

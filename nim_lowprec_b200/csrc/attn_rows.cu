@@ -72,8 +72,10 @@ struct Shape {
   static constexpr int STAGES = 24576 / (2 * HALF);
   static constexpr int RING = STAGES * STAGE;
   static constexpr int SMEM = kWarps * RING + kWarps * kWarps * D * 4;
-  [[maybe_unused]] static constexpr int E = D % 64 == 0 ? 16 : 8;  // int8: elements per key read
 };
+
+// Elements of an int8 key that a lane reads at once.
+__device__ constexpr int key_read(int dim) { return dim % 64 == 0 ? 16 : 8; }
 
 // Where piece `c` of row `r` is.  16-bit rows: so that the eight rows of a
 // matrix read meet in no bank.  int8 rows of 128 bytes: so that neither reads
@@ -153,7 +155,7 @@ template <class C, int D>
 __device__ __forceinline__ int key_dim(int k, int c4, int i) {
   if constexpr (!C::kInt8) return k * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8;
   else {
-    constexpr int E = Shape<C, D>::E;
+    constexpr int E = key_read(D);
     return (k / (E / 4)) * 4 * E + c4 * E + (k % (E / 4)) * 4 + i;
   }
 }
@@ -397,13 +399,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
             }
           }
       } else {
-        constexpr int LW = S::E / 4;
+        constexpr int E = key_read(D), LW = E / 4;
 #pragma unroll
-        for (int x = 0; x < D / (4 * S::E); ++x)
+        for (int x = 0; x < D / (4 * E); ++x)
 #pragma unroll
           for (int n = 0; n < S::NG; ++n) {
             uint32_t kw[LW];
-            const int byte = x * 4 * S::E + c4 * S::E;
+            const int byte = x * 4 * E + c4 * E;
             lds_words<LW>(kw, st + place<C, D>(n * 8 + g8, byte >> 4) + (byte & 15));
 #pragma unroll
             for (int y = 0; y < LW; ++y) {
@@ -595,9 +597,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
     }
     // ---- an item of several CTAs: the one that arrives last joins the parts
     if (!alone) {
-      __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
+        __threadfence();  // (for the block's stores: they are before the barrier)
         const uint32_t n = static_cast<uint32_t>(sh.last - sh.first);
         s_last = atomicInc(a.counters + sh.first, n) == n;
         __threadfence();
@@ -605,25 +607,36 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
       __syncthreads();
       if (s_last) {
         for (int row = warp; row < rows; row += kWarps) {
-          // the parts' maxima and sums by lanes, then the outputs in CTA order
+          // in CTA order, four parts' loads on their way together
           float ro[DL], rm = -INFINITY, rl = 0.0f;
 #pragma unroll
           for (int i = 0; i < DL; ++i) ro[i] = 0.0f;
-          for (int x = sh.first + lane; x <= sh.last; x += 32)
-            rm = fmaxf(rm, __ldcg(a.partials + slot_of(x, w.item0, w.per) * static_cast<int64_t>(kSlot) +
-                                  kRows * D + row));
+          for (int x0 = sh.first; x0 <= sh.last; x0 += 4) {
+            float pm[4], pl[4], po[4][DL];
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) rm = fmaxf(rm, __shfl_xor_sync(0xffffffffu, rm, x));
-          const float ref = rm == -INFINITY ? 0.0f : rm;
-#pragma unroll 4
-          for (int x = sh.first; x <= sh.last; ++x) {
-            const float* other =
-                a.partials + slot_of(x, w.item0, w.per) * static_cast<int64_t>(kSlot);
-            const float f = ex2(__ldcg(other + kRows * D + row) - ref);
-            rl = fmaf(__ldcg(other + kRows * D + kRows + row), f, rl);
+            for (int y = 0; y < 4; ++y) {
+              const bool on = x0 + y <= sh.last;
+              const float* part = a.partials + slot_of(min(x0 + y, sh.last), w.item0, w.per) *
+                                                   static_cast<int64_t>(kSlot);
+              pm[y] = on ? __ldcg(part + kRows * D + row) : -INFINITY;
+              pl[y] = on ? __ldcg(part + kRows * D + kRows + row) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < DL; ++i)
-              ro[i] = fmaf(__ldcg(other + row * D + lane + 32 * i), f, ro[i]);
+              for (int i = 0; i < DL; ++i) po[y][i] = on ? __ldcg(part + row * D + lane + 32 * i) : 0.0f;
+            }
+            const float mn = fmaxf(fmaxf(rm, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3]));
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = ex2(rm - ref);
+            rl *= f;
+#pragma unroll
+            for (int i = 0; i < DL; ++i) ro[i] *= f;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float g = ex2(pm[y] - ref);
+              rl = fmaf(pl[y], g, rl);
+#pragma unroll
+              for (int i = 0; i < DL; ++i) ro[i] = fmaf(po[y][i], g, ro[i]);
+            }
+            rm = mn;
           }
           finish(row, ro, rm, rl);
         }
