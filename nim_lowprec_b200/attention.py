@@ -56,6 +56,11 @@ def _cuda(t, name):
     return t
 
 
+def _strides(t):
+    """Of pages, tokens and heads; a dimension of one may have any, and needs none."""
+    return _I3(*(st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride())))
+
+
 class KVCache:
     """Pages of keys and values, [pages, pageSize, kvHeads, headDim] each, in fp16, bf16 or
     int8.  The head dimension is contiguous; the other strides are free (a cache that keeps
@@ -80,7 +85,7 @@ class KVCache:
         s = _CacheStruct()
         s.k, s.v = k.data_ptr(), v.data_ptr()
         s.pages, s.page_size, s.kv_heads, s.head_dim = k.shape
-        s.k_strides, s.v_strides = _I3(*k.stride()[:3]), _I3(*v.stride()[:3])
+        s.k_strides, s.v_strides = _strides(k), _strides(v)
         s.dtype = _CACHE_TYPES[k.dtype]
         if int8:
             for t, name in ((kScales, "kScales"), (vScales, "vScales")):
@@ -91,8 +96,7 @@ class KVCache:
                 if t.device != k.device:
                     raise ValueError("scales on another device than the pages")
             s.k_scales, s.v_scales = kScales.data_ptr(), vScales.data_ptr()
-            s.k_scale_strides = _I3(*kScales.stride())
-            s.v_scale_strides = _I3(*vScales.stride())
+            s.k_scale_strides, s.v_scale_strides = _strides(kScales), _strides(vScales)
         self.k, self.v, self.kScales, self.vScales = k, v, kScales, vScales
         self.device = k.device
         self._index = k.device.index
@@ -183,6 +187,9 @@ def pagedAttention(cache, blockTables, qStart, seqLens, q, out, scale=None, wind
         key = (index, fast.current_stream(index))
         workspace = _workspaces.get(key)
         if workspace is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("pagedAttention: a captured call needs a workspace of its own "
+                                   "(attentionWorkspace(), made before the capture)")
             workspace = _workspaces[key] = attentionWorkspace(cache.device)
     status = fast.paged_attention(cache._ref, index, cache._dim, blockTables, qStart, seqLens, q, out,
                                   cache._scale if scale is None else scale, window, sinks, lse, workspace)

@@ -1,6 +1,6 @@
 // attn.cuh -- what the paged-attention kernels share: their arguments, the
-// split of the work over the grid, the visible keys of a row, and the exact
-// recomputation of a row whose sum is not finite.
+// split of the work over the grid, the visible keys of a row, and the care for
+// what masked keys hold.
 //
 // Work split.  The query rows of request b and key head h are the pairs (new
 // token t, query head g of the group), r = t * G + g, in blocks of RB rows.
@@ -294,71 +294,6 @@ __device__ __forceinline__ int page_of(const Args& a, int b, int j) {
   return valid_page(a, entry_of(a, b, j));
 }
 
-template <class C>
-__device__ __forceinline__ float cache_elem(const Pool& p, int64_t row, int64_t srow, int d) {
-  if constexpr (C::kInt8) {
-    return static_cast<float>(reinterpret_cast<const int8_t*>(p.data)[row + d]) * p.scales[srow];
-  } else {
-    return C::to_float(reinterpret_cast<const uint16_t*>(p.data)[row + d]);
-  }
-}
-
-// One query row by one warp, key by key over its visible keys alone, fp32.
-// The tiled kernels give masked keys the weight 0; a 0 times an infinity or a
-// NaN that a masked key's value holds is a NaN.  So a row that ends not
-// finite is computed again here, where masked keys are never read: it is
-// finite if the row's own keys are.
-template <class C, int D>
-__device__ __noinline__ void exact_row(const Args& a, int b, int head, int t, int g) {
-  const int lane = threadIdx.x & 31;
-  const Request r = request(a, b);
-  const int pos = r.base + t;
-  const int qh = head * a.group + g;
-  const int64_t qrow = (r.start + t) * a.q_token + qh * a.q_head;
-  float q[D / 32], o[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    q[i] = load_elem(a.q, a.q_type, qrow + lane + 32 * i);
-    o[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  const int end = min(pos + 1, r.limit);
-  const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-  for (int j = 0; j < end; ++j) {
-    if (j < lo && j >= a.sinks) j = lo;
-    if (j >= end) break;
-    const int page = page_of(a, b, j);
-    if (page < 0) continue;
-    const int off = page_offset(a, j);
-    const int64_t kr = page * a.k.page + off * a.k.token + head * a.k.head;
-    const int64_t ks = page * a.k.spage + off * a.k.stoken + head * a.k.shead;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      s = fmaf(q[i], cache_elem<C>(a.k, kr, ks, lane + 32 * i), s);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= a.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float ref = mn == -INFINITY ? 0.0f : mn;
-    const float c = ex2(m - ref), p = ex2(s - ref);
-    m = mn;
-    l = fmaf(l, c, p);
-    const int64_t vr = page * a.v.page + off * a.v.token + head * a.v.head;
-    const int64_t vs = page * a.v.spage + off * a.v.stoken + head * a.v.shead;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      o[i] = fmaf(o[i], c, p * cache_elem<C>(a.v, vr, vs, lane + 32 * i));
-  }
-  const int64_t orow = (r.start + t) * a.o_token + qh * a.o_head;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    store_elem(a.out, a.q_type, orow + lane + 32 * i, l == 0.0f ? 0.0f : __fdiv_rn(o[i], l));
-  if (a.lse && lane == 0)
-    a.lse[static_cast<int64_t>(r.start + t) * a.heads + qh] =
-        l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-}
-
 // ------------------------------------------------------- cache formats
 
 struct CF16 {
@@ -374,6 +309,55 @@ struct CBF16 {
 struct CI8 {  // codes are widened to fp16, which holds them exactly
   static constexpr bool kInt8 = true, kBf16 = false;
 };
+
+// Masked keys.  A masked key's weight is 0, but 0 times an infinity or a NaN in
+// its value is a NaN, which no row that does not see the key may get.  So where
+// a tile of keys is not seen whole by all rows of an item (its last keys, a
+// window's edge, holes in the table), values that are not finite are replaced by
+// zeros in shared memory and the tile's first key is noted; afterwards those
+// values are added to the outputs of the rows that do see them, which makes them
+// what the sum over the row's own keys is.  Tiles that all rows see need none of
+// this, and neither do finite values.
+
+// 16 bytes of values; returns whether one was replaced.
+template <class C>
+__device__ __forceinline__ bool clear_bad(uint8_t* p) {
+  constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
+  uint4 u = *reinterpret_cast<uint4*>(p);
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (w[i] & kExp) == kExp, hi = (w[i] >> 16 & kExp) == kExp;
+    w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+    bad = bad || lo || hi;
+  }
+  if (bad) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  return bad;
+}
+__device__ __forceinline__ bool clear_bad_scale(float* p) {
+  const bool bad = !finite(*p);
+  if (bad) *p = 0.0f;
+  return bad;
+}
+
+// Value d of key j of request b and key head h, if it is not finite, else 0.
+template <class C>
+__device__ __forceinline__ float bad_value(const Args& a, int b, int h, int page, int j, int d) {
+  const int off = page_offset(a, j);
+  const int64_t row = page * a.v.page + off * a.v.token + h * a.v.head + d;
+  float v;
+  if constexpr (C::kInt8)
+    v = static_cast<float>(reinterpret_cast<const int8_t*>(a.v.data)[row]) *
+        a.v.scales[page * a.v.spage + off * a.v.stoken + h * a.v.shead];
+  else
+    v = C::to_float(reinterpret_cast<const uint16_t*>(a.v.data)[row]);
+  return finite(v) ? 0.0f : v;
+}
+// Whether a row at position pos sees key j (the page aside).
+__device__ __forceinline__ bool sees(const Args& a, const Request& r, int pos, int j) {
+  return j <= pos && j < r.limit && (a.window == 0 || j > pos - a.window || j < a.sinks);
+}
 
 // (a, b) rounded to the 16-bit type of the tensor-core operands, a in the low half
 template <class C>

@@ -53,6 +53,7 @@ constexpr int kSoftThreads = 256;
 constexpr int kLoadThreads = 128;
 constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroups: setmaxnreg)
 constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
+constexpr int kBad = 32;               // tiles with cleared values that are noted one by one
 constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
 constexpr int kMinUnits = 2;
 // What an item costs beside its keys, in key tiles (queries, start, outputs: 7 to
@@ -105,7 +106,7 @@ struct Shared {
   int last;
   uint32_t there[8][4];           // keys of a tile that are loaded
   float xmax[2][2][128], xsum[2][128];
-  int bad[128];
+  int nbad[8], badkey[8][kBad];     // per item: tiles with cleared values, their first keys
   int64_t koff[3][128], voff[3][128];  // rows of a tile in the cache, -1: zeros
 };
 template <int N>
@@ -188,6 +189,23 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
   bool lap = false;     // the ring has been filled once
   uint32_t tile = 0;    // key tiles so far, over all items: meta slot
 
+  uint32_t item = 0;    // items so far, whose notes are in place item % 8
+  // Tile i is seen whole by all rows of the item: keys up to the first row's
+  // position, from the last row's window on.
+  auto whole = [&](int i, uint32_t slot) {
+    const int key0 = w.key(i);
+    const int p_first = w.rq.base + w.block * F::ROWS / a.group;
+    const int lo_last = a.window > 0 ? w.rq.base + (w.block * F::ROWS + w.rows - 1) / a.group - a.window + 1 : 0;
+    const uint32_t* th = sh.there[slot % F::META];
+    return key0 + kKeys - 1 <= p_first && (key0 >= lo_last || key0 + kKeys <= a.sinks) &&
+           (th[0] & th[1] & th[2] & th[3]) == 0xffffffffu;
+  };
+  auto note = [&](bool bad, int place, int key0) {
+    if (__any_sync(0xffffffffu, bad) && (t & 31) == 0) {
+      const int n = atomicAdd(&sh.nbad[place], 1);
+      if (n < kBad) sh.badkey[place][n] = key0;
+    }
+  };
   // The table's entry for key t of the item's tile i: looked up a tile ahead.
   int next_entry = -1;
   auto look = [&](int i) {
@@ -220,13 +238,32 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
   if constexpr (!C::kInt8) {
     Ring<F::STAGES> told;   // the next tile to signal
     int untold = 0;
-    auto tell = [&] {
+    // of the tiles not yet signalled, oldest first: values to look through?
+    uint32_t look_through = 0;
+    int key_q[3] = {0, 0, 0}, item_q[3] = {0, 0, 0};
+    auto tell = [&] {  // (the oldest one's copies have landed)
+      if (look_through & 1u) {
+        uint8_t* p = ring + told.stage * F::TILE;
+        bool bad = false;
+#pragma unroll 4
+        for (int i = 0; i < RPT; ++i) {
+          const int r = row0 + i * RPP;
+#pragma unroll
+          for (int x = 0; x < (CPR + LPR - 1) / LPR; ++x)
+            if (x * LPR + sub < CPR) bad |= clear_bad<typename F::P>(p + x * kBlock + r * 128 + ((sub ^ (r & 7)) << 4));
+        }
+        __syncwarp();
+        note(bad, item_q[0], key_q[0]);
+      }
+      look_through >>= 1;
+      key_q[0] = key_q[1], key_q[1] = key_q[2];
+      item_q[0] = item_q[1], item_q[1] = item_q[2];
       fence_async();
       mbar_arrive(&sh.full[told.stage]);
       told.next();
       --untold;
     };
-    auto put = [&](const Pool& pool, const int64_t* offs) {
+    auto put = [&](const Pool& pool, const int64_t* offs, int value_tile) {
       if (lap && !mbar_test(&sh.empty[at.stage], at.phase ^ 1)) {
         // no room yet: what is on its way must not wait for it
         cp_wait<0>();
@@ -248,6 +285,13 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
       cp_commit();
       at.next();
       lap = lap || at.stage == 0;
+      if (value_tile >= 0 && !whole(value_tile, tile + value_tile)) {
+        look_through |= 1u << untold;
+        const int key0 = w.key(value_tile), place = item % 8;
+        if (untold == 0) key_q[0] = key0, item_q[0] = place;
+        else if (untold == 1) key_q[1] = key0, item_q[1] = place;
+        else key_q[2] = key0, item_q[2] = place;
+      }
       if (++untold > 2) {  // three tiles in flight
         cp_wait<2>();
         tell();
@@ -258,21 +302,22 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
       if (F::TILES == 2) {
         for (int i = 0; i < w.n; ++i) {
           locate(i, tile + i);
-          put(a.k, sh.koff[(tile + i) % 3]);
-          put(a.v, sh.voff[(tile + i) % 3]);
+          put(a.k, sh.koff[(tile + i) % 3], -1);
+          put(a.v, sh.voff[(tile + i) % 3], i);
         }
       } else {
         locate(0, tile);
-        put(a.k, sh.koff[tile % 3]);
+        put(a.k, sh.koff[tile % 3], -1);
         for (int i = 0; i < w.n; ++i) {
           if (i + 1 < w.n) {
             locate(i + 1, tile + i + 1);
-            put(a.k, sh.koff[(tile + i + 1) % 3]);
+            put(a.k, sh.koff[(tile + i + 1) % 3], -1);
           }
-          put(a.v, sh.voff[(tile + i) % 3]);
+          put(a.v, sh.voff[(tile + i) % 3], i);
         }
       }
       tile += w.n;
+      ++item;
       w.close(a);
     }
     cp_wait<0>();
@@ -348,8 +393,14 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
         cp_wait<F::RAW - 1>();
         if (lap) mbar_wait(&sh.empty[at.stage], at.phase ^ 1, &sh.abort);
         int i;
-        if (kind(q, i)) widen(typename F::P{}, slot);
-        else widen(typename F::Q{}, slot);
+        if (kind(q, i)) {
+          widen(typename F::P{}, slot);
+        } else {
+          widen(typename F::Q{}, slot);
+          // (the value scales came with the keys; the softmax has not seen them)
+          if (!whole(i, tile + i))
+            note(clear_bad_scale(&scales->v[(tile + i) % F::META][t]), item % 8, w.key(i));
+        }
         fence_async();
         mbar_arrive(&sh.full[at.stage]);
         at.next();
@@ -358,6 +409,7 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
         slot = slot + 1 == F::RAW ? 0 : slot + 1;
       }
       tile += w.n;
+      ++item;
       w.close(a);
     }
     cp_wait<0>();
@@ -592,7 +644,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
   const int d1 = kTwo ? D : (wg ? D : D == 64 ? 32 : 64);
   constexpr int OB = (kTwo ? D : D == 64 ? 32 : 64) / 32;  // blocks of 32 of them
   uint32_t tiles = 0;  // key tiles so far, over all items: meta slot, S buffer
-  uint32_t ns = 0, npv = 0;
+  uint32_t ns = 0, npv = 0, item = 0;
 
   while (w.open(a)) {
     const bool live = !kTwo || tile == 0 || w.rows > 128;  // warpgroup uniform
@@ -802,7 +854,9 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     // from here on the reference in units of log2 (sums carry kUp, like O)
     m = m == -INFINITY ? -INFINITY : m * c;
 
-    // 32 columns of this CTA's outputs
+    // 32 columns of this CTA's outputs, with what clear_bad took from keys that
+    // the row sees
+    const int nbad = sh.nbad[item % 8];
     auto column_block = [&](int b, float* v) {
       if constexpr (kTwo) {
         uint32_t u[32];
@@ -814,6 +868,17 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       } else {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = o[32 * b + e];
+      }
+#pragma unroll 1
+      for (int i = 0; i < (nbad <= kBad ? nbad : w.n); ++i) {
+        const int key0 = nbad <= kBad ? sh.badkey[item % 8][i] : w.key(i);
+#pragma unroll 1
+        for (int j = key0; j < key0 + kKeys; ++j) {
+          const int page = ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
+          if (page < 0) continue;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] += bad_value<C>(a, w.b, w.head, page, j, d0 + 32 * b + e);
+        }
       }
     };
     // ---- an item of several CTAs: leave the partial, the last one joins
@@ -850,7 +915,6 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     if (final) {
       const bool joined = ss.last > ss.first;
       float inv = 0.0f, ref = 0.0f;
-      bool good = true;
       if (live) {
         if (joined) {
           m = -INFINITY, l = 0.0f;
@@ -864,7 +928,6 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
             l = fmaf(__ldcg(o + (D + 1) * F::ROWS + r), ex2(__ldcg(o + D * F::ROWS + r) - ref), l);
           }
         }
-        good = finite(l);
       }
       const int t = rr / a.group, g = rr % a.group;
       const int qh = w.head * a.group + g;
@@ -889,10 +952,6 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
           float v[32];
           if (joined) joined_block(d, v);
           else column_block(b, v);
-          float s = 0.0f;  // not finite if one of them is not
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s = fmaf(v[e], 0.0f, s);
-          good = good && s == 0.0f;
           if (ok) {
             if (a.q_vec && a.q_type == LP_F32) {
               float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + orow + d);
@@ -922,24 +981,12 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
           a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
               l == 0.0f ? -INFINITY : (m + (log2f(l) - F::kUpLog)) * kLn2;
       }
-      if constexpr (!kTwo) {  // one answer for the row's two halves; its stores are done
-        if (wg == 1) sh.bad[row] = !good;
-        __threadfence_block();
-        named_bar(2, kSoftThreads);
-        if (wg == 0) good = good && !sh.bad[row];
-        else good = true;
-      }
-      __syncwarp();
-      uint32_t again = __ballot_sync(0xffffffffu, live && ok && !good);
-      while (again) {
-        const int x = __ffs(again) - 1;
-        again &= again - 1;
-        const int row_x = w.block * F::ROWS + tile * 128 + (warp & 3) * 32 + x;
-        exact_row<C, D>(a, w.b, w.head, row_x / a.group, row_x % a.group);
-      }
-      __syncwarp();
     }
-    if constexpr (!kTwo) named_bar(2, kSoftThreads);  // sh.bad, sh.last are free
+    // both warpgroups are done with the notes (the loaders come back to this
+    // place eight items on, which is further than the ring reaches)
+    named_bar(2, kSoftThreads);
+    if (threadIdx.x == 0) sh.nbad[item % 8] = 0;
+    ++item;
     fence_before();
     w.close(a);
   }
@@ -968,6 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
     }
     mbar_init(&sh.done, 1);
     sh.abort = 0;
+    for (int x = 0; x < 8; ++x) sh.nbad[x] = 0;
     mbar_fence_init();
   }
   if (warp == 12) tmem_alloc(&sh.tmem, 512);

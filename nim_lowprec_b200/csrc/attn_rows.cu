@@ -45,6 +45,7 @@ constexpr int kItemUnits = 16;  // what an item costs beside its keys, in units
 constexpr int kTop = 14;       // queries and weights are below 2^kTop in 16 bits
 // fp16: second parts, at most 2^(kTop - 11), are held times 2^kLow
 constexpr int kLow = 12;
+constexpr int kBad = 32;  // steps with cleared values that a warp notes one by one
 
 // The types of the two products: queries x keys, weights x values.  An int8
 // code is exact in both 16-bit types.  With the keys fp16 carries the queries
@@ -364,6 +365,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    int nbad = 0, badkey = 0;  // steps with values that were cleared; the lane-th one's first key
 
     const int steps = warp < w.n ? (w.n - warp + kWarps - 1) / kWarps * SPU : 0;
 #pragma unroll 1
@@ -371,12 +373,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
       asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
       __syncwarp();  // this step has landed for all lanes, and all are done with the one before
       issue(stage == 0 ? S::STAGES - 1 : stage - 1);
-      const uint8_t* st = ring + stage * S::STAGE;
+      uint8_t* st = ring + stage * S::STAGE;
       const uint32_t st_s = ring_s + stage * S::STAGE;
       if (++stage == S::STAGES) stage = 0;
       const uint2 info = *reinterpret_cast<const uint2*>(st + 2 * S::HALF + S::SCALES);
       const uint32_t there = info.x;
       const int key0 = static_cast<int>(info.y);
+      const bool all = there == (S::KS == 32 ? 0xffffffffu : 0xffffu) &&
+                       key0 + S::KS - 1 <= p_first && (key0 >= lo_last || key0 + S::KS <= a.sinks);
+      if (!all) {  // see clear_bad
+        bool bad = false;
+        if constexpr (C::kInt8) {
+          bad = clear_bad_scale(reinterpret_cast<float*>(st + 2 * S::HALF) + S::KS + lane);
+        } else {
+#pragma unroll 4
+          for (int i = 0; i < N; ++i)
+            if (in) bad |= clear_bad<V>(st + S::HALF + place<C, D>(r0 + i * RPI, c));
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+          if (nbad < kBad) badkey = lane == nbad ? key0 : badkey;
+          ++nbad;
+        }
+        __syncwarp();
+      }
 
       // ---- scores
       float sc[S::NG][4];
@@ -415,8 +434,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
           }
       }
       // ---- weights: log2-domain scores, masks, running maximum
-      const bool all = there == (S::KS == 32 ? 0xffffffffu : 0xffffu) &&
-                       key0 + S::KS - 1 <= p_first && (key0 >= lo_last || key0 + S::KS <= a.sinks);
       const float* sks = reinterpret_cast<const float*>(st + 2 * S::HALF);
       float t[S::NG][2];
       float mx = -INFINITY, lnew = 0.0f;
@@ -525,6 +542,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
       }
     }
 
+    // ---- values that were cleared, for the rows that see them (one that was not
+    // cleared and is added again changes nothing: it is not finite)
+#pragma unroll 1
+    for (int s = 0; s < (nbad <= kBad ? nbad : steps); ++s) {
+      const int u = warp + s / SPU * kWarps;
+      const int key0 = nbad <= kBad ? __shfl_sync(0xffffffffu, badkey, s) : w.key(u) + s % SPU * S::KS;
+#pragma unroll 1
+      for (int j = key0; j < key0 + S::KS; ++j) {
+        const int page = row_ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
+        if (page < 0) continue;
+#pragma unroll
+        for (int i = 0; i < S::TILES; ++i) {
+          o[i][0] += bad_value<C>(a, w.b, w.head, page, j, value_dim<C, D>(2 * c4, i));
+          o[i][1] += bad_value<C>(a, w.b, w.head, page, j, value_dim<C, D>(2 * c4 + 1, i));
+        }
+      }
+    }
     // ---- join the warps that had steps: a row of the block by one warp
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -541,21 +575,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
     auto finish = [&](int row, const float* ro, float rm, float rl) {
       const int rr = w.block * kRows + row;
       const int t = rr / a.group, g = rr % a.group;
-      bool good = finite(rl);
+      const int qh = w.head * a.group + g;
+      const int64_t orow = (w.rq.start + t) * a.o_token + qh * a.o_head;
 #pragma unroll
-      for (int i = 0; i < DL; ++i) good = good && finite(ro[i]);
-      if (__all_sync(0xffffffffu, good)) {
-        const int qh = w.head * a.group + g;
-        const int64_t orow = (w.rq.start + t) * a.o_token + qh * a.o_head;
-#pragma unroll
-        for (int i = 0; i < DL; ++i)
-          store_elem(a.out, a.q_type, orow + lane + 32 * i, rl == 0.0f ? 0.0f : __fdiv_rn(ro[i], rl));
-        if (a.lse && lane == 0)
-          a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
-              rl == 0.0f ? -INFINITY : (rm + (log2f(rl) - kTop)) * kLn2;
-      } else {
-        exact_row<C, D>(a, w.b, w.head, t, g);
-      }
+      for (int i = 0; i < DL; ++i)
+        store_elem(a.out, a.q_type, orow + lane + 32 * i, rl == 0.0f ? 0.0f : __fdiv_rn(ro[i], rl));
+      if (a.lse && lane == 0)
+        a.lse[static_cast<int64_t>(w.rq.start + t) * a.heads + qh] =
+            rl == 0.0f ? -INFINITY : (rm + (log2f(rl) - kTop)) * kLn2;
     };
 
     for (int row0 = 0; row0 < rows; row0 += kWarps) {

@@ -91,8 +91,8 @@ lp_rows rows(PyObject* o, const char* name, int64_t dim, int device) {
   r.data = t.data_ptr();
   r.tokens = t.size(0);
   r.heads = t.size(1);
-  r.token_stride = t.stride(0);
-  r.head_stride = t.stride(1);
+  r.token_stride = r.tokens > 1 ? t.stride(0) : 0;  // (a dimension of one may have any)
+  r.head_stride = r.heads > 1 ? t.stride(1) : 0;
   r.reserved = 0;
   return r;
 }

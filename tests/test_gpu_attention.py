@@ -131,6 +131,47 @@ def test_masked_places_may_hold_anything(bad, x, cache, lens, window):
     assert not bool(torch.isfinite(out[last]).all())
 
 
+@pytest.mark.parametrize("x,cache", [("fp32", "fp16"), ("bf16", "bf16"), ("fp32", "int8"),
+                                     ("bf16", "int8")])
+@pytest.mark.parametrize("n", [3, 100])
+def test_bad_values_among_many_partly_seen_tiles(x, cache, n):
+    """More tiles with holes and bad values than are noted one by one."""
+    m = R.make(22, [(9000, n)], 2, 1, 64, 16, x, cache)
+    c = m["cache"]
+    m["table"][0, 3::8] = -1
+    pages = m["table"][0, 1::8].long()
+    pages = pages[(pages >= 0)][:-2]
+    if cache == "int8":
+        c.vScales[pages, 5] = math.inf
+    else:
+        c.v[pages, 5] = math.inf
+    out = torch.empty_like(m["q"])
+    L.pagedAttention(c, m["table"], m["qstart"], m["seq"], m["q"], out)
+    assert not bool(torch.isfinite(out).any())
+    # and one that only the last row sees, far from them
+    c.v[:] = 1
+    if cache == "int8":
+        c.vScales[:] = 1.0
+    last = 9000 + n - 1
+    at = (int(m["table"][0, last // 16]), last % 16)
+    if cache == "int8":
+        c.vScales[at] = math.nan
+    else:
+        c.v[at] = math.nan
+    L.pagedAttention(c, m["table"], m["qstart"], m["seq"], m["q"], out)
+    assert bool(torch.isfinite(out[:-1]).all()) and not bool(torch.isfinite(out[-1]).any())
+    assert bool(((out[:-1].float() - 1).abs() < 0.01).all())
+
+
+def test_a_cache_full_of_nan_stays_so():
+    for x, cache in (("fp32", "fp16"), ("bf16", "bf16")):
+        m = R.make(23, [(700, 300), (50, 1)], 4, 2, 128, 16, x, cache)
+        m["cache"].v[:] = math.nan
+        out = torch.zeros_like(m["q"])
+        L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out, window=200)
+        assert bool(torch.isnan(out).all())
+
+
 def test_seen_nan_key_and_infinite_scores():
     m = R.make(14, [(64, 1), (64, 40)], 2, 2, 64, 16, "fp32", "fp16")
     m["cache"].k[int(m["table"][0, 1]), 3] = math.nan
@@ -267,3 +308,64 @@ def test_queued_gemvs_run_before_the_attention_that_reads_them():
 def test_no_device_error():
     torch.cuda.synchronize()
     assert N.device_error() == 0
+
+
+def test_python_refusals():
+    m = R.make(24, [(9, 2), (0, 1)], 4, 2, 64, 16)
+    c, tab, qs, seq, q = m["cache"], m["table"], m["qstart"], m["seq"], m["q"]
+    out = torch.empty_like(q)
+
+    def call(cache=c, tab=tab, qs=qs, seq=seq, q=q, out=out, **kw):
+        L.pagedAttention(cache, tab, qs, seq, q, out, **kw)
+    for kw, error in (
+            (dict(q=q.double()), TypeError), (dict(q=q.cpu()), TypeError),
+            (dict(out=out.half()), N.NativeError), (dict(seq=seq.long()), TypeError),
+            (dict(qs=qs[:-1].clone()), AssertionError), (dict(tab=tab[:1]), AssertionError),
+            (dict(tab=tab.long()), TypeError), (dict(tab=tab.t().contiguous().t()), ValueError),
+            (dict(q=q[:, :3], out=out[:, :3]), AssertionError), (dict(q=q[0]), AssertionError),
+            (dict(q=q[:, :, ::2]), AssertionError), (dict(window=-1), AssertionError),
+            (dict(window=1.5), TypeError), (dict(scale="x"), TypeError),
+            (dict(scale=math.nan), N.NativeError),
+            (dict(lse=torch.empty(3, 4, device="cuda").half()), TypeError),
+            (dict(lse=torch.empty(2, 4, device="cuda")), AssertionError),
+            (dict(workspace=torch.zeros(64, dtype=torch.uint8, device="cuda")), AssertionError),
+            (dict(workspace=torch.zeros(64, device="cuda")), TypeError),
+            (dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), ValueError)):
+        with pytest.raises(error):
+            call(**kw)
+    k = torch.zeros(2, 16, 1, 64, dtype=torch.float16, device="cuda")
+    s = torch.zeros(2, 16, 1, device="cuda")
+    for args, error in (((k.float(), k.float()), TypeError), ((k, k.bfloat16()), TypeError),
+                        ((k.to(torch.int8),) * 2, TypeError), ((k, k, s, s), TypeError),
+                        ((k[0], k[0]), AssertionError), ((k, k[:1]), AssertionError),
+                        ((k.to(torch.int8),) * 2 + (s, s[:1]), AssertionError),
+                        ((k[..., ::2], k[..., ::2]), ValueError),
+                        ((k.to(torch.int8),) * 2 + (s, s.half()), TypeError)):
+        with pytest.raises(error):
+            L.KVCache(*args)
+    odd = torch.zeros(4, 16, 1, 200, dtype=torch.float16, device="cuda")
+    with pytest.raises(N.NativeError):  # rows off their 16-byte boundaries
+        call(cache=L.KVCache(odd[..., 1:65], odd[..., 1:65]), q=q[:, :1], out=out[:, :1])
+    x = torch.zeros(3, 1, 64, device="cuda")
+    slots = torch.zeros(3, dtype=torch.int64, device="cuda")
+    cc = L.KVCache(k, k.clone())
+    for args, error in (((x, x[:2], slots), AssertionError), ((x, x, slots[:2]), AssertionError),
+                        ((x, x.half(), slots), N.NativeError), ((x, x, slots.int()), TypeError),
+                        ((x[..., :32], x, slots), AssertionError)):
+        with pytest.raises(error):
+            L.storeKV(cc, *args)
+
+
+def test_a_capture_without_a_workspace_is_refused():
+    m = R.make(25, [(9, 1)], 2, 1, 64, 16)
+    out = torch.empty_like(m["q"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    L.attention._workspaces.pop((0, side.cuda_stream), None)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(g, stream=side):
+            out.zero_()
+            L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out)
+    torch.cuda.synchronize()
+    R.check(m)
