@@ -34,6 +34,16 @@
 // outputs in the softmax's registers (measured against 64 bits on five prompts
 // of up to 4700 keys: 5e-6 without, under 1e-6 with).
 //
+// What bounds it: 16-bit queries the softmax and the products in turn.  4096
+// tokens over 16384 cached, 32 heads on 8 key heads of 128, bf16: 1.13 ms by
+// itself (1090 TFLOP/s, 67 % of a cuBLAS bf16 product's rate), 1.28 ms back to
+// back under the power limit; the special-function unit alone needs 0.5 ms, the
+// products 0.76.  Tried and slower there: a third of the exponentials by a
+// polynomial on the fp32 pipes (+3 %), the weights' first half handed over early
+// (+0.4 %), the row's maximum chunk by chunk in one pass (+9 %).  fp32 over an
+// int8 cache: 5 products where 16 bits take 2, and shared memory, which they and
+// the loaders share (350 KB per key tile, 2750 cycles of about 6700).
+//
 // The running maximum moves only when a row's grows by more than 2^8 (the
 // weights stay below 2^8 times 1, or 2^15 with fp16's extra 2^7): the sums are
 // the same and O is rescaled a few times per row rather than per key tile.
@@ -55,7 +65,7 @@ constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroup
 constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
 constexpr int kBad = 32;               // tiles with cleared values that are noted one by one
 constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
-constexpr int kMinUnits = 2;
+constexpr int kMinUnits = 2;  // (100 tokens over 4000 keys: 46 us with 1 or 2, 48 with 6, 54 with 12)
 // What an item costs beside its keys, in key tiles (queries, start, outputs: 7 to
 // 13 us against 1.2 to 2.5 us per tile).  Five fp32 prompts over an int8 cache,
 // some of them short: 406 us with 2, 317 with 4, 311 with 7.
@@ -668,6 +678,9 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     const int last_w = w.rq.base + (w.block * F::ROWS + min(r0 + 31, w.rows - 1)) / a.group;
     const int lo_w = a.window > 0 ? last_w - a.window + 1 : 0;
     const float grow = kLazy / c;
+    // a warp without rows only keeps the barriers' count (its lanes' weights, and
+    // so their outputs, are whatever tensor memory holds)
+    const bool warp_ok = r0 < w.rows;
 
     float m = -INFINITY, l = 0.0f;  // reference (in scores) and sum
     float o[kTwo ? 1 : OB * 32];    // one row tile: the outputs
@@ -707,6 +720,13 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         if (kTwo) mbar_wait(&sh.sfull[x], ns++ & 1, &sh.abort);
         else mbar_wait(&sh.sfull[x], slot >> 1 & 1, &sh.abort);
         fence_after();
+        if (!warp_ok) {
+          if (!kTwo) named_bar(2, kSoftThreads);
+          fence_before();
+          mbar_arrive(&sh.pfull[x]);
+          ++npv;
+          continue;
+        }
         uint32_t see[COLS / 32];
         bool full = key0 + COLS - 1 <= pos_w && (key0 >= lo_w || key0 + COLS <= a.sinks);
 #pragma unroll
@@ -842,7 +862,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         ++npv;
       }
       wait_pv(tiles + w.n - 1);
-      gather(1.0f);
+      if (warp_ok) gather(1.0f);
     }
     tiles += w.n;
     if constexpr (!kTwo) {  // both halves' sums
@@ -887,7 +907,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     constexpr int64_t kSlot = static_cast<int64_t>(F::ROWS) * (D + 2);
     if (ss.last > ss.first) {
       float* mine = a.partials + slot_of(blockIdx.x, w.item0, w.per) * kSlot;
-      if (live) {
+      if (live && warp_ok) {
 #pragma unroll
         for (int b = 0; b < OB; ++b) {
           const int d = d0 + 32 * b;
@@ -915,18 +935,32 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     if (final) {
       const bool joined = ss.last > ss.first;
       float inv = 0.0f, ref = 0.0f;
-      if (live) {
-        if (joined) {
-          m = -INFINITY, l = 0.0f;
-          for (int k = ss.first; k <= ss.last; ++k) {
-            const float* o = a.partials + slot_of(k, w.item0, w.per) * kSlot;
-            m = fmaxf(m, __ldcg(o + D * F::ROWS + r));
+      // parts' loads go out four at a time: a trip to L2 each would cost more than
+      // the keys of a part
+      constexpr int kTogether = 4;
+      auto part_of = [&](int k) {
+        return a.partials + slot_of(min(k, ss.last), w.item0, w.per) * kSlot;
+      };
+      if (joined && live && warp_ok) {
+        m = -INFINITY, l = 0.0f;
+        for (int k = ss.first; k <= ss.last; k += kTogether) {
+          float pm[kTogether], pl[kTogether], mn = m;
+#pragma unroll
+          for (int y = 0; y < kTogether; ++y) {
+            const float* part = part_of(k + y);
+            pm[y] = __ldcg(part + D * F::ROWS + r);
+            pl[y] = __ldcg(part + (D + 1) * F::ROWS + r);
           }
-          ref = m == -INFINITY ? 0.0f : m;
-          for (int k = ss.first; k <= ss.last; ++k) {
-            const float* o = a.partials + slot_of(k, w.item0, w.per) * kSlot;
-            l = fmaf(__ldcg(o + (D + 1) * F::ROWS + r), ex2(__ldcg(o + D * F::ROWS + r) - ref), l);
+#pragma unroll
+          for (int y = 0; y < kTogether; ++y) {
+            if (k + y > ss.last) pm[y] = -INFINITY, pl[y] = 0.0f;
+            mn = fmaxf(mn, pm[y]);
           }
+          ref = mn == -INFINITY ? 0.0f : mn;
+          l *= ex2(m - ref);
+#pragma unroll
+          for (int y = 0; y < kTogether; ++y) l = fmaf(pl[y], ex2(pm[y] - ref), l);
+          m = mn;
         }
       }
       const int t = rr / a.group, g = rr % a.group;
@@ -936,14 +970,25 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       auto joined_block = [&](int d, float* v) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = 0.0f;
-        for (int k = ss.first; k <= ss.last; ++k) {
-          const float* part = a.partials + slot_of(k, w.item0, w.per) * kSlot;
-          const float f = ex2(__ldcg(part + D * F::ROWS + r) - ref);
+        for (int k = ss.first; k <= ss.last; k += kTogether) {
+          float f[kTogether], u[kTogether][32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = fmaf(__ldcg(part + (d + e) * F::ROWS + r), f, v[e]);
+          for (int y = 0; y < kTogether; ++y) {
+            const float* part = part_of(k + y);
+            f[y] = __ldcg(part + D * F::ROWS + r);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) u[y][e] = __ldcg(part + (d + e) * F::ROWS + r);
+          }
+#pragma unroll
+          for (int y = 0; y < kTogether; ++y) {
+            if (k + y > ss.last) break;
+            const float g = ex2(f[y] - ref);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = fmaf(u[y][e], g, v[e]);
+          }
         }
       };
-      if (live) {
+      if (live && warp_ok) {
         inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
         for (int b = 0; b < OB; ++b) {

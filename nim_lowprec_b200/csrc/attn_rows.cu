@@ -27,6 +27,12 @@
 //   * The tensor cores serve here to keep the arithmetic (8 rows: 16 fma per
 //     cached byte) off the fp32 pipe; at 8 rows a tile of 128 x N tcgen05
 //     rows would be 94 % padding, and the bytes bound the time either way.
+// Measured: two requests of 131000 keys, 64 heads on 8 key heads of 128, bf16,
+// 199 us (5.4 TB/s, 82 % of a copy's rate; what is missing is the spread of the
+// SMs' shares of the bandwidth, 157 us on average); 32 requests under a window
+// of 4000, heads of 64, 54 us (4.2 TB/s; 16 us of start and join); 53 requests of
+// up to 16000 keys over an int8 cache with fp32 queries, 215 us (3.8 TB/s; issue
+// bound: widening the codes and three parts of the weights).
 #include "attn.cuh"
 
 namespace lp {
@@ -40,8 +46,10 @@ constexpr int kRows = 8;
 constexpr int kUnit = 32;  // keys per unit: a warp's share of a round
 // A CTA takes at least this many units: fewer would cost more in the join of
 // the partial results than the spread over more SMs gives back.
-constexpr int kMinUnits = 4;
-constexpr int kItemUnits = 16;  // what an item costs beside its keys, in units
+constexpr int kMinUnits = 4;  // (one request of 1000 keys: 14.9 us with 1 or 4, 17.2 with 12)
+// What an item costs beside its keys, in units (about 4 us against 0.25): 32
+// requests under a window 75 us with 8, 56 with 16, 56 with 32.
+constexpr int kItemUnits = 16;
 constexpr int kTop = 14;       // queries and weights are below 2^kTop in 16 bits
 // fp16: second parts, at most 2^(kTop - 11), are held times 2^kLow
 constexpr int kLow = 12;

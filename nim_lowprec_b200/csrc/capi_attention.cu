@@ -12,8 +12,16 @@ constexpr int64_t kIntMax = 0x7fffffff;
 constexpr int64_t kCounterBytes = 4096;  // one 4-byte counter per CTA of a launch
 constexpr int64_t kSlotRows = 256;       // most rows of a partial result
 constexpr int64_t kSlotDim = 128;
-// Mean query rows per request and key head from which the chunk kernel is used.
-constexpr int64_t kChunkRows = 32;
+// Mean query rows (tokens x group) per request and key head from which the chunk
+// kernel is used.  The rows kernel reads the keys again for every 8 rows, the
+// chunk kernel's tiles cost the same for 1 row and 128; where requests x key
+// heads are few, the repeated reads spread over idle SMs.  4000 cached keys,
+// bf16, rows / chunk kernel in us: 16 requests x 8 key heads 16 rows 86 / 94,
+// 32 rows 179 / 96; x 32 heads 8 rows 182 / 288, 16 rows 355 / 291, 32 rows
+// 699 / 295; one request x 8 heads 32 rows 27 / 41, 64 rows 35 / 42, 128 rows
+// 53 / 44 (fp32 over int8: 35 / 40, 48 / 42, 75 / 47).
+constexpr int64_t kChunkRows = 24, kChunkRowsFew = 64;
+constexpr int64_t kFew = 32;  // requests x key heads
 
 #define LP_REQUIRE(cond)              \
   do {                                \
@@ -192,8 +200,8 @@ int lp_paged_attention(const lp_kv_cache* cache, const int32_t* block_tables, in
   a.scale_log2 = scale * 1.4426950408889634f;
   a.counters = static_cast<uint32_t*>(workspace);
   a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-  // mean rows per request and key head; a tile of the chunk kernel has 128 or 256
-  const bool chunk = q->tokens * a.group >= kChunkRows * n;
+  const int64_t rows = n * cache->kv_heads < kFew ? kChunkRowsFew : kChunkRows;
+  const bool chunk = q->tokens * a.group >= rows * n;
   return chunk ? lp::launch_attn_chunk(a, cache->dtype, cache->head_dim, S(stream))
                : lp::launch_attn_rows(a, cache->dtype, cache->head_dim, S(stream));
 }
