@@ -62,7 +62,8 @@ __device__ __forceinline__ Request request(const Args& a, int b) {
   Request r;
   r.start = min(max(__ldg(a.qstart + b), 0), a.tokens);
   r.n = min(max(__ldg(a.qstart + b + 1), r.start), a.tokens) - r.start;
-  const int seq = max(__ldg(a.seqlens + b), 0);
+  // (below 2^31 by more than a tile, so that key numbers do not wrap)
+  const int seq = min(max(__ldg(a.seqlens + b), 0), 0x7fffff00);
   r.base = seq - r.n;
   r.limit = static_cast<int>(
       min(static_cast<int64_t>(seq), static_cast<int64_t>(a.table_width) * a.page_size));
@@ -322,9 +323,14 @@ struct CI8 {  // codes are widened to fp16, which holds them exactly
 // 16 bytes of values; returns whether one was replaced.
 template <class C>
 __device__ __forceinline__ bool clear_bad(uint8_t* p) {
-  constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
-  uint4 u = *reinterpret_cast<uint4*>(p);
+  constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u, kOne = C::kBf16 ? 0x0080u : 0x0400u;
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
   uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  // an exponent of all ones plus one carries into the sign's place
+  uint32_t carry = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) carry |= (w[i] & (kExp | kExp << 16)) + (kOne | kOne << 16);
+  if (!(carry & 0x80008000u)) return false;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -332,7 +338,7 @@ __device__ __forceinline__ bool clear_bad(uint8_t* p) {
     w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
     bad = bad || lo || hi;
   }
-  if (bad) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   return bad;
 }
 __device__ __forceinline__ bool clear_bad_scale(float* p) {

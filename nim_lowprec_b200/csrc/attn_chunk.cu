@@ -63,7 +63,8 @@ constexpr int kSoftThreads = 256;
 constexpr int kLoadThreads = 128;
 constexpr int kThreads = kSoftThreads + kLoadThreads + 128;  // (whole warpgroups: setmaxnreg)
 constexpr int kBlock = 128 * 128;      // bytes of 128 rows x 64 16-bit elements
-constexpr int kBad = 32;               // tiles with cleared values that are noted one by one
+constexpr int kBad = 16;               // tiles with cleared values that are noted one by one
+constexpr int kPlaces = 16;            // items whose notes are held
 constexpr float kLazy = 8.0f;          // log2 of the growth that moves the maximum
 constexpr int kMinUnits = 2;  // (100 tokens over 4000 keys: 46 us with 1 or 2, 48 with 6, 54 with 12)
 // What an item costs beside its keys, in key tiles (queries, start, outputs: 7 to
@@ -94,8 +95,8 @@ struct Cfg {
   static constexpr int SMEM = 1024 + TILES * NQ * TILE + STAGES * TILE + RAW * RAW_TILE;
   // Registers per thread of the roles' warpgroups; 128 each at launch.  One row
   // tile's softmax holds 64 scores and up to 64 outputs, two tiles' 128 scores.
-  static constexpr int SOFT_REGS = TILES == 2 ? 200 : 216;
-  static constexpr int LOAD_REGS = TILES == 2 ? 64 : 48;
+  static constexpr int SOFT_REGS = TILES == 2 ? 200 : 208;
+  static constexpr int LOAD_REGS = 64;
   static constexpr int MMA_REGS = TILES == 2 ? 48 : 32;
   static_assert(2 * SOFT_REGS + LOAD_REGS + MMA_REGS == 4 * 128, "");
   // fp16 weights are held times 2^7, bf16 has the range without
@@ -116,7 +117,7 @@ struct Shared {
   int last;
   uint32_t there[8][4];           // keys of a tile that are loaded
   float xmax[2][2][128], xsum[2][128];
-  int nbad[8], badkey[8][kBad];     // per item: tiles with cleared values, their first keys
+  int nbad[kPlaces], badkey[kPlaces][kBad];     // per item: tiles with cleared values, their first keys
   int64_t koff[3][128], voff[3][128];  // rows of a tile in the cache, -1: zeros
 };
 template <int N>
@@ -199,7 +200,7 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
   bool lap = false;     // the ring has been filled once
   uint32_t tile = 0;    // key tiles so far, over all items: meta slot
 
-  uint32_t item = 0;    // items so far, whose notes are in place item % 8
+  uint32_t item = 0;    // items so far, whose notes are in place item % kPlaces
   // Tile i is seen whole by all rows of the item: keys up to the first row's
   // position, from the last row's window on.
   auto whole = [&](int i, uint32_t slot) {
@@ -297,7 +298,7 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
       lap = lap || at.stage == 0;
       if (value_tile >= 0 && !whole(value_tile, tile + value_tile)) {
         look_through |= 1u << untold;
-        const int key0 = w.key(value_tile), place = item % 8;
+        const int key0 = w.key(value_tile), place = item % kPlaces;
         if (untold == 0) key_q[0] = key0, item_q[0] = place;
         else if (untold == 1) key_q[1] = key0, item_q[1] = place;
         else key_q[2] = key0, item_q[2] = place;
@@ -409,7 +410,7 @@ __device__ __forceinline__ void load_role(const Args& a, WalkOf<F> w, Shared& sh
           widen(typename F::Q{}, slot);
           // (the value scales came with the keys; the softmax has not seen them)
           if (!whole(i, tile + i))
-            note(clear_bad_scale(&scales->v[(tile + i) % F::META][t]), item % 8, w.key(i));
+            note(clear_bad_scale(&scales->v[(tile + i) % F::META][t]), item % kPlaces, w.key(i));
         }
         fence_async();
         mbar_arrive(&sh.full[at.stage]);
@@ -876,7 +877,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
 
     // 32 columns of this CTA's outputs, with what clear_bad took from keys that
     // the row sees
-    const int nbad = sh.nbad[item % 8];
+    const int nbad = sh.nbad[item % kPlaces];
     auto column_block = [&](int b, float* v) {
       if constexpr (kTwo) {
         uint32_t u[32];
@@ -891,7 +892,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       }
 #pragma unroll 1
       for (int i = 0; i < (nbad <= kBad ? nbad : w.n); ++i) {
-        const int key0 = nbad <= kBad ? sh.badkey[item % 8][i] : w.key(i);
+        const int key0 = nbad <= kBad ? sh.badkey[item % kPlaces][i] : w.key(i);
 #pragma unroll 1
         for (int j = key0; j < key0 + kKeys; ++j) {
           const int page = ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
@@ -1027,10 +1028,9 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
               l == 0.0f ? -INFINITY : (m + (log2f(l) - F::kUpLog)) * kLn2;
       }
     }
-    // both warpgroups are done with the notes (the loaders come back to this
-    // place eight items on, which is further than the ring reaches)
-    named_bar(2, kSoftThreads);
-    if (threadIdx.x == 0) sh.nbad[item % 8] = 0;
+    // A place half the round ahead: the item that had it is behind both warpgroups,
+    // and the loaders are not there yet (the ring reaches five items).
+    if (threadIdx.x == 0) sh.nbad[(item + kPlaces / 2) % kPlaces] = 0;
     ++item;
     fence_before();
     w.close(a);
@@ -1060,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_chunk(const __grid_constan
     }
     mbar_init(&sh.done, 1);
     sh.abort = 0;
-    for (int x = 0; x < 8; ++x) sh.nbad[x] = 0;
+    for (int x = 0; x < kPlaces; ++x) sh.nbad[x] = 0;
     mbar_fence_init();
   }
   if (warp == 12) tmem_alloc(&sh.tmem, 512);

@@ -355,7 +355,10 @@ __device__ __forceinline__ void store_i8(uint8_t* p, float* scale, const float* 
   const float s = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
   uint32_t w[N / 4];
   codes<N>(w, x, s);
-  if (active) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (active) {
+    if constexpr (N == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
   if (write_scale) *scale = s;
 }
 
@@ -452,6 +455,15 @@ template <int X, int T, bool STORE>
 int launch_rows_t(const RowsArgs& a, bool vec, cudaStream_t st) {
   // fp32 rows out: 4 elements, so that a warp writes whole lines
   constexpr int N = STORE ? (T == LP_I8 ? 16 : 8) : X == LP_F32 ? 4 : 8;
+  if constexpr (N == 16) {
+    // Few rows: 8 elements a lane, whose chain is shorter (61 x 8 rows of 128:
+    // 3.4 us against 4.6; 4096 x 32: 41 against 31).
+    if (a.items * a.dim <= int64_t{device_info().sm_count} * kRowThreads * 8) {
+      if (a.dim <= 64) return launch_rows_l<X, T, 8, 8, STORE>(a, vec, st);
+      if (a.dim <= 128) return launch_rows_l<X, T, 16, 8, STORE>(a, vec, st);
+      return launch_rows_l<X, T, 32, 8, STORE>(a, vec, st);
+    }
+  }
   if (a.dim <= 64) return launch_rows_l<X, T, 64 / N, N, STORE>(a, vec, st);
   if (a.dim <= 128) return launch_rows_l<X, T, 128 / N, N, STORE>(a, vec, st);
   constexpr int W = N == 4 ? 8 : N;  // (a row's lanes are in one warp)
@@ -531,7 +543,7 @@ int launch_assign_pages(const int32_t* ctx, const int32_t* add, int64_t requests
   const int64_t want = std::max((tokens + kAssignThreads - 1) / kAssignThreads,
                                 (requests + kAssignThreads / 32 - 1) / (kAssignThreads / 32));
   const int grid = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(want, device_info().sm_count)));
+      std::max<int64_t>(1, std::min<int64_t>(want, device_info().sm_count * 3ll)));
   k_assign_pages<<<grid, kAssignThreads, 0, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
