@@ -371,8 +371,8 @@ int lp_dequantize_nvfp4(const uint8_t *codes, int64_t codes_len, const uint8_t *
 
 /* The cache: element (page, token, head, i) of k is at
  * k[page*k_strides[0] + token*k_strides[1] + head*k_strides[2] + i], strides
- * in elements, so pages may hold tokens x heads or heads x tokens.  Rows
- * start on 16-byte boundaries (pointers and strides).  LP_I8: the value is
+ * in elements and not negative, so pages may hold tokens x heads or heads x
+ * tokens.  Rows start on 16-byte boundaries (pointers and strides).  LP_I8: the value is
  * code * scale, the scale of (page, token, head) found by its own strides. */
 typedef struct lp_kv_cache {
   void *k, *v;
@@ -385,7 +385,8 @@ typedef struct lp_kv_cache {
 } lp_kv_cache;
 
 /* Rows of head_dim elements: row (token, head) at
- * data[token*token_stride + head*head_stride]; any strides and alignment. */
+ * data[token*token_stride + head*head_stride]; any alignment, strides from 0 to
+ * 2^31 - 1. */
 typedef struct lp_rows {
   void *data;
   int64_t tokens, heads, token_stride, head_stride;

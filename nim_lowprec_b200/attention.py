@@ -17,9 +17,8 @@ try:  # as in dequant: importing the package needs no torch
 except Exception:  # pragma: no cover
     torch = None
 
-_ROW_TYPES, _CACHE_TYPES = {}, {}
+_CACHE_TYPES = {}
 if torch is not None:
-    _ROW_TYPES = {torch.float32: N.LP_F32, torch.float16: N.LP_F16, torch.bfloat16: N.LP_BF16}
     _CACHE_TYPES = {torch.float16: N.LP_F16, torch.bfloat16: N.LP_BF16, torch.int8: N.LP_I8}
 
 _I3 = ctypes.c_int64 * 3
