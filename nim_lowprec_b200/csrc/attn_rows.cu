@@ -24,6 +24,10 @@
 //     largest keep 22 bits.
 //   * An int8 cache's scales are per (token, head): a key's multiplies its
 //     score, a value's its weight, so the codes go into the products exactly.
+//   * A step's products start from zero and are added to the outputs in fp32
+//     registers, rounded: left in the product's own sum they are cut off at
+//     each one, which takes 1.0e-4 to 1.6e-4 off 131000 keys of one sign
+//     (errors now 3e-7, 1e-7 at 16000 keys and below).
 //   * The tensor cores serve here to keep the arithmetic (8 rows: 16 fma per
 //     cached byte) off the fp32 pipe; at 8 rows a tile of 128 x N tcgen05
 //     rows would be 94 % padding, and the bytes bound the time either way.
@@ -33,6 +37,8 @@
 // of 4000, heads of 64, 54 us (4.2 TB/s; 16 us of start and join); 53 requests of
 // up to 16000 keys over an int8 cache with fp32 queries, 215 us (3.8 TB/s; issue
 // bound: widening the codes and three parts of the weights).
+#include <type_traits>
+
 #include "attn.cuh"
 
 namespace lp {
@@ -111,6 +117,40 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a * b.
+template <class C>
+__device__ __forceinline__ void mma_new(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (C::kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// o += weights x values of N times 16 keys, third parts (T3) first.  (32 keys at
+// once: one addition to o for two.  An int8 step of 32 keys x 128 takes 5 % more
+// time than with sums in the product, others nothing that shows.)
+template <class V, bool T3, int N, int M>
+__device__ __forceinline__ void add_products(float* o, const uint32_t (&pa)[N][4],
+                                             const uint32_t (&pc)[M][4], const uint32_t (&b)[N][2]) {
+  float d[4];
+  if constexpr (T3) {
+    mma_new<V>(d, pc[0], b[0][0], b[0][1]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) mma<V>(d, pc[i], b[i][0], b[i][1]);
+    mma<V>(d, pa[0], b[0][0], b[0][1]);
+  } else {
+    mma_new<V>(d, pa[0], b[0][0], b[0][1]);
+  }
+#pragma unroll
+  for (int i = 1; i < N; ++i) mma<V>(d, pa[i], b[i][0], b[i][1]);
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) upk(add2(pk(o[i], o[i + 1]), pk(d[i], d[i + 1])), o[i], o[i + 1]);
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -150,13 +190,12 @@ __device__ __forceinline__ void lds_words(uint32_t* r, const uint8_t* p) {
 }
 
 // Head dimension of column n of output tile i.  16-bit values are read as
-// matrices, in order.  A lane reads int8 values as one piece of 16 or 8 codes
-// (D = 96: 8, then 4), and takes tile i's from its code i.
+// matrices, in order.  A lane reads int8 values as pieces of 8 codes (the last
+// of D = 96: 4), and takes tile i's from its code i.
 template <class C, int D>
 __device__ __forceinline__ int value_dim(int n, int i) {
   if constexpr (!C::kInt8) return i * 8 + n;
-  else if constexpr (D == 96) return i < 8 ? n * 8 + i : 64 + n * 4 + (i - 8);
-  else return n * (D / 8) + i;
+  else return i < 8 ? n * 8 + i : 64 + n * (D / 8 - 8) + (i - 8);
 }
 // Head dimension of the first of a lane's four elements in k16 step k: of the
 // queries, and of the keys that meet them (16-bit keys: the second pair is 8 on).
@@ -493,60 +532,68 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
         m = mn;
       }
       l += lnew;
-      // ---- outputs: p in two or three parts times the values
+      // ---- outputs: p in two or three parts times the values, 16 or 32 keys at once
+      constexpr int KK = S::KS / 16;
+      uint32_t pa[KK][4], pc[T3 ? KK : 1][4];
 #pragma unroll
-      for (int kk = 0; kk < S::KS / 16; ++kk) {
-        uint32_t pa[4], pc[4] = {0u, 0u, 0u, 0u};
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float p0 = p[2 * kk + h][0], p1 = p[2 * kk + h][1];
           const uint32_t hi = pack16<V>(p0, p1);
           const float r0 = (p0 - low16<V>(hi)) * kUpV, r1 = (p1 - high16<V>(hi)) * kUpV;
-          pa[2 * h] = hi;
-          pa[2 * h + 1] = pack16<V>(r0, r1);
-          if constexpr (T3)
-            pc[2 * h] = pack16<V>(r0 - low16<V>(pa[2 * h + 1]), r1 - high16<V>(pa[2 * h + 1]));
+          pa[kk][2 * h] = hi;
+          pa[kk][2 * h + 1] = pack16<V>(r0, r1);
+          if constexpr (T3) {
+            const uint32_t lo = pa[kk][2 * h + 1];
+            pc[kk][2 * h] = pack16<V>(r0 - low16<V>(lo), r1 - high16<V>(lo));
+            pc[kk][2 * h + 1] = 0u;
+          }
         }
-        if constexpr (!C::kInt8) {
+      if constexpr (!C::kInt8) {
 #pragma unroll
-          for (int i = 0; i < S::TILES; i += 2) {
-            uint32_t vb[4];  // 16 keys x 16 dimensions, transposed
-            ldmatrix4_t(vb, st_s + S::HALF + place<C, D>(kk * 16 + (lane & 15), i + (lane >> 4)));
-            mma<V>(o[i], pa, vb[0], vb[1]);
-            mma<V>(o[i + 1], pa, vb[2], vb[3]);
-            if constexpr (T3) {
-              mma<V>(o[i], pc, vb[0], vb[1]);
-              mma<V>(o[i + 1], pc, vb[2], vb[3]);
-            }
+        for (int i = 0; i < S::TILES; i += 2) {
+          uint32_t vb[KK][4];  // 16 keys x 16 dimensions, transposed
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            ldmatrix4_t(vb[kk], st_s + S::HALF + place<C, D>(kk * 16 + (lane & 15), i + (lane >> 4)));
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            uint32_t b[KK][2];
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) b[kk][0] = vb[kk][2 * y], b[kk][1] = vb[kk][2 * y + 1];
+            add_products<V, T3>(o[i + y], pa, pc, b);
           }
-        } else {
-          constexpr int VE = D / 8, VP = D == 128 ? 16 : 8, VW = VE / 4;
-          uint32_t vw[4][VW];
+        }
+      } else {
+        // W words of codes a row: the first eight tiles' codes, then the others'
+        auto tiles = [&](auto words, int first_byte, int tile) {
+          constexpr int W = decltype(words)::value;
+          uint32_t vw[KK][4][W];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = kk * 16 + (x >> 1) * 8 + 2 * c4 + (x & 1);
-            const uint8_t* row = st + S::HALF;
-            const int byte = g8 * VP;
-            lds_words<VP / 4>(vw[x], row + place<C, D>(key, byte >> 4) + (byte & 15));
-            if constexpr (VE > VP) {
-              const int rest = 64 + g8 * 4;
-              lds_words<1>(vw[x] + VP / 4, row + place<C, D>(key, rest >> 4) + (rest & 15));
+          for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = kk * 16 + (x >> 1) * 8 + 2 * c4 + (x & 1);
+              const int byte = first_byte + g8 * (4 * W);
+              lds_words<W>(vw[kk][x], st + S::HALF + place<C, D>(key, byte >> 4) + (byte & 15));
             }
-          }
 #pragma unroll
-          for (int x = 0; x < VW; ++x) {
-            const uint32_t x0 = prmt(vw[0][x], vw[1][x], 0x5140u), x1 = prmt(vw[0][x], vw[1][x], 0x7362u);
-            const uint32_t y0 = prmt(vw[2][x], vw[3][x], 0x5140u), y1 = prmt(vw[2][x], vw[3][x], 0x7362u);
+          for (int x = 0; x < W; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t sel = e & 1 ? 0x4342u : 0x4140u;
-              const uint32_t b0 = codes_bf16(e < 2 ? x0 : x1, sel);
-              const uint32_t b1 = codes_bf16(e < 2 ? y0 : y1, sel);
-              mma<V>(o[4 * x + e], pa, b0, b1);
-              if constexpr (T3) mma<V>(o[4 * x + e], pc, b0, b1);
+              const uint32_t sel = e & 1 ? 0x4342u : 0x4140u, pair = e < 2 ? 0x5140u : 0x7362u;
+              uint32_t b[KK][2];
+#pragma unroll
+              for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  b[kk][y] = codes_bf16(prmt(vw[kk][2 * y][x], vw[kk][2 * y + 1][x], pair), sel);
+              add_products<V, T3>(o[tile + 4 * x + e], pa, pc, b);
             }
-          }
-        }
+        };
+        tiles(std::integral_constant<int, 2>{}, 0, 0);
+        if constexpr (D > 64) tiles(std::integral_constant<int, (D - 64) / 32>{}, 64, 8);
       }
     }
 

@@ -1,0 +1,65 @@
+"""pagedAttention over long contexts of values of one sign, where a bias of the sums would show:
+sums that were cut off instead of rounded would all come out low."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():  # pragma: no cover
+    pytest.skip("no CUDA device", allow_module_level=True)
+
+import nim_lowprec_b200 as L  # noqa: E402
+import attention_refs as R  # noqa: E402
+
+
+def positive(keys, new, requests, x, cache, dim, heads=1):
+    """Requests that share one table of `keys` keys, values close to 1, flat weights.  One key
+    head: with more requests than CTAs, an item's keys are added up by one or two of them."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(keys + dim)
+    ps = 64
+    pages = -(-keys // ps)
+    shape = (pages, ps, 1, dim)
+    if cache == "int8":
+        k = torch.randint(-127, 128, shape, generator=g, device="cuda", dtype=torch.int8)
+        v = torch.randint(90, 128, shape, generator=g, device="cuda", dtype=torch.int8)
+        ks = torch.full(shape[:3], 0.01, device="cuda")
+        vs = 0.009 + 0.001 * torch.rand(shape[:3], generator=g, device="cuda")
+        c = L.KVCache(k, v, ks, vs)
+    else:
+        k, v = (torch.randn(shape, generator=g, device="cuda") for _ in range(2))
+        c = L.KVCache(k.to(R.DT[cache]), (1 + 0.1 * v).to(R.DT[cache]))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = 0.05 * torch.randn(requests * new, heads, dim, generator=g, device="cuda")
+    return dict(cache=c, table=torch.arange(pages, **i32)[None].repeat(requests, 1),
+                qstart=torch.arange(requests + 1, **i32) * new,
+                seq=torch.full((requests,), keys, **i32), q=q.to(R.DT[x]))
+
+
+def run(m, look, scale=None, window=0):
+    """Every request, held to 64 bits in the first `look`: (relative errors, s)."""
+    out = torch.full_like(m["q"], math.nan)
+    L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out, window=window)
+    rows = int(m["qstart"][look])
+    o, _, amp, big = R.attention(m["cache"], m["table"][:look], m["qstart"][:look + 1],
+                                 m["seq"][:look], m["q"][:rows], m["q"].shape[2] ** -0.5, window)
+    assert bool(torch.isfinite(out).all())
+    return out[:rows], o, amp, big
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("cache", ["fp16", "bf16", "int8"])
+def test_fp32_sums_of_single_tokens_are_rounded(cache, dim):
+    """A warp adds up at most n = keys / 64 steps in fp32 (fewer where a step has 32 keys), each
+    sum rounded once: errors of at most 2^-24 of the sum, independent of one another, so 5
+    sqrt(n) 2^-24 in the numerator and as much in the denominator (5 standard deviations of
+    errors that were all at their limit).  Within a step at most 6 products are cut off, each
+    by less than 2^-23 of the step's sum, which is all that may show in the mean."""
+    keys = 131000
+    out, o, amp, big = run(positive(keys, 1, 400, "fp32", cache, dim), 48)
+    e = (out.double() - o) / o
+    sums = 2 * 5 * math.sqrt(keys / 64) * 2.0 ** -24
+    assert bool((e.abs() <= 2.0 ** -19 * (big[..., None] + 1) + sums).all()), float(e.abs().max())
+    assert abs(float(e.mean())) <= 2.0 ** -20, float(e.mean())
