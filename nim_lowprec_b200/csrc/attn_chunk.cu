@@ -1029,8 +1029,13 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
               l == 0.0f ? -INFINITY : (m + (log2f(l) - F::kUpLog)) * kLn2;
       }
     }
-    // A place half the round ahead: the item that had it is behind both warpgroups,
-    // and the loaders are not there yet (the ring reaches five items).
+    // The warpgroups meet every half round of places.  (With two row tiles nothing
+    // else holds the first one while the second one is in a tile's outputs: items
+    // of one tile need only the first.)  So they are fewer than kPlaces / 2 items
+    // apart, and the place half the round ahead, whose last item is kPlaces / 2
+    // back, is behind both; the loaders, whose ring reaches five items, are not
+    // there yet, and the places that they write belonged to items further back.
+    if (kTwo && item % (kPlaces / 2) == kPlaces / 2 - 1) named_bar(2, kSoftThreads);
     if (threadIdx.x == 0) sh.nbad[(item + kPlaces / 2) % kPlaces] = 0;
     ++item;
     fence_before();

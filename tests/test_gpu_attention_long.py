@@ -63,3 +63,50 @@ def test_fp32_sums_of_single_tokens_are_rounded(cache, dim):
     sums = 2 * 5 * math.sqrt(keys / 64) * 2.0 ** -24
     assert bool((e.abs() <= 2.0 ** -19 * (big[..., None] + 1) + sums).all()), float(e.abs().max())
     assert abs(float(e.mean())) <= 2.0 ** -20, float(e.mean())
+
+
+@pytest.mark.parametrize("x,cache,heads,kv", [("bf16", "bf16", 4, 4), ("fp16", "fp16", 6, 2),
+                                              ("bf16", "int8", 2, 2)])
+def test_infinities_of_long_items_before_many_short_ones(x, cache, heads, kv):
+    """A prompt that fills both row tiles, with infinities that only later rows see, before
+    dozens of short requests (one row tile each) with infinities of their own: every row gets
+    those that it sees and no others, whichever half of the kernel is ahead."""
+    lens = ([(100, 768 * kv // heads)] + [(37 * i % 90, 26 + i % 9) for i in range(39)]) * 12
+    m = R.make(40, lens, heads, kv, 64, 16, x, cache)
+    c, tab = m["cache"], m["table"]
+    clean = L.KVCache(c.k, c.v.clone(), c.kScales,
+                      None if c.vScales is None else c.vScales.clone())
+    seen = []  # per request: the keys that hold an infinity
+    for b, (ctx, new) in enumerate(lens):
+        at = [ctx + new - 1, ctx + new // 2, ctx + new // 3] if new > 100 else [ctx + new - 2]
+        seen.append(at)
+        for j in at:
+            where = (int(tab[b, j // 16]), j % 16)
+            if cache == "int8":
+                c.v[where] = 1
+                c.vScales[where] = math.inf
+            else:
+                c.v[where][:, ::3] = math.inf
+                clean.v[where][:, ::3] = 0
+            if cache == "int8":
+                clean.v[where] = 1
+    for _ in range(3):
+        out = torch.full_like(m["q"], math.nan)
+        L.pagedAttention(c, tab, m["qstart"], m["seq"], m["q"], out)
+        if _ == 0:
+            first = out
+        assert torch.equal(first.isinf(), out.isinf())
+        assert torch.equal(torch.where(first.isinf(), 0, first), torch.where(out.isinf(), 0, out))
+    hot = torch.zeros(out.shape[0], dtype=torch.bool, device="cuda")
+    for b, (ctx, new) in enumerate(lens):
+        t0 = int(m["qstart"][b])
+        hot[t0 + min(seen[b]) - ctx:t0 + new] = True
+    inf = torch.zeros_like(out, dtype=torch.bool)
+    inf[hot] = True
+    if cache != "int8":
+        inf[:, :, [d for d in range(64) if d % 3]] = False
+    assert torch.equal(torch.isposinf(out), inf)
+    o, _, amp, big = R.attention(clean, tab, m["qstart"], m["seq"], m["q"], 64 ** -0.5)
+    ok = ~inf
+    d = (out.double() - o).abs()
+    assert bool((d <= R.tolerance(o, amp, big, out.dtype))[ok].all())
