@@ -32,7 +32,12 @@
 // which over a few thousand keys would show in an fp32 result.  So there (one
 // row tile) small parts come first, and a key tile's product is added to the
 // outputs in the softmax's registers (measured against 64 bits on five prompts
-// of up to 4700 keys: 5e-6 without, under 1e-6 with).
+// of up to 4700 keys: 5e-6 without, under 1e-6 with).  With two row tiles and
+// tables of more than 16384 keys (bf16 weights: 131072), a sum leaves tensor memory
+// for the workspace every so many tiles: values of one sign came out 5.9e-4 low
+// over 131000 keys and 1.8e-3 over 400000 in fp16, now within its rounding.  (In
+// one kernel for all lengths that took 4 to 7 % more time of short items, for the
+// registers; long ones pay 2 to 3 %.)
 //
 // What bounds it: 16-bit queries the softmax and the products in turn.  4096
 // tokens over 16384 cached, 32 heads on 8 key heads of 128, bf16: 1.13 to 1.2 ms by
@@ -74,13 +79,15 @@ constexpr int kMinUnits = 2;  // (100 tokens over 4000 keys: 46 us with 1 or 2, 
 constexpr int kItemUnits = 6;
 
 // C: the cache's format; Q: type of the operands of Q K^T, P: of P V;
-// NQ, NP: parts of queries and weights.
-template <class C_, class Q_, class P_, int NQ_, int NP_, int TILES_, int D_>
+// NQ, NP: parts of queries and weights; LONG (two row tiles): items may have more
+// than HOLD key tiles.
+template <class C_, class Q_, class P_, int NQ_, int NP_, int TILES_, int D_, bool LONG_>
 struct Cfg {
   using C = C_;
   using Q = Q_;
   using P = P_;
   static constexpr int NQ = NQ_, NP = NP_, TILES = TILES_, D = D_;
+  static constexpr bool LONG = LONG_;
   static constexpr int BLOCKS = (D + 63) / 64;
   static constexpr int TILE = BLOCKS * kBlock;  // bytes of a Q part, K or V tile
   static constexpr int STAGES = C::kInt8 ? (D == 64 ? 4 : 3) : D == 64 ? 8 : NQ == 3 ? 3 : 4;
@@ -103,6 +110,10 @@ struct Cfg {
   // fp16 weights are held times 2^7, bf16 has the range without
   static constexpr float kUp = P::kBf16 ? 1.0f : 128.0f;
   static constexpr float kUpLog = P::kBf16 ? 0.0f : 7.0f;
+  // Two row tiles: key tiles whose sum stays in tensor memory.  8 products a tile,
+  // each cut off, take 0.6e-6 of the sum a tile: up to 0.7e-4 of an fp16 result and
+  // 0.6e-3 of a bf16 one, a sixth of what its rounding is.
+  static constexpr int HOLD = P::kBf16 ? 1024 : 128;
 };
 
 template <class F>
@@ -519,13 +530,14 @@ __device__ __forceinline__ void mma_role(const Args& a, WalkOf<F> w, Shared& sh,
         const uint32_t vs = at.stage;
         at.next();
         const bool more = i + 1 < n;
-        pv(0, 0, vs, i == 0, nt == 1);
+        const bool first = F::LONG ? i % F::HOLD == 0 : i == 0;
+        pv(0, 0, vs, first, nt == 1);
         if (more) {
           wait_tile();
           qk(0, 0, at.stage, nt == 1);
         }
         if (nt == 2) {
-          pv(1, 1, vs, i == 0, true);
+          pv(1, 1, vs, first, true);
           if (more) qk(1, 1, at.stage, true);
         }
         if (more) at.next();
@@ -712,6 +724,15 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       else mbar_wait(&sh.pvdone[slot & 1], slot >> 1 & 1, &sh.abort);
       fence_after();
     };
+    // LONG: after each HOLD tiles their sum goes to the place of the item's
+    // partial (which takes it at the end), with the reference that it is in units of.
+    constexpr int64_t kSlot = static_cast<int64_t>(F::ROWS) * (D + 2);
+    auto place = [&] { return a.partials + slot_of(blockIdx.x, w.item0, w.per) * kSlot + r; };
+    // the factor that takes the held sums to the reference of now
+    auto since_held = [&](const float* held) {
+      const float mh = held[D * F::ROWS];
+      return mh == -INFINITY ? 0.0f : ex2((mh - m) * c);
+    };
     if (live) {
       for (int i = 0; i < w.n; ++i) {
         const int key0 = w.key(i) + col0;
@@ -862,6 +883,24 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         fence_before();
         mbar_arrive(&sh.pfull[x]);
         ++npv;
+        if (F::LONG && (i + 1) % F::HOLD == 0 && i + 1 < w.n) {
+          wait_pv(slot);
+          float* held = place();
+          const float f = i + 1 > F::HOLD ? since_held(held) : 0.0f;
+#pragma unroll 1
+          for (int d = 0; d < D; d += 16) {
+            uint32_t u[16];
+            tmem_ld16(tm + o_col(tile) + d, u);
+            tmem_wait_ld();
+            tie(u, 16);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float* h = held + (d + e) * F::ROWS;
+              *h = i + 1 > F::HOLD ? fmaf(*h, f, __uint_as_float(u[e])) : __uint_as_float(u[e]);
+            }
+          }
+          held[D * F::ROWS] = m;
+        }
       }
       wait_pv(tiles + w.n - 1);
       if (warp_ok) gather(1.0f);
@@ -873,6 +912,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       l += sh.xsum[1 - wg][row];
       named_bar(2, kSoftThreads);
     }
+    const float f_held = F::LONG && live && warp_ok && w.n > F::HOLD ? since_held(place()) : 0.0f;
     // from here on the reference in units of log2 (sums carry kUp, like O)
     m = m == -INFINITY ? -INFINITY : m * c;
 
@@ -887,6 +927,11 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
         tie(u, 32);
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
+        if (F::LONG && w.n > F::HOLD) {
+          const float* held = place() + 32 * b * F::ROWS;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = fmaf(held[e * F::ROWS], f_held, v[e]);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = o[32 * b + e];
@@ -906,7 +951,6 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     // ---- an item of several CTAs: leave the partial, the last one joins
     bool final = true;
     const Sharers ss = sharers(w.item0, w.un.n, w.per);
-    constexpr int64_t kSlot = static_cast<int64_t>(F::ROWS) * (D + 2);
     if (ss.last > ss.first) {
       float* mine = a.partials + slot_of(blockIdx.x, w.item0, w.per) * kSlot;
       if (live && warp_ok) {
@@ -1114,14 +1158,28 @@ int launch(const Args& a, cudaStream_t st) {
   return cuda_status(cudaGetLastError());
 }
 
-template <class C, class Q, class P, int NQ, int NP, int TILES>
+template <class C, class Q, class P, int NQ, int NP, int TILES, bool LONG>
 int launch_dim(const Args& a, int dim, cudaStream_t st) {
   switch (dim) {
-    case 64: return launch<Cfg<C, Q, P, NQ, NP, TILES, 64>>(a, st);
-    case 96: return launch<Cfg<C, Q, P, NQ, NP, TILES, 96>>(a, st);
-    case 128: return launch<Cfg<C, Q, P, NQ, NP, TILES, 128>>(a, st);
+    case 64: return launch<Cfg<C, Q, P, NQ, NP, TILES, 64, LONG>>(a, st);
+    case 96: return launch<Cfg<C, Q, P, NQ, NP, TILES, 96, LONG>>(a, st);
+    case 128: return launch<Cfg<C, Q, P, NQ, NP, TILES, 128, LONG>>(a, st);
     default: return LP_ERR_UNSUPPORTED;
   }
+}
+
+// One row tile.
+template <class C, class Q, class P, int NQ, int NP>
+int launch_one(const Args& a, int dim, cudaStream_t st) {
+  return launch_dim<C, Q, P, NQ, NP, 1, false>(a, dim, st);
+}
+// Two, by whether the tables have room for items of more than HOLD key tiles.
+template <class C, class Q, class P>
+int launch_two(const Args& a, int dim, cudaStream_t st) {
+  constexpr int64_t keys = int64_t{Cfg<C, Q, P, 1, 1, 2, 64, true>::HOLD} * kKeys;
+  return int64_t{a.table_width} * a.page_size > keys
+             ? launch_dim<C, Q, P, 1, 1, 2, true>(a, dim, st)
+             : launch_dim<C, Q, P, 1, 1, 2, false>(a, dim, st);
 }
 
 }  // namespace
@@ -1133,15 +1191,15 @@ int launch_dim(const Args& a, int dim, cudaStream_t st) {
 int launch_attn_chunk(const attn::Args& a, int cache_type, int dim, cudaStream_t st) {
   const bool f32 = a.q_type == LP_F32, f16 = a.q_type == LP_F16;
   if (cache_type == LP_F16)  // a bf16 query is exact in scaled fp16
-    return f32 ? launch_dim<CF16, CF16, CF16, 2, 2, 1>(a, dim, st)
-               : launch_dim<CF16, CF16, CF16, 1, 1, 2>(a, dim, st);
+    return f32 ? launch_one<CF16, CF16, CF16, 2, 2>(a, dim, st)
+               : launch_two<CF16, CF16, CF16>(a, dim, st);
   if (cache_type == LP_BF16)
-    return f32   ? launch_dim<CBF16, CBF16, CBF16, 3, 3, 1>(a, dim, st)
-           : f16 ? launch_dim<CBF16, CBF16, CBF16, 2, 2, 1>(a, dim, st)
-                 : launch_dim<CBF16, CBF16, CBF16, 1, 1, 2>(a, dim, st);
-  return f32   ? launch_dim<CI8, CF16, CBF16, 2, 3, 1>(a, dim, st)
-         : f16 ? launch_dim<CI8, CF16, CBF16, 1, 2, 1>(a, dim, st)
-               : launch_dim<CI8, CBF16, CBF16, 1, 1, 2>(a, dim, st);
+    return f32   ? launch_one<CBF16, CBF16, CBF16, 3, 3>(a, dim, st)
+           : f16 ? launch_one<CBF16, CBF16, CBF16, 2, 2>(a, dim, st)
+                 : launch_two<CBF16, CBF16, CBF16>(a, dim, st);
+  return f32   ? launch_one<CI8, CF16, CBF16, 2, 3>(a, dim, st)
+         : f16 ? launch_one<CI8, CF16, CBF16, 1, 2>(a, dim, st)
+               : launch_two<CI8, CBF16, CBF16>(a, dim, st);
 }
 
 unsigned int take_error_attn_chunk() {

@@ -110,3 +110,55 @@ def test_infinities_of_long_items_before_many_short_ones(x, cache, heads, kv):
     ok = ~inf
     d = (out.double() - o).abs()
     assert bool((d <= R.tolerance(o, amp, big, out.dtype))[ok].all())
+
+
+@pytest.mark.parametrize("x,cache", [("fp16", "fp16"), ("bf16", "fp16")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunk_sums_over_hundreds_of_thousands_of_keys(x, cache, dim):
+    """16-bit results take one rounding of the output and one of each weight; what the tensor
+    cores' sums are cut off by has to stay well below that: 1024 products of 16 keys, each cut
+    by less than 2^-23 of a sum that is half the whole on average."""
+    out, o, amp, big = run(positive(300000, 128, 160, x, cache, dim, heads=2), 4)
+    tol = R.tolerance(o, amp, big, out.dtype) + 1024 * 2.0 ** -24 * amp
+    d = (out.double() - o).abs()
+    assert bool((d <= tol).all()), float((d / o).max())
+
+
+@pytest.mark.parametrize("x,cache,keys,dims", [("fp16", "fp16", 40000, (64, 96, 128)),
+                                               ("bf16", "bf16", 280000, (64, 128)),
+                                               ("bf16", "int8", 150000, (64,))])
+@pytest.mark.parametrize("requests", [1, 42])
+def test_long_chunks_whose_maxima_grow(x, cache, keys, dims, requests):
+    """Sums that leave tensor memory in parts: keys that grow along the context, so that the
+    running maximum moves after each part, items in one CTA and cut between CTAs."""
+    for dim in dims:
+        m = positive(keys, 100, requests, x, cache, dim, heads=4)
+        c = m["cache"]
+        g = torch.Generator(device="cuda")
+        g.manual_seed(dim)
+        sign = torch.randint(0, 2, c.v.shape[:2], generator=g, device="cuda")[..., None, None] * 2 - 1
+        c.v.mul_(sign.to(c.v.dtype))
+        ramp = torch.linspace(0.2, 3.0, keys // 64 + 1, device="cuda")[:c.pages, None, None]
+        if cache == "int8":
+            c.kScales.mul_(ramp)
+        else:
+            c.k.mul_(ramp[..., None].to(c.k.dtype))
+        m["q"].mul_(30)
+        for window in (0, keys - 3000):
+            out, o, amp, big = run(m, min(requests, 2), window=window)
+            tol = R.tolerance(o, amp, big, out.dtype) + 2.0 ** -13 * amp
+            assert bool(((out.double() - o).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("x,cache", [("fp16", "fp16"), ("bf16", "fp16"), ("bf16", "bf16"),
+                                     ("bf16", "int8")])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_short_requests_in_tables_with_room_for_long_ones(x, cache, dim):
+    """The table's width may choose the kernel; the results do not show it."""
+    m = R.make(41, [(0, 70), (5, 33), (130, 129), (300, 1), (511, 250)], 4, 2, dim, 16, x, cache,
+               tail=math.nan)
+    narrow = R.check(m, window=200, sinks=3)
+    wide = torch.full((5, 10000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :m["table"].shape[1]] = m["table"]
+    m["table"] = wide[:, :9000]
+    assert torch.equal(R.check(m, window=200, sinks=3), narrow)
