@@ -402,8 +402,11 @@ typedef struct lp_rows {
  * (requests + 1: first flat token of each request), seq_lens (ctx + new),
  * and for each flat token its slot and position, -1 past the last token and
  * (the slot) where there is no page; free_head_out = the next free entry.
- * positions may be null.  free_head_out must not be free_head: the two
- * alternate from step to step.  Negative lengths count as 0. */
+ * positions may be null.  What is written (tables, starts, lengths, slots,
+ * positions, the next free entry) must not overlap anything else that the
+ * call is given, or it is refused (LP_ERR_ARG): seq_lens and free_head_out
+ * alternate with ctx_lens and free_head from step to step.  Negative lengths
+ * count as 0. */
 int lp_assign_pages(const int32_t *ctx_lens, int64_t ctx_lens_len, const int32_t *new_lens,
                     int64_t new_lens_len, int64_t page_size, const int32_t *free_pages,
                     int64_t free_pages_len, const int32_t *free_head, int32_t *block_tables,

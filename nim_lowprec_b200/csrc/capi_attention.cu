@@ -36,6 +36,24 @@ cudaStream_t S(lp_stream_t s) {
 
 bool bad(const void* p, int64_t len) { return len > 0 && p == nullptr; }
 
+// Rows of `width` bytes, `stride` apart (contiguous memory is one row).
+struct Span {
+  uintptr_t p;
+  uint64_t rows, width, stride;
+};
+Span span(const void* p, int64_t n, int64_t size) {
+  return {reinterpret_cast<uintptr_t>(p), n > 0 ? 1u : 0u, static_cast<uint64_t>(n * size), 0};
+}
+// Whether a byte of `rows` is one of `one`'s, which is contiguous.
+bool overlap(const Span& rows, const Span& one) {
+  const uintptr_t p = rows.p, b = one.p, e = one.p + one.width;
+  if (!rows.rows || !rows.width || !one.rows || e <= p) return false;
+  // the last row that begins before one's end
+  uint64_t r = rows.rows - 1;
+  if (r && rows.stride) r = std::min(r, (e - 1 - p) / rows.stride);
+  return p + r * rows.stride + rows.width > b;
+}
+
 int64_t elem_size(int t) { return t == LP_F32 ? 4 : t == LP_I8 ? 1 : 2; }
 
 int check_cache(const lp_kv_cache* c) {
@@ -115,8 +133,24 @@ int lp_assign_pages(const int32_t* ctx_lens, int64_t ctx_lens_len, const int32_t
   LP_REQUIRE(positions == nullptr || positions_len == slots_len);
   if (bad(ctx_lens, n) || bad(new_lens, n) || bad(seq_lens, n) || !q_start) return LP_ERR_ARG;
   if (bad(free_pages, free_pages_len) || bad(block_tables, n * table_width)) return LP_ERR_ARG;
-  if (bad(slots, slots_len) || !free_head || !free_head_out || free_head == free_head_out)
-    return LP_ERR_ARG;
+  if (bad(slots, slots_len) || !free_head || !free_head_out) return LP_ERR_ARG;
+  // Every block reads all the lengths, and tokens read the free list, while others write
+  // their results: nothing that is written may lie on anything else.
+  const Span in[] = {span(ctx_lens, n, 4), span(new_lens, n, 4), span(free_pages, free_pages_len, 4),
+                     span(free_head, 1, 4)};
+  const Span out[] = {span(q_start, n + 1, 4), span(seq_lens, n, 4), span(slots, slots_len, 8),
+                      span(positions, positions ? slots_len : 0, 4), span(free_head_out, 1, 4)};
+  const Span table{reinterpret_cast<uintptr_t>(block_tables), static_cast<uint64_t>(n),
+                   static_cast<uint64_t>(table_width) * 4, static_cast<uint64_t>(table_stride) * 4};
+  for (const Span& i : in)
+    if (overlap(table, i)) return LP_ERR_ARG;
+  for (const Span& o : out) {
+    if (overlap(table, o)) return LP_ERR_ARG;
+    for (const Span& i : in)
+      if (overlap(i, o)) return LP_ERR_ARG;
+    for (const Span& x : out)
+      if (&x != &o && overlap(x, o)) return LP_ERR_ARG;
+  }
   return lp::launch_assign_pages(ctx_lens, new_lens, n, page_size, free_pages, free_pages_len,
                                  free_head, block_tables, table_stride, table_width, q_start,
                                  seq_lens, slots, slots_len, positions, free_head_out, S(stream));

@@ -112,6 +112,45 @@ def test_page_assignments_that_are_refused(change, status):
     assert assign(**change) == status
 
 
+INPUTS = dict(ctx=3, new=3, free=9, head=1)  # and their lengths
+OUTPUTS = dict(qs=4, seq=3, slots=7, pos=7, out=1)
+
+
+def apart(**kw):
+    """assign() with every array in a place of its own."""
+    a = {name: ctypes.c_void_p((16 + i) << 20)
+         for i, name in enumerate([*INPUTS, *OUTPUTS, "tables"])}
+    a.update(kw)
+    return a
+
+
+def test_page_assignments_refuse_outputs_on_other_arrays():
+    """Blocks read the lengths and the free list while others write: an output on an input, as
+    in lengths updated in place, would be a race."""
+    at = apart()
+    for o, n in OUTPUTS.items():
+        size = 8 if o == "slots" else 4
+        for other, length in (*INPUTS.items(), *OUTPUTS.items()):
+            if other == o:
+                continue
+            p, bytes_ = at[other].value, length * (8 if other == "slots" else 4)
+            assert assign(**apart(**{o: at[other]})) == N.LP_ERR_ARG, (o, other)
+            # and by one byte at either end
+            for q in (p + bytes_ - 1, p - n * size + 1):
+                assert assign(**apart(**{o: ctypes.c_void_p(q)})) == N.LP_ERR_ARG, (o, other)
+
+
+def test_page_assignments_refuse_tables_on_other_arrays():
+    """Three rows of four entries, ten apart: what lies between the rows is not theirs."""
+    base = apart()["tables"].value
+    for name, n in (*INPUTS.items(), *OUTPUTS.items()):
+        size = 4 * n * (2 if name == "slots" else 1)
+        for row in range(3):
+            for q in (base + 40 * row, base + 40 * row + 15, base + 40 * row - size + 1):
+                a = apart(**{name: ctypes.c_void_p(q)})
+                assert assign(**a, stride=10) == N.LP_ERR_ARG, (name, row)
+
+
 def attend(c=None, q=None, out=None, **kw):
     c, q, out = c or cache(), q or rows(heads=4, token_stride=256), out or rows(heads=4)
     a = dict(tables=P, width=4, stride=4, qs=P, qs_n=4, seq=P, seq_n=3, q=ctypes.byref(q),

@@ -250,3 +250,38 @@ def test_empty_calls():
     L.loadKV(c2, torch.arange(7, device="cuda"), got, torch.empty_like(x))
     want, s = expected(x, "int8")
     assert same(got, want.float() * s[..., None])
+
+
+def test_assign_arrays_side_by_side():
+    """Arrays that touch, and one between the rows of the table, are taken; lengths updated in
+    place are not."""
+    ctx, new, ps, free = [5, 0, 31, 16], [3, 40, 1, 0], 8, list(range(20, 5, -1))
+    n, tokens, width = len(ctx), sum(new) + 2, 7
+    buf = torch.full((400,), -1, dtype=torch.int32, device="cuda")
+    at = [0]
+
+    def take(k, values=()):
+        t = buf[at[0]:at[0] + k]
+        at[0] += k
+        if values:
+            t.copy_(i32(list(values)))
+        return t
+    c, a, f, head = take(n, ctx), take(n, new), take(len(free), free), take(1, [1])
+    seq, qs, pos = take(n), take(n + 1), take(tokens)
+    take(at[0] % 2)
+    slots = take(2 * tokens).view(torch.int64)
+    rows = take(n * (width + 3)).view(n, width + 3)
+    table, out = rows[:, :width], rows[1, width:width + 1]
+    start = np.full((n, width), -1, np.int32)
+    for b, x in enumerate(ctx):
+        start[b, :-(-x // ps)] = 30 + b
+    table.copy_(torch.from_numpy(start))
+    want = R.assign_pages(ctx, new, ps, free, 1, start.copy(), tokens)
+    L.assignPages(c, a, ps, f, head, table, qs, seq, slots, pos, out)
+    for name, got in dict(table=table, qstart=qs, seq=seq, slots=slots, pos=pos, head=out).items():
+        assert np.array_equal(got.cpu().numpy().reshape(-1), np.asarray(want[name]).reshape(-1)), name
+    assert c.tolist() == ctx and a.tolist() == new and f.tolist() == free and head.tolist() == [1]
+    for wrong in (dict(seq=c), dict(seq=a), dict(out=head), dict(qs=buf[n - 1:2 * n])):
+        k = {**dict(seq=seq, qs=qs, out=out), **wrong}
+        with pytest.raises(L._native.NativeError):
+            L.assignPages(c, a, ps, f, head, table, k["qs"], k["seq"], slots, pos, k["out"])
