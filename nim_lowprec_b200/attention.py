@@ -180,16 +180,17 @@ def pagedAttention(cache, blockTables, qStart, seqLens, q, out, scale=None, wind
     defaults to headDim ** -0.5.  lse (fp32 [tokens, heads] or None) receives the logarithm of
     each row's sum of exponentials.  A row that sees no key gives zeros (lse -inf).
 
-    Without `workspace` one is kept per device and stream; pass your own
-    (attentionWorkspace()) to graphs that may be replayed on other streams."""
+    Without `workspace` one is kept per device and stream.  A call that is captured into a graph
+    must bring its own (attentionWorkspace(), made before the capture; ``RuntimeError``): the
+    graph may be replayed on any stream, beside calls and graphs that use the kept one."""
     fast, index = _fast(), cache._index
     if workspace is None:
+        if fast.capturing(index):
+            raise RuntimeError("pagedAttention: a captured call needs a workspace of its own "
+                               "(attentionWorkspace(), made before the capture)")
         key = (index, fast.current_stream(index))
         workspace = _workspaces.get(key)
         if workspace is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("pagedAttention: a captured call needs a workspace of its own "
-                                   "(attentionWorkspace(), made before the capture)")
             workspace = _workspaces[key] = attentionWorkspace(cache.device)
     status = fast.paged_attention(cache._ref, index, cache._dim, blockTables, qStart, seqLens, q, out,
                                   cache._scale if scale is None else scale, window, sinks, lse, workspace)

@@ -12,6 +12,7 @@
 #include <ATen/core/Tensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdarg>
@@ -210,6 +211,17 @@ PyObject* current_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Whether a device's current stream is being captured into a graph.
+PyObject* capturing(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return entry(n, 1, [&] {
+    const int dev = static_cast<int>(number(a[0]));
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(dev).stream(), &status) != cudaSuccess)
+      (void)cudaGetLastError();  // (a launch would say the same)
+    return PyBool_FromLong(status != cudaStreamCaptureStatusNone);
+  });
+}
+
 #define LP_METHOD(name, f) \
   { name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
@@ -218,6 +230,7 @@ PyMethodDef methods[] = {
     LP_METHOD("load_kv", (move_kv<false>)),
     LP_METHOD("paged_attention", paged_attention),
     LP_METHOD("current_stream", current_stream),
+    LP_METHOD("capturing", capturing),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, methods,

@@ -369,3 +369,48 @@ def test_a_capture_without_a_workspace_is_refused():
             L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out)
     torch.cuda.synchronize()
     R.check(m)
+
+
+def test_a_capture_after_calls_on_its_stream_is_refused_without_a_workspace():
+    """The workspace that such calls left behind belongs to the stream, not to a graph that may
+    be replayed beside it."""
+    m = R.make(26, [(300, 1)], 4, 2, 64, 16)
+    out = torch.empty_like(m["q"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(g, stream=side):
+            out.zero_()
+            L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out)
+    torch.cuda.synchronize()
+    R.check(m)
+
+
+def test_graphs_with_workspaces_of_their_own_run_side_by_side():
+    m = R.make(27, [(9000, 1), (300, 40), (7000, 1)], 8, 2, 128, 16, "bf16", "bf16")
+    first = R.check(m)
+    capture, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    outs, spaces, graphs = [], [], []
+    for _ in streams:
+        outs.append(torch.zeros_like(first))
+        spaces.append(L.attentionWorkspace())
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=capture):
+            for _ in range(20):
+                L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], outs[-1],
+                                 workspace=spaces[-1])
+    for _ in range(5):
+        for s, g, o in zip(streams, graphs, outs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                o.fill_(math.nan)
+                g.replay()
+        eager = torch.empty_like(first)
+        L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], eager)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, first) and all(torch.equal(o, first) for o in outs)
