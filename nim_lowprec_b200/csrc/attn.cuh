@@ -360,6 +360,46 @@ __device__ __forceinline__ float bad_value(const Args& a, int b, int h, int page
     v = C::to_float(reinterpret_cast<const uint16_t*>(a.v.data)[row]);
   return finite(v) ? 0.0f : v;
 }
+// Of values d .. d + 31 of key j: those that are +inf or NaN, and -inf or NaN, a
+// bit each.
+template <class C>
+__device__ __forceinline__ void bad_columns(const Args& a, int h, int page, int j, int d,
+                                            uint32_t& up, uint32_t& down) {
+  const int off = page_offset(a, j);
+  const int64_t row = page * a.v.page + off * a.v.token + h * a.v.head + d;
+  up = down = 0;
+  if constexpr (C::kInt8) {
+    const float s = a.v.scales[page * a.v.spage + off * a.v.stoken + h * a.v.shead];
+    if (finite(s)) return;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(a.v.data + row);  // (rows are aligned)
+    uint32_t above = 0, below = 0;  // codes over and under 0
+#pragma unroll 1
+    for (int e = 0; e < 32; e += 4) {
+      const uint32_t w = __ldg(p++);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int code = static_cast<int8_t>(w >> (8 * y) & 255u);
+        above |= (code > 0 ? 1u : 0u) << (e + y);
+        below |= (code < 0 ? 1u : 0u) << (e + y);
+      }
+    }
+    // a code of 0 gives NaN, and so does a scale
+    up = s > 0.0f ? ~below : s < 0.0f ? ~above : 0xffffffffu;
+    down = s > 0.0f ? ~above : s < 0.0f ? ~below : 0xffffffffu;
+  } else {
+    constexpr uint32_t kInf = C::kBf16 ? 0x7f80u : 0x7c00u;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(a.v.data + 2 * row);  // (rows are aligned)
+#pragma unroll 1
+    for (int e = 0; e < 32; e += 2) {
+      const uint32_t w = __ldg(p++);
+      const uint32_t x = w & 0xffffu, y = w >> 16;
+      up |= ((x & 0x7fffu) > kInf || x == kInf ? 1u << e : 0u) |
+            ((y & 0x7fffu) > kInf || y == kInf ? 2u << e : 0u);
+      down |= (x >= (kInf | 0x8000u) || (x < 0x8000u && x > kInf) ? 1u << e : 0u) |
+              (y >= (kInf | 0x8000u) || (y < 0x8000u && y > kInf) ? 2u << e : 0u);
+    }
+  }
+}
 // Whether a row at position pos sees key j (the page aside).
 __device__ __forceinline__ bool sees(const Args& a, const Request& r, int pos, int j) {
   return j <= pos && j < r.limit && (a.window == 0 || j > pos - a.window || j < a.sinks);

@@ -916,9 +916,38 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     // from here on the reference in units of log2 (sums carry kUp, like O)
     m = m == -INFINITY ? -INFINITY : m * c;
 
-    // 32 columns of this CTA's outputs, with what clear_bad took from keys that
-    // the row sees
-    const int nbad = sh.nbad[item % kPlaces];
+    // What clear_bad took from keys that the row sees: per block of 32 columns, those
+    // with a +inf or NaN and those with a -inf or NaN.  A lane looks at one key for all
+    // the warp's rows, so 32 keys cost a few trips to L2.  (Each row for itself took
+    // 1.6 us a key and block: at 300000 keys in an item, all of them to be looked at,
+    // longer than the other roles wait.  One row tile keeps that form where few tiles
+    // are noted: without it the compiler gives the key loop fewer registers, five
+    // fp32 prompts over an int8 cache 324 us with both forms, 366 with one.)
+    uint32_t up[OB] = {}, down[OB] = {};
+    const int nbad = live && warp_ok ? sh.nbad[item % kPlaces] : 0;
+#pragma unroll 1
+    for (int i = 0; i < 4 * (nbad > kBad ? w.n : kTwo ? nbad : 0); ++i) {
+      const int key0 = (nbad > kBad ? w.key(i / 4) : sh.badkey[item % kPlaces][i / 4]) + 32 * (i % 4);
+      const int j = key0 + (threadIdx.x & 31);
+      const int page = j < w.rq.limit ? page_of(a, w.b, j) : -1;
+      uint32_t see = __ballot_sync(0xffffffffu, page >= 0) & below(pos + 1 - key0) &
+                     (~below(lo - key0) | below(a.sinks - key0));
+      if (!ok) see = 0;
+#pragma unroll
+      for (int b = 0; b < OB; ++b) {
+        if (d0 + 32 * b >= d1) break;
+        uint32_t u = 0, d = 0;
+        if (page >= 0) bad_columns<C>(a, w.head, page, j, d0 + 32 * b, u, d);
+        uint32_t keys = __ballot_sync(0xffffffffu, (u | d) != 0);
+        while (keys) {
+          const int s = __ffs(keys) - 1;
+          keys &= keys - 1;
+          const uint32_t us = __shfl_sync(0xffffffffu, u, s), ds = __shfl_sync(0xffffffffu, d, s);
+          if (see >> s & 1u) up[b] |= us, down[b] |= ds;
+        }
+      }
+    }
+    // 32 columns of this CTA's outputs
     auto column_block = [&](int b, float* v) {
       if constexpr (kTwo) {
         uint32_t u[32];
@@ -936,15 +965,24 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = o[32 * b + e];
       }
-#pragma unroll 1
-      for (int i = 0; i < (nbad <= kBad ? nbad : w.n); ++i) {
-        const int key0 = nbad <= kBad ? sh.badkey[item % kPlaces][i] : w.key(i);
-#pragma unroll 1
-        for (int j = key0; j < key0 + kKeys; ++j) {
-          const int page = ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
-          if (page < 0) continue;
+      if (up[b] | down[b]) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += bad_value<C>(a, w.b, w.head, page, j, d0 + 32 * b + e);
+        for (int e = 0; e < 32; ++e) {
+          if (up[b] >> e & 1u) v[e] += INFINITY;
+          if (down[b] >> e & 1u) v[e] -= INFINITY;
+        }
+      }
+      if constexpr (!kTwo) {
+#pragma unroll 1
+        for (int i = 0; i < (nbad > kBad ? 0 : nbad); ++i) {
+          const int key0 = sh.badkey[item % kPlaces][i];
+#pragma unroll 1
+          for (int j = key0; j < key0 + kKeys; ++j) {
+            const int page = ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
+            if (page < 0) continue;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] += bad_value<C>(a, w.b, w.head, page, j, d0 + 32 * b + e);
+          }
         }
       }
     };

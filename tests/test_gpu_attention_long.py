@@ -162,3 +162,43 @@ def test_short_requests_in_tables_with_room_for_long_ones(x, cache, dim):
     wide[:, :m["table"].shape[1]] = m["table"]
     m["table"] = wide[:, :9000]
     assert torch.equal(R.check(m, window=200, sinks=3), narrow)
+
+
+@pytest.mark.parametrize("x,cache,dim", [("bf16", "bf16", 128), ("fp32", "fp16", 64),
+                                         ("fp32", "int8", 64)])
+def test_infinities_everywhere_in_long_contexts_with_holes(x, cache, dim):
+    """Every tile is seen in part and holds infinities, in all items at once: what that costs
+    stays far from the time after which the kernel's roles give up waiting for one another."""
+    keys, requests, new = 600000, 148, 128
+    pages = 64
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k = torch.zeros(pages, 16, 1, dim, device="cuda", dtype=R.DT[cache])
+    v = torch.ones_like(k)
+    col = torch.arange(dim, device="cuda") % 4
+    if cache == "int8":
+        v[..., col == 1] = -1
+        v[..., col == 3] = 0
+        s = torch.full((pages, 16, 1), math.inf, device="cuda")
+        c = L.KVCache(k, v, torch.ones_like(s), s)
+        want = torch.tensor([math.inf, -math.inf, math.inf, math.nan], device="cuda")
+    else:
+        v[..., col == 0] = math.inf
+        v[..., col == 1] = -math.inf
+        v[:, ::2, :, col == 2] = math.inf
+        v[:, 1::2, :, col == 2] = -math.inf
+        c = L.KVCache(k, v)
+        want = torch.tensor([math.inf, -math.inf, math.nan, 1.0], device="cuda")
+    table = torch.randint(0, pages, (requests, keys // 16), **i32)
+    table[:, ::3] = -1
+    q = torch.zeros(requests * new, 1, dim, device="cuda", dtype=R.DT[x])
+    out = torch.full_like(q, 7.0)
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    L.pagedAttention(c, table, torch.arange(requests + 1, **i32) * new,
+                     torch.full((requests,), keys, **i32), q, out)
+    end.record()
+    end.synchronize()
+    assert L._native.device_error() == 0
+    assert torch.allclose(out.float(), want[col].expand_as(out), rtol=2.0 ** -18, atol=0,
+                          equal_nan=True)
+    assert start.elapsed_time(end) < 1000.0
