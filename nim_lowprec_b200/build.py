@@ -40,14 +40,22 @@ BINDING = os.path.join(HERE, "_torch_binding.so")
 
 
 def build_binding(force: bool = False) -> None:
-    """_torch_binding.so against the installed torch (skipped without torch)."""
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    if not force and not _stale(BINDING, [src, OUT, os.path.join(INCLUDE, "lowprec_cuda.h")]):
-        return
+    """_torch_binding.so against the installed torch; skipped without torch, and with a torch
+    that has no CUDA.  A binding for another torch or Python is built again."""
     try:
         import torch
         from torch.utils import cpp_extension
     except ImportError:
+        return
+    if torch.version.cuda is None:
+        print("_torch_binding: skipped, the installed torch is without CUDA")
+        return
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    stamp = os.path.join(OBJDIR, "torch_binding.for")
+    this = f"torch {torch.__version__}, Python {sys.version}"
+    known = open(stamp).read() if os.path.exists(stamp) else ""
+    if not force and known == this and not _stale(
+            BINDING, [src, OUT, os.path.join(INCLUDE, "lowprec_cuda.h")]):
         return
     import sysconfig
     cuda = os.path.dirname(os.path.dirname(NVCC))
@@ -60,6 +68,8 @@ def build_binding(force: bool = False) -> None:
            "-l:" + os.path.basename(OUT), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
            "-Wl,-rpath,$ORIGIN"]
     subprocess.run(cmd, check=True)
+    with open(stamp, "w") as f:
+        f.write(this)
 
 
 def sources():
