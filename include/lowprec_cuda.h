@@ -381,7 +381,7 @@ typedef struct lp_kv_cache {
   int64_t k_strides[3], v_strides[3];
   int64_t k_scale_strides[3], v_scale_strides[3];
   int32_t dtype;    /* LP_F16, LP_BF16, LP_I8 */
-  int32_t head_dim; /* a multiple of 16, at most 256; attention: 64, 96, 128 */
+  int32_t head_dim; /* store, load: a multiple of 16, at most 256; attention: 64, 96, 128 */
 } lp_kv_cache;
 
 /* Rows of head_dim elements: row (token, head) at
@@ -440,11 +440,25 @@ int lp_paged_attention_workspace(int64_t *bytes);
  * (an entry in [0, pages)), and, with window > 0, j > p - window or
  * j < sinks.  Query head h reads key head h div (heads / kv_heads).
  *   out = sum_j exp(s_j) v_j / sum_j exp(s_j),  s_j = scale * (q . k_j)
- * in fp32 inside, rounded once to out's type (= q's); lse (may be null;
- * tokens x heads) = log sum_j exp(s_j).  A row that sees no key gives zeros
- * and -inf.  Keys that a row does not see do not touch it, whatever they
- * hold.  Rows of q outside every request are left alone in out.  out must
- * not overlap q. */
+ * lse (may be null; tokens x heads) = log sum_j exp(s_j).  out has q's type.
+ *
+ * Scores, maxima, sums and outputs are fp32 and out is rounded once from
+ * them, but the products take 16-bit operands.  Queries and cached elements
+ * are exact in those, or (fp32 queries) split into parts of 22 bits or more.
+ * Weights exp(s_j - max), with int8 pages times the value's scale, are split
+ * likewise for fp32 results.  For 16-bit results they are split into two
+ * parts of 16 bits together (22 over fp16 pages) in calls of few rows.  In
+ * calls of chunks (24 rows of q x group per request and key head on average;
+ * 64 where requests x key heads < 32) each is rounded once, to fp16 over
+ * fp16 pages and to bf16 for bf16 results over bf16 and int8 pages (fp16
+ * results over those: two bf16 parts).  So a token's 16-bit result may differ
+ * by that rounding between a call of its own and a chunk.
+ *
+ * A row that sees no key gives zeros and -inf.  Keys that a row does not see
+ * do not touch it, whatever they hold.  Values that are not finite make the
+ * results that see them not finite, where an infinity may also come out as a
+ * NaN; keys that are not finite may make their rows NaN.  Rows of q outside
+ * every request are left alone in out.  out must not overlap q. */
 int lp_paged_attention(const lp_kv_cache *cache, const int32_t *block_tables, int64_t table_width,
                        int64_t table_stride, const int32_t *q_start, int64_t q_start_len,
                        const int32_t *seq_lens, int64_t seq_lens_len, const lp_rows *q,

@@ -64,7 +64,8 @@ class KVCache:
     """Pages of keys and values, [pages, pageSize, kvHeads, headDim] each, in fp16, bf16 or
     int8.  The head dimension is contiguous; the other strides are free (a cache that keeps
     heads outside of tokens is passed as ``t.transpose(1, 2)``), rows start on 16-byte
-    boundaries.  int8 pages come with fp32 scales [pages, pageSize, kvHeads], one per (token,
+    boundaries.  headDim: storeKV and loadKV take multiples of 16 up to 256, pagedAttention
+    64, 96 and 128 alone.  int8 pages come with fp32 scales [pages, pageSize, kvHeads], one per (token,
     head).  The tensors stay the caller's; the cache keeps references to them."""
 
     def __init__(self, k, v, kScales=None, vScales=None):
@@ -106,7 +107,7 @@ class KVCache:
 
     @classmethod
     def allocate(cls, pages, pageSize, kvHeads, headDim, dtype, device="cuda"):
-        """A new cache, zeroed."""
+        """A new cache, zeroed.  (headDim: see above; pagedAttention takes 64, 96 and 128.)"""
         def new(*shape, dt):
             return torch.zeros(*shape, dtype=dt, device=device)
         k, v = (new(pages, pageSize, kvHeads, headDim, dt=dtype) for _ in range(2))
@@ -177,8 +178,10 @@ def pagedAttention(cache, blockTables, qStart, seqLens, q, out, scale=None, wind
     qStart[b]:qStart[b + 1], the last of them at position seqLens[b] - 1, its keys those that
     blockTables[b] holds.  A token at position p sees key j if j <= p and, with a window,
     j > p - window or j < sinks.  heads is a multiple of the cache's kvHeads.  `scale`
-    defaults to headDim ** -0.5.  lse (fp32 [tokens, heads] or None) receives the logarithm of
-    each row's sum of exponentials.  A row that sees no key gives zeros (lse -inf).
+    defaults to headDim ** -0.5.  out must not share memory with q.  lse (fp32 [tokens, heads] or None) receives the logarithm of
+    each row's sum of exponentials.  A row that sees no key gives zeros (lse -inf).  fp32
+    results are fp32 throughout; 16-bit ones round each weight once to 16 bits in calls of
+    chunks (include/lowprec_cuda.h says which).
 
     Without `workspace` one is kept per device and stream.  A call that is captured into a graph
     must bring its own (attentionWorkspace(), made before the capture; ``RuntimeError``): the
