@@ -40,19 +40,23 @@
 // registers; long ones pay 2 to 3 %.)
 //
 // What bounds it: 16-bit queries the softmax and the products in turn.  4096
-// tokens over 16384 cached, 32 heads on 8 key heads of 128, bf16: 1.13 to 1.2 ms by
-// itself (1030 to 1090 TFLOP/s, 63 to 67 % of a cuBLAS bf16 product's rate), 1.28 to
-// 1.32 ms back to back under the power limit; the special-function unit alone needs 0.5 ms, the
+// tokens over 16384 cached, 32 heads on 8 key heads of 128, bf16: 1.18 to 1.2 ms by
+// itself (1030 to 1050 TFLOP/s, 63 to 64 % of a cuBLAS bf16 product's rate), 1.28 to
+// 1.34 ms back to back under the power limit; the special-function unit alone needs 0.5 ms, the
 // products 0.76.  Tried and slower there: a third of the exponentials by a
 // polynomial on the fp32 pipes (+3 %), the weights' first half handed over early
 // (+0.4 %), the row's maximum chunk by chunk in one pass (+9 %).  fp32 over an
 // int8 cache: 5 products where 16 bits take 2, and shared memory, which they and
 // the loaders share (350 KB per key tile, 2750 cycles of about 6700): five prompts
-// of up to 700 tokens over up to 4700 keys 0.31 ms.
+// of up to 700 tokens over up to 4700 keys 0.32 ms.  Registers: the softmax role and
+// the one that issues the products spill (in kernels of one role each, bf16 128
+// dimensions, 120 and 304 bytes of stores; fp32 over int8 1508 and 276; the loaders
+// none), and what the compiler keeps in the key loop changes with code far from it.
 //
 // The running maximum moves only when a row's grows by more than 2^8 (the
 // weights stay below 2^8 times 1, or 2^15 with fp16's extra 2^7): the sums are
-// the same and O is rescaled a few times per row rather than per key tile.
+// the same and O is rescaled a few times per row rather than per key tile (a
+// published refinement of the running-maximum softmax).
 #include <type_traits>
 
 #include "attn.cuh"

@@ -5,8 +5,8 @@
 //
 // One pass over the keys with a running maximum and sum per row.  What bounds
 // it is the cache's bytes, so the design serves the loads:
-//   * A CTA takes up to 8 query rows of one key head (all query heads of the
-//     group), so keys and values are read once for the group.  Two CTAs of
+//   * A CTA takes up to 8 query rows of one key head, so keys and values are read
+//     once for a group of up to 8 query heads (twice for 9 to 16, ...).  Two CTAs of
 //     four warps share an SM: one joins its rows while the other streams.
 //   * Each warp streams for itself: steps of 16 to 32 keys (keys and values,
 //     8 KB) go by cp.async into its own ring of 24 KB, two to five steps ahead
@@ -32,11 +32,12 @@
 //     cached byte) off the fp32 pipe; at 8 rows a tile of 128 x N tcgen05
 //     rows would be 94 % padding, and the bytes bound the time either way.
 // Measured: two requests of 131000 keys, 64 heads on 8 key heads of 128, bf16,
-// 199 us (5.4 TB/s, 82 % of a copy's rate; what is missing is the spread of the
+// 200 us (5.4 TB/s, 82 % of a copy's rate; what is missing is the spread of the
 // SMs' shares of the bandwidth, 157 us on average); 32 requests under a window
-// of 4000, heads of 64, 54 us (4.2 TB/s; 16 us of start and join); 53 requests of
-// up to 16000 keys over an int8 cache with fp32 queries, 215 us (3.8 TB/s; issue
-// bound: widening the codes and three parts of the weights).
+// of 4000, heads of 64, 55 us (4.2 TB/s; 16 us of start and join); 53 requests of
+// up to 16000 keys over an int8 cache with fp32 queries, 228 us (3.6 TB/s), with
+// bf16 ones 213: latency at two warps per scheduler, each of which issues every
+// 4 cycles (49 % of the issue slots, 29 % of the tensor pipe, 57 % of DRAM).
 #include <type_traits>
 
 #include "attn.cuh"
