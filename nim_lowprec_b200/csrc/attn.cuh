@@ -318,7 +318,9 @@ struct CI8 {  // codes are widened to fp16, which holds them exactly
 // zeros in shared memory and the tile's first key is noted; afterwards those
 // values are added to the outputs of the rows that do see them, which makes them
 // what the sum over the row's own keys is.  Tiles that all rows see need none of
-// this, and neither do finite values.
+// this, and neither do finite values.  (There an infinity meets its weight's parts
+// one by one, and a part of 0 makes a NaN of it: a row that sees an infinity has a
+// result that is not finite, but not always the infinity.)
 
 // 16 bytes of values; returns whether one was replaced.
 template <class C>
