@@ -401,8 +401,8 @@ typedef struct lp_rows {
  * rows table_stride apart); -1 where the list has run out.  Out: q_start
  * (requests + 1: first flat token of each request), seq_lens (ctx + new),
  * and for each flat token its slot and position, -1 past the last token and
- * (the slot) where there is no page; free_head_out = the next free entry.
- * positions may be null.  What is written (tables, starts, lengths, slots,
+ * (the slot) where there is no page; free_head_out = the next free entry, at
+ * most free_pages_len.  positions may be null.  What is written (tables, starts, lengths, slots,
  * positions, the next free entry) must not overlap anything else that the
  * call is given, or it is refused (LP_ERR_ARG): seq_lens and free_head_out
  * alternate with ctx_lens and free_head from step to step.  Negative lengths

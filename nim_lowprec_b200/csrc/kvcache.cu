@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kAssignThreads) k_assign_pages(const AssignArg
   if (blockIdx.x == 0 && t == 0) {
     a.qstart[a.requests] = static_cast<int32_t>(min(total, static_cast<int64_t>(INT32_MAX)));
     a.free_head_out[0] = static_cast<int32_t>(
-        min(head + s_page[kAssignThreads], max(a.free_len, head)));
+        min(head + s_page[kAssignThreads], a.free_len));
   }
 
   // ---- slots and positions: one token per thread

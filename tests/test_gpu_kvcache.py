@@ -285,3 +285,15 @@ def test_assign_arrays_side_by_side():
         k = {**dict(seq=seq, qs=qs, out=out), **wrong}
         with pytest.raises(L._native.NativeError):
             L.assignPages(c, a, ps, f, head, table, k["qs"], k["seq"], slots, pos, k["out"])
+
+
+@pytest.mark.parametrize("head", [4, 5, 9])
+def test_assign_from_the_end_of_the_free_list(head):
+    """A head at or past the end of the list gives no page, and the next one is its end."""
+    ctx, new, ps = [3, 8], [9, 1], 4
+    table = np.full((2, 6), -1, np.int32)
+    table[0, 0], table[1, :2] = 11, (12, 13)
+    want = R.assign_pages(ctx, new, ps, [7, 6, 5, 4], head, table.copy(), 12)
+    got = run_assign(ctx, new, ps, [7, 6, 5, 4], head, table, 12)
+    for name, w in want.items():
+        assert np.array_equal(got[name].cpu().numpy().reshape(-1), np.asarray(w).reshape(-1)), name
