@@ -132,9 +132,10 @@ def assignPages(ctxLens, newLens, pageSize, freePages, freeHead, blockTables, qS
     taken, in request order, from freePages[freeHead[0]:] and written into blockTables[b]
     (-1 once the list has run out).  Written: qStart [requests + 1], seqLens, and per flat
     token its slot (int64) and position; -1 past the last token and where there is no page.
-    freeHeadOut[0] is the next free entry, at most the list's length.  No output may share memory with an input or
-    another output (``NativeError``): seqLens and freeHeadOut are other tensors than ctxLens
-    and freeHead, and take turns with them from step to step.  positions may be None.  Whole numbers are int32, slots int64."""
+    freeHeadOut[0] is the next free entry, at most the list's length.  No output may share
+    memory with an input or another output (``NativeError``): seqLens and freeHeadOut are other
+    tensors than ctxLens and freeHead, and take turns with them from step to step.  positions
+    may be None.  Whole numbers are int32, slots int64."""
     status = _fast().assign_pages(ctxLens, newLens, pageSize, freePages, freeHead, blockTables, qStart,
                                   seqLens, slots, positions, freeHeadOut)
     if status:
