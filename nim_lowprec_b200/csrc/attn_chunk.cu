@@ -118,6 +118,13 @@ struct Cfg {
   // each cut off, take 0.6e-6 of the sum a tile: up to 0.7e-4 of an fp16 result and
   // 0.6e-3 of a bf16 one, a sixth of what its rounding is.
   static constexpr int HOLD = P::kBf16 ? 1024 : 128;
+  // Cleared values of few tiles are looked for by each row for itself, not by lanes
+  // for all of a warp's rows.  That is slower, but finite caches pay neither, and
+  // which of the two loops is there decides what the compiler keeps in registers in
+  // the key loop: 1536 tokens over 6000, 32/8 heads of 96, bf16 201 us (by lanes 230),
+  // fp16 207 (226); five fp32 prompts over int8 324 (366); but bf16 over int8, heads of
+  // 96, 387 (361), and bf16 heads of 128, 60 short requests, 110 (106).
+  static constexpr bool BY_ROW = TILES == 1 || (D == 96 && !C::kInt8);
 };
 
 template <class F>
@@ -924,13 +931,11 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     // with a +inf or NaN and those with a -inf or NaN.  A lane looks at one key for all
     // the warp's rows, so 32 keys cost a few trips to L2.  (Each row for itself took
     // 1.6 us a key and block: at 300000 keys in an item, all of them to be looked at,
-    // longer than the other roles wait.  One row tile keeps that form where few tiles
-    // are noted: without it the compiler gives the key loop fewer registers, five
-    // fp32 prompts over an int8 cache 324 us with both forms, 366 with one.)
+    // longer than the other roles wait.  BY_ROW keeps that form for few tiles.)
     uint32_t up[OB] = {}, down[OB] = {};
     const int nbad = live && warp_ok ? sh.nbad[item % kPlaces] : 0;
 #pragma unroll 1
-    for (int i = 0; i < 4 * (nbad > kBad ? w.n : kTwo ? nbad : 0); ++i) {
+    for (int i = 0; i < 4 * (nbad > kBad ? w.n : F::BY_ROW ? 0 : nbad); ++i) {
       const int key0 = (nbad > kBad ? w.key(i / 4) : sh.badkey[item % kPlaces][i / 4]) + 32 * (i % 4);
       const int j = key0 + (threadIdx.x & 31);
       const int page = j < w.rq.limit ? page_of(a, w.b, j) : -1;
@@ -976,7 +981,7 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
           if (down[b] >> e & 1u) v[e] -= INFINITY;
         }
       }
-      if constexpr (!kTwo) {
+      if constexpr (F::BY_ROW) {
 #pragma unroll 1
         for (int i = 0; i < (nbad > kBad ? 0 : nbad); ++i) {
           const int key0 = sh.badkey[item % kPlaces][i];
