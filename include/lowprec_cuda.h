@@ -455,9 +455,10 @@ int lp_paged_attention_workspace(int64_t *bytes);
  * by that rounding between a call of its own and a chunk.
  *
  * A row that sees no key gives zeros and -inf.  Keys that a row does not see
- * do not touch it, whatever they hold.  Values that are not finite make the
- * results that see them not finite, where an infinity may also come out as a
- * NaN; keys that are not finite may make their rows NaN.  Rows of q outside
+ * do not touch it, whatever they hold.  Values that are not finite give the
+ * rows that see them the sum's infinity or NaN (a NaN too where a chunk's one
+ * part of the weight is 0: under 2^-32 of the row's largest in fp16, 2^-126 in
+ * bf16); keys that are not finite may make their rows NaN.  Rows of q outside
  * every request are left alone in out.  out must not overlap q. */
 int lp_paged_attention(const lp_kv_cache *cache, const int32_t *block_tables, int64_t table_width,
                        int64_t table_stride, const int32_t *q_start, int64_t q_start_len,

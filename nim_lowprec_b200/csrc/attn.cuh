@@ -318,9 +318,10 @@ struct CI8 {  // codes are widened to fp16, which holds them exactly
 // zeros in shared memory and the tile's first key is noted; afterwards those
 // values are added to the outputs of the rows that do see them, which makes them
 // what the sum over the row's own keys is.  Tiles that all rows see need none of
-// this, and neither do finite values.  (There an infinity meets its weight's parts
-// one by one, and a part of 0 makes a NaN of it: a row that sees an infinity has a
-// result that is not finite, but not always the infinity.)
+// this, and neither do finite values.  But where a weight has several parts, an
+// infinity meets them one by one, and a part of 0 makes a NaN of it; so an output
+// that is not finite, in a row whose sum of weights is, is found again from all the
+// keys that the row sees.
 
 // 16 bytes of values; returns whether one was replaced.
 template <class C>
@@ -347,6 +348,11 @@ __device__ __forceinline__ bool clear_bad_scale(float* p) {
   const bool bad = !finite(*p);
   if (bad) *p = 0.0f;
   return bad;
+}
+
+// Bits of keys key0 .. key0 + 31 that are below x.
+__device__ __forceinline__ uint32_t below(int x) {
+  return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
 }
 
 // Value d of key j of request b and key head h, if it is not finite, else 0.

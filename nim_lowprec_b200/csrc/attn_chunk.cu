@@ -191,11 +191,6 @@ __device__ __forceinline__ void tie(uint32_t* r, int n) {
   for (int i = 0; i < 32; ++i)
     if (i < n) asm volatile("" : "+r"(r[i]));
 }
-// Bits of keys key0 .. key0 + 31 that are below x.
-__device__ __forceinline__ uint32_t below(int x) {
-  return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u;
-}
-
 // Where a role is in the ring of key and value tiles.
 template <int STAGES>
 struct Ring {
@@ -934,9 +929,19 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
     // longer than the other roles wait.  BY_ROW keeps that form for few tiles.)
     uint32_t up[OB] = {}, down[OB] = {};
     const int nbad = live && warp_ok ? sh.nbad[item % kPlaces] : 0;
+    // All tiles are looked through where too many are noted and, with several parts of
+    // the weights, where an output is not finite though the row's sum is: an infinity
+    // that met the parts one by one is a NaN by now.
+    bool all_tiles = nbad > kBad;
+    if constexpr (F::NP > 1) {
+      float f0 = 0.0f, f1 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < OB * 32; e += 2) f0 = fmaf(o[e], 0.0f, f0), f1 = fmaf(o[e + 1], 0.0f, f1);
+      all_tiles = __any_sync(0xffffffffu, warp_ok && f0 + f1 != 0.0f && finite(l)) || all_tiles;
+    }
 #pragma unroll 1
-    for (int i = 0; i < 4 * (nbad > kBad ? w.n : F::BY_ROW ? 0 : nbad); ++i) {
-      const int key0 = (nbad > kBad ? w.key(i / 4) : sh.badkey[item % kPlaces][i / 4]) + 32 * (i % 4);
+    for (int i = 0; i < 4 * (all_tiles ? w.n : F::BY_ROW ? 0 : nbad); ++i) {
+      const int key0 = (all_tiles ? w.key(i / 4) : sh.badkey[item % kPlaces][i / 4]) + 32 * (i % 4);
       const int j = key0 + (threadIdx.x & 31);
       const int page = j < w.rq.limit ? page_of(a, w.b, j) : -1;
       uint32_t see = __ballot_sync(0xffffffffu, page >= 0) & below(pos + 1 - key0) &
@@ -977,13 +982,13 @@ __device__ __forceinline__ void soft_role(const Args& a, WalkOf<F> w, Shared& sh
       if (up[b] | down[b]) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          if (up[b] >> e & 1u) v[e] += INFINITY;
-          if (down[b] >> e & 1u) v[e] -= INFINITY;
+          const bool u = up[b] >> e & 1u, d = down[b] >> e & 1u;
+          if (u || d) v[e] = u && d ? NAN : u ? INFINITY : -INFINITY;
         }
       }
       if constexpr (F::BY_ROW) {
 #pragma unroll 1
-        for (int i = 0; i < (nbad > kBad ? 0 : nbad); ++i) {
+        for (int i = 0; i < (all_tiles ? 0 : nbad); ++i) {
           const int key0 = sh.badkey[item % kPlaces][i];
 #pragma unroll 1
           for (int j = key0; j < key0 + kKeys; ++j) {

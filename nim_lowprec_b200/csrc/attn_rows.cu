@@ -35,8 +35,8 @@
 // 200 us (5.4 TB/s, 82 % of a copy's rate; what is missing is the spread of the
 // SMs' shares of the bandwidth, 157 us on average); 32 requests under a window
 // of 4000, heads of 64, 55 us (4.2 TB/s; 16 us of start and join); 53 requests of
-// up to 16000 keys over an int8 cache with fp32 queries, 228 us (3.6 TB/s), with
-// bf16 ones 213: latency at two warps per scheduler, each of which issues every
+// up to 16000 keys over an int8 cache with fp32 queries, 233 us (3.5 TB/s), with
+// bf16 ones 217: latency at two warps per scheduler, each of which issues every
 // 4 cycles (49 % of the issue slots, 29 % of the tensor pipe, 57 % of DRAM).
 #include <type_traits>
 
@@ -598,26 +598,54 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_rows(const __grid_constant
       }
     }
 
-    // ---- values that were cleared, for the rows that see them (one that was not
-    // cleared and is added again changes nothing: it is not finite)
-#pragma unroll 1
-    for (int s = 0; s < (nbad <= kBad ? nbad : steps); ++s) {
-      const int u = warp + s / SPU * kWarps;
-      const int key0 = nbad <= kBad ? __shfl_sync(0xffffffffu, badkey, s) : w.key(u) + s % SPU * S::KS;
-#pragma unroll 1
-      for (int j = key0; j < key0 + S::KS; ++j) {
-        const int page = row_ok && sees(a, w.rq, pos, j) ? page_of(a, w.b, j) : -1;
-        if (page < 0) continue;
+    // ---- values that are not finite, for the rows that see them: cleared ones of the
+    // steps noted; and where an output is not finite, all (an infinity that met a
+    // weight's parts one by one is a NaN by now), unless the row's sum is none either.
+    // A lane looks at one key.
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float f0 = 0.0f, f1 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < S::TILES; ++i) {
-          o[i][0] += bad_value<C>(a, w.b, w.head, page, j, value_dim<C, D>(2 * c4, i));
-          o[i][1] += bad_value<C>(a, w.b, w.head, page, j, value_dim<C, D>(2 * c4 + 1, i));
+    for (int i = 0; i < S::TILES; ++i) {
+      f0 = fmaf(o[i][0], 0.0f, f0), f1 = fmaf(o[i][1], 0.0f, f1);
+      f0 = fmaf(o[i][2], 0.0f, f0), f1 = fmaf(o[i][3], 0.0f, f1);
+    }
+    const bool all_steps = __any_sync(0xffffffffu, f0 + f1 != 0.0f && finite(l)) || nbad > kBad;
+    if (all_steps || nbad) {
+#pragma unroll 1
+      for (int b = 0; b < D / 32; ++b) {
+        uint32_t up = 0, down = 0;  // of the block's columns: a +inf or NaN, a -inf or NaN
+#pragma unroll 1
+        for (int s = 0; s < (all_steps ? steps : nbad); ++s) {
+          const int key0 = all_steps ? w.key(warp + s / SPU * kWarps) + s % SPU * S::KS
+                                     : __shfl_sync(0xffffffffu, badkey, s);
+          const int j = key0 + lane;
+          const int page = lane < S::KS && j < w.rq.limit ? page_of(a, w.b, j) : -1;
+          uint32_t see = __ballot_sync(0xffffffffu, page >= 0) & below(pos + 1 - key0) &
+                         (~below(row_lo - key0) | below(a.sinks - key0));
+          if (!row_ok) see = 0;
+          uint32_t x = 0, y = 0;
+          if (page >= 0) bad_columns<C>(a, w.head, page, j, 32 * b, x, y);
+          uint32_t keys = __ballot_sync(0xffffffffu, (x | y) != 0);
+          while (keys) {
+            const int k = __ffs(keys) - 1;
+            keys &= keys - 1;
+            const uint32_t xs = __shfl_sync(0xffffffffu, x, k), ys = __shfl_sync(0xffffffffu, y, k);
+            if (see >> k & 1u) up |= xs, down |= ys;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < S::TILES; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int d = value_dim<C, D>(2 * c4 + y, i) - 32 * b;
+            if (d < 0 || d >= 32 || !((up | down) >> d & 1u)) continue;
+            o[i][y] = !(up >> d & 1u) ? -INFINITY : down >> d & 1u ? NAN : INFINITY;
+            o[i][y + 2] = 0.0f;
+          }
       }
     }
     // ---- join the warps that had steps: a row of the block by one warp
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (warp < w.n && c4 == 0) {
       s_m[warp][g8] = m;
       s_l[warp][g8] = l;

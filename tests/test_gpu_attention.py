@@ -414,3 +414,49 @@ def test_graphs_with_workspaces_of_their_own_run_side_by_side():
         L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], eager)
         torch.cuda.synchronize()
         assert torch.equal(eager, first) and all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("x,cache", PAIRS)
+def test_infinities_that_every_row_sees(x, cache, dim, n):
+    """Values that are not finite in tiles that all rows see whole, at lengths that end with a
+    tile: each column has the sum that the definition gives, an infinity or a NaN."""
+    m = R.make(28, [(128 - n, n), (320 - n, n), (500, n)], 4, 2, dim, 16, x, cache)
+    c = m["cache"]
+    if cache == "int8":  # (fp16 results are not to overflow)
+        c.vScales.clamp_(max=100.0)
+    col = torch.arange(dim, device="cuda") % 8
+    for b, (i, j) in enumerate([(5, 21), (0, 17), (7, 37)]):  # keys that are seen by all rows
+        first, second = ((int(m["table"][b, k // 16]), k % 16) for k in (i, j))
+        if cache == "int8":
+            c.vScales[first] = (math.inf, -math.inf, math.nan)[b]
+            if b == 1:  # codes of one sign against the other's infinity
+                c.vScales[second] = math.inf
+            continue
+        c.v[first][:, col == 0] = math.inf
+        c.v[first][:, col == 1] = -math.inf
+        c.v[first][:, col == 2] = math.inf
+        c.v[second][:, col == 2] = -math.inf
+        c.v[second][:, col == 3] = math.nan
+        c.v[second][:, col == 4] = math.inf
+    R.check(m)
+
+
+def test_rows_of_nan_beside_infinities():
+    """A NaN in a query makes its row NaN and leaves the others what they are."""
+    for n in (1, 90):
+        for x, cache in (("fp32", "fp16"), ("fp32", "int8"), ("bf16", "bf16")):
+            m = R.make(29, [(128 - n, n), (320 - n, n)], 4, 2, 64, 16, x, cache)
+            if cache == "int8":
+                m["cache"].vScales[int(m["table"][1, 0]), 3] = math.inf
+            else:
+                m["cache"].v[int(m["table"][1, 0]), 3] = math.inf
+            out = torch.empty_like(m["q"])
+            L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], out)
+            m["q"][n, 1, 7] = math.nan
+            got = R.torch.empty_like(out)
+            L.pagedAttention(m["cache"], m["table"], m["qstart"], m["seq"], m["q"], got)
+            assert bool(torch.isnan(got[n, 1]).all())
+            got[n, 1] = out[n, 1]
+            assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(out, nan=7.0))
