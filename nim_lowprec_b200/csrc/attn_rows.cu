@@ -35,7 +35,7 @@
 // 200 us (5.4 TB/s, 82 % of a copy's rate; what is missing is the spread of the
 // SMs' shares of the bandwidth, 157 us on average); 32 requests under a window
 // of 4000, heads of 64, 55 us (4.2 TB/s; 16 us of start and join); 53 requests of
-// up to 16000 keys over an int8 cache with fp32 queries, 233 us (3.5 TB/s), with
+// up to 16000 keys over an int8 cache with fp32 queries, 232 us (3.5 TB/s), with
 // bf16 ones 217: latency at two warps per scheduler, each of which issues every
 // 4 cycles (49 % of the issue slots, 29 % of the tensor pipe, 57 % of DRAM).
 #include <type_traits>
