@@ -367,7 +367,10 @@ int lp_dequantize_nvfp4(const uint8_t *codes, int64_t codes_len, const uint8_t *
 #define LP_F32 0
 #define LP_F16 1
 #define LP_BF16 2
-#define LP_I8 3 /* cache only: int8 codes, one fp32 scale per (token, head) */
+#define LP_I8 3 /* int8 codes: the cache's (one fp32 scale per token and head), 8-bit rows */
+#define LP_E4M3 4 /* 8-bit rows and experts' weights: MXFP8 codes */
+#define LP_E2M1 5 /* experts' weights: MXFP4 codes */
+#define LP_E8M0 6 /* scales 2^(code - 127) in a byte */
 
 /* The cache: element (page, token, head, i) of k is at
  * k[page*k_strides[0] + token*k_strides[1] + head*k_strides[2] + i], strides
@@ -466,6 +469,115 @@ int lp_paged_attention(const lp_kv_cache *cache, const int32_t *block_tables, in
                        const lp_rows *out, float scale, int64_t window, int64_t sinks, float *lse,
                        int64_t lse_len, void *workspace, int64_t workspace_len,
                        lp_stream_t stream);
+
+/* ======================= 8-bit rows, router and experts ================ */
+/* The sparse feed-forward layer between two attentions (no counterpart in the
+ * reference): the norm that turns the residual stream into 8-bit rows, the router,
+ * products with the experts' weights, and the sum of a token's experts.  Device
+ * pointers, stream-ordered, nothing allocated.  Outputs must not overlap inputs
+ * or each other, except where it says so. */
+
+/* Rows of a matrix: element (r, c) at data[r*stride + c]; any alignment, strides in
+ * elements from 0 to 2^31 - 1. */
+typedef struct lp_matrix {
+  void *data;
+  int64_t rows, cols, stride;
+  int32_t dtype; /* LP_F32, LP_F16, LP_BF16 */
+  int32_t reserved;
+} lp_matrix;
+
+/* 8-bit rows: value (r, c) = codes[r*code_stride + c] * scale(r, c div group), the
+ * scale at scales[r*scale_stride + c div group].
+ *   LP_E4M3  MXFP8: group 32, scales E8M0 bytes, 2^(floor(log2 absmax) - 8) (the
+ *            scale of lp_calibrate_mx with elem_emax 8; 1 for a block of zeros), codes
+ *            e4m3, rounded to nearest even, magnitudes over 448 to 448; a block with an
+ *            infinity keeps it, a NaN stays one and does not count for the scale
+ *   LP_I8    groups of 32, 64, 128 or 256, scales fp32, the bytes that
+ *            lp_calibrate_symmetric (qmax 127) and lp_quantize_batch give: xq and
+ *            x_scales of lp_dequant_gemm_q8 / _i4q8 and their GEMVs
+ * cols is a multiple of the group. */
+typedef struct lp_rows8 {
+  void *codes, *scales;
+  int64_t rows, cols, code_stride, scale_stride;
+  int32_t dtype, group;
+} lp_rows8;
+
+/* x as 8-bit rows, and the values of 8-bit rows (rounded once to dst's type). */
+int lp_quantize_rows(const lp_matrix *x, const lp_rows8 *out, lp_stream_t stream);
+int lp_dequantize_rows(const lp_rows8 *rows, const lp_matrix *dst, lp_stream_t stream);
+
+/* r = x + residual, rounded to the residual's type; n = r / sqrt(mean(r^2) + eps) * weight
+ * over each row, in fp32.  Out, each may be null: total = r, y = n (any type), q = n as
+ * 8-bit rows.  residual may be null (r = x); total has the residual's type (x's without
+ * one), which is x's or LP_F32.  total may be x or the residual itself, y may be x.
+ * At most 32768 columns. */
+int lp_add_rms_norm(const lp_matrix *x, const lp_matrix *residual, const void *weight,
+                    int64_t weight_len, int32_t weight_type, float eps, const lp_matrix *total,
+                    const lp_matrix *y, const lp_rows8 *q, lp_stream_t stream);
+
+/* Bytes of workspace that lp_route_experts and lp_expert_gemm take on the current device.
+ * It is zeroed once, when it is allocated; every call leaves it ready for the next one on
+ * the same stream.  Calls that may run at the same time need one each. */
+int lp_experts_workspace(int64_t *bytes);
+
+/* Each token's k experts (k at most 32, experts at most 1024) and the order of their rows.
+ * logits: tokens x experts.  Out, tokens x k: experts (the k largest logits, largest
+ * first, of equal ones the lower expert), weights exp(l_j - l_max) / s with s the sum
+ * over the chosen (renormalize) or over all experts, and places, each pair's row: rows
+ * are sorted by expert, then by token.  offsets (experts + 1): expert e has rows
+ * offsets[e] .. offsets[e+1].  row_token (tokens x k): each row's token; rows from
+ * offsets[experts] on are left alone.  A logit of -inf or NaN is never chosen: a token
+ * with fewer than k others gets expert -1, place -1 and weight 0 in the rest. */
+int lp_route_experts(const lp_matrix *logits, float *weights, int64_t weights_len,
+                     int32_t *experts, int64_t experts_len, int32_t *offsets, int64_t offsets_len,
+                     int32_t *row_token, int64_t row_token_len, int32_t *places,
+                     int64_t places_len, int64_t k, int32_t renormalize, void *workspace,
+                     int64_t workspace_len, lp_stream_t stream);
+
+/* Experts' weights as the products read them (their layout is this library's own).
+ * rows x cols of each expert; gated: the first half of the rows are the gate's, the
+ * second the up projection's.  cols a multiple of 32, gated rows of 64. */
+typedef struct lp_expert_weights {
+  void *tiles, *scales;
+  int64_t experts, rows, cols;
+  int32_t dtype; /* LP_E2M1 (MXFP4), LP_E4M3 (MXFP8) */
+  int32_t gated;
+} lp_expert_weights;
+
+/* Bytes of tiles and scales of such weights (pointers are not looked at), and the laying
+ * out: codes experts x rows x cols (LP_E2M1: packed as lp_quantize_f4_packed packs them,
+ * two to a byte; codes_len counts bytes), scales experts x rows x cols / 32 (LP_F32:
+ * powers of two, as lp_calibrate_mx writes them; or LP_E8M0). */
+int lp_expert_weights_bytes(const lp_expert_weights *w, int64_t *tile_bytes, int64_t *scale_bytes);
+int lp_expert_weights_pack(const void *codes, int64_t codes_len, const void *scales,
+                           int64_t scales_len, int32_t scale_type, const lp_expert_weights *out,
+                           lp_stream_t stream);
+
+/* y[r, m] = sum_c W[e][m, c] x[t, c] for the rows r of every expert e (offsets as
+ * lp_route_experts writes them; values outside the rows are clamped), t = row_token[r], or
+ * r where row_token is null.  x: LP_E4M3 rows, codes 16-byte aligned with strides that
+ * are multiples of 16.  out has row_token_len rows (x's without row_token); rows of no
+ * expert are left alone.  A row_token outside x counts as a row of zeros.
+ * Products are exact, sums fp32, results rounded once. */
+int lp_expert_gemm(const lp_expert_weights *w, const lp_rows8 *x, const int32_t *offsets,
+                   int64_t offsets_len, const int32_t *row_token, int64_t row_token_len,
+                   const lp_matrix *out, void *workspace, int64_t workspace_len,
+                   lp_stream_t stream);
+
+/* The same with gated weights, g = y[r, f] and u = y[r, rows / 2 + f]:
+ * out = g / (1 + exp(-g)) * u, rounded from fp32 to LP_E4M3 rows of rows / 2 columns
+ * (codes 16-byte aligned, strides multiples of 16). */
+int lp_expert_gemm_gated(const lp_expert_weights *w, const lp_rows8 *x, const int32_t *offsets,
+                         int64_t offsets_len, const int32_t *row_token, int64_t row_token_len,
+                         const lp_rows8 *out, void *workspace, int64_t workspace_len,
+                         lp_stream_t stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] * rows[places[t, j]], summed in fp32 in the
+ * order of j; places outside rows add nothing; residual may be null, or out itself, and
+ * has out's type. */
+int lp_combine_experts(const lp_matrix *rows, const float *weights, int64_t weights_len,
+                       const int32_t *places, int64_t places_len, const lp_matrix *residual,
+                       const lp_matrix *out, lp_stream_t stream);
 
 /* ======================= host-pointer drop-in forms ==================== */
 /* Same arguments and meaning as the lp_* forms above, HOST pointers, no

@@ -19,6 +19,9 @@ from .dequant import (  # noqa: F401
     fp32Mode, gemmNVFP4, setFp32Mode)
 from .attention import (  # noqa: F401
     KVCache, assignPages, attentionWorkspace, loadKV, pagedAttention, storeKV)
+from .experts import (  # noqa: F401
+    ExpertWeights, addRmsNorm, combineExperts, dequantizeRows, expertGemm, expertGemmGated,
+    expertsWorkspace, quantizeRows, routeExperts)
 from .ggml import QK, QK_K, BlockQ4_0, BlockQ4_K, BlockQ6_K, BlockQ8_0  # noqa: F401
 from . import parallel  # noqa: F401  (LpPool's row-sharded forms)
 

@@ -25,6 +25,9 @@ LP_F32 = 0  # element types of the paged cache and its rows
 LP_F16 = 1
 LP_BF16 = 2
 LP_I8 = 3
+LP_E4M3 = 4  # 8-bit rows and experts' weights
+LP_E2M1 = 5
+LP_E8M0 = 6
 
 LP_FP32_FAST = 0
 LP_FP32_EXACT = 1
@@ -119,6 +122,16 @@ SIGNATURES = {
     "lp_load_kv": "ppnppp",
     "lp_paged_attention_workspace": "p",
     "lp_paged_attention": "ppnnpnpnppfnnpnpnp",
+    "lp_quantize_rows": "ppp",
+    "lp_dequantize_rows": "ppp",
+    "lp_add_rms_norm": "pppnifpppp",
+    "lp_experts_workspace": "p",
+    "lp_route_experts": "ppnpnpnpnpnnipnp",
+    "lp_expert_weights_bytes": "ppp",
+    "lp_expert_weights_pack": "pnpnipp",
+    "lp_expert_gemm": "pppnpnppnp",
+    "lp_expert_gemm_gated": "pppnpnppnp",
+    "lp_combine_experts": "ppnpnppp",
     "lph_pool_init": "pi",
     "lph_pool_shutdown": "p",
     "lph_pool_thread_count": "p",

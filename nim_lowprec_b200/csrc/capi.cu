@@ -157,6 +157,8 @@ int lp_device_error(void) {
   if (!e) e = e4;
   const unsigned int e5 = lp::take_error_attn_chunk();
   if (!e) e = e5;
+  const unsigned int e6 = lp::take_error_experts();
+  if (!e) e = e6;
   return static_cast<int>(e);
 }
 

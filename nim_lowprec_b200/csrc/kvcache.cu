@@ -1,12 +1,11 @@
 // kvcache.cu -- the paged key/value cache: page tables and slot maps from
 // request lengths (assignPages), rows written to slots (storeKV) and read
 // back (loadKV).
-#include <cuda_bf16.h>
-
 #include <algorithm>
 
 #include "lp_device.cuh"
 #include "lp_internal.h"
+#include "rows.cuh"
 
 namespace lp {
 namespace {
@@ -207,53 +206,6 @@ struct RowsArgs {
   int64_t slots_end;  // pages * page_size
 };
 
-__device__ __forceinline__ uint32_t pack_h(float a, float b) {
-  return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(a))) |
-         static_cast<uint32_t>(__half_as_ushort(__float2half_rn(b))) << 16;
-}
-__device__ __forceinline__ uint32_t pack_b(float a, float b) {
-  return static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(a))) |
-         static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(b))) << 16;
-}
-
-// Eight elements of type T at p.  VEC: p is on a boundary of its 16-byte (or,
-// int8, 8-byte) pieces; else element by element.
-template <int T, bool VEC>
-__device__ __forceinline__ void load8(float* x, const uint8_t* p) {
-  if constexpr (T == LP_F32) {
-    if constexpr (VEC) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(p));
-      const float4 w = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-      x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __ldg(reinterpret_cast<const float*>(p) + i);
-    }
-  } else {
-    uint32_t w[4];
-    if constexpr (VEC) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-    } else {
-      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = __ldg(h + 2 * i) | static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (T == LP_F16) {
-        x[2 * i] = h2f(w[i] & 0xffffu);
-        x[2 * i + 1] = h2f(w[i] >> 16);
-      } else {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ void load16_i8(float* x, const uint8_t* p) {
   const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -289,62 +241,6 @@ __device__ __forceinline__ void load_cache(float* x, const uint8_t* p) {
         x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
     }
   }
-}
-
-template <int T, bool VEC>
-__device__ __forceinline__ void store8(uint8_t* p, const float* x) {
-  if constexpr (T == LP_F32) {
-    if constexpr (VEC) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) reinterpret_cast<float*>(p)[i] = x[i];
-    }
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = T == LP_F16 ? pack_h(x[2 * i], x[2 * i + 1]) : pack_b(x[2 * i], x[2 * i + 1]);
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        reinterpret_cast<unsigned short*>(p)[i] =
-            static_cast<unsigned short>(w[i >> 1] >> (16 * (i & 1)));
-    }
-  }
-}
-
-constexpr int size_of(int t) { return t == LP_F32 ? 4 : t == LP_I8 ? 1 : 2; }
-
-// Codes of x / s, rounded half away from zero, four to a word.  The quotient is exact where it decides something.  x * (1 / s) is off by at most
-// 2^-22 of 127, so a result further than 2^-14 from the middle between two
-// whole numbers rounds as the quotient does; others (and what is not finite)
-// are divided.  (Sixteen divisions a thread took three times the bytes' time.)
-template <int N>
-__device__ __forceinline__ void codes(uint32_t* w, const float* x, float s) {
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the whole number
-  const float inv = __fdiv_rn(1.0f, s);
-  bool sure = true;
-  uint32_t q[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = fmul(x[i], inv);
-    const float z = fadd(y, kMagic);
-    q[i] = __float_as_uint(z);
-    sure = sure && fabsf(fadd(y, -fadd(z, -kMagic))) < 0.5f - 6.1e-5f;  // (not for a NaN)
-  }
-  if (!sure) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      q[i] = static_cast<uint32_t>(
-          static_cast<int>(fminf(fmaxf(roundf(__fdiv_rn(x[i], s)), -128.0f), 127.0f)));
-  }
-#pragma unroll
-  for (int i = 0; i < N / 4; ++i)
-    w[i] = prmt(prmt(q[4 * i], q[4 * i + 1], 0x0040u), prmt(q[4 * i + 2], q[4 * i + 3], 0x0040u), 0x5410u);
 }
 
 // A lane's N elements of a row, of which L lanes hold one.

@@ -149,12 +149,29 @@ struct Args;
 int launch_attn_rows(const attn::Args& a, int cache_type, int dim, cudaStream_t st);
 int launch_attn_chunk(const attn::Args& a, int cache_type, int dim, cudaStream_t st);
 
+// 8-bit rows (rows8.cu), the router (route.cu) and the experts' products (experts.cu)
+constexpr int kRouteExperts = 1024;  // most experts
+constexpr int kRouteCtas = 128;      // most CTAs that count
+int launch_norm(const lp_matrix& x, const lp_matrix* residual, const void* weight, int weight_type, float eps,
+                const lp_matrix* total, const lp_matrix* y, const lp_rows8* q, bool vec, cudaStream_t st);
+int launch_quantize_rows(const lp_matrix& x, const lp_rows8& q, bool vec, cudaStream_t st);
+int launch_dequantize_rows(const lp_rows8& q, const lp_matrix& x, bool vec, cudaStream_t st);
+int launch_combine(const lp_matrix& rows, const float* weights, const int32_t* places, int64_t k,
+                   const lp_matrix* residual, const lp_matrix& out, bool vec, cudaStream_t st);
+int launch_route(const lp_matrix& logits, float* weights, int32_t* experts, int32_t* offsets, int32_t* row_token,
+                 int32_t* places, int64_t k, int renorm, int32_t* counts, cudaStream_t st);
+int launch_pack_experts(const void* codes, const void* scales, int scale_type, const lp_expert_weights& w,
+                        cudaStream_t st);
+int launch_experts(const lp_expert_weights& w, const lp_rows8& x, const int32_t* offsets, const int32_t* row_token,
+                   int64_t rows, const lp_matrix* out, const lp_rows8* out8, void* workspace, cudaStream_t st);
+
 // error words of the translation units whose kernels wait (read + clear)
 unsigned int take_error_gemv();
 unsigned int take_error_gemm_tc();
 unsigned int take_error_pool();
 unsigned int take_error_gemm_fp4();
 unsigned int take_error_attn_chunk();
+unsigned int take_error_experts();
 
 // While on (this thread only), the lp_* entry points run their shape and
 // argument checks and return without launching anything (capi.cu).

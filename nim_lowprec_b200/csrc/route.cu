@@ -1,0 +1,251 @@
+// route.cu -- routeExperts: each token's k experts, their weights, and the rows
+// (one per token and choice) sorted by expert.
+//
+//   chosen = the k largest logits (ties: the lower expert), w_j = exp(l_j - l_max) / s,
+//   s = the sum over the chosen, or over all experts;
+//   row order: by expert, then by token;  offsets[e] = rows of experts before e
+//
+// Latency bounds it.  A warp holds a token's logits and takes the largest k times
+// (two reductions a time).  Few tokens: one CTA does all.  More: one launch
+// chooses and counts per CTA and expert, one turns the counts of all CTAs into
+// offsets (each CTA for itself) and places its rows in order, so that no atomics
+// decide an order.
+#include <algorithm>
+
+#include "lp_device.cuh"
+#include "lp_internal.h"
+#include "rows.cuh"
+
+namespace lp {
+namespace {
+
+constexpr int kMaxPer = kRouteExperts / 32;  // logits a lane holds
+constexpr int kPairs = 2048;                 // (token, choice) pairs placed at a time
+constexpr int kThreads = 512;
+constexpr int kOneCta = 64;                  // tokens that one CTA takes
+
+struct RouteArgs {
+  const uint8_t* logits;
+  int64_t stride;  // bytes
+  int type;
+  float* weights;
+  int32_t *experts, *offsets, *row_token, *places;
+  int32_t* counts;  // [CTAs][experts]
+  int64_t tokens, per;  // of a CTA
+  int n, k, renorm;
+};
+
+// A key that orders as the logits do; 0 for -inf and NaN, which are never chosen.
+__device__ __forceinline__ uint32_t key_of(float l) {
+  if (!(l > -__int_as_float(0x7f800000))) return 0u;
+  const uint32_t u = __float_as_uint(l + 0.0f);  // (-0 orders as 0)
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ float logit(const RouteArgs& a, int64_t t, int e) {
+  const uint8_t* p = a.logits + t * a.stride + int64_t{e} * size_of(a.type);
+  if (a.type == LP_F32) return *reinterpret_cast<const float*>(p);
+  const uint32_t h = *reinterpret_cast<const unsigned short*>(p);
+  return a.type == LP_F16 ? h2f(h) : __uint_as_float(h << 16);
+}
+
+// One warp: the choices of token t; lane j holds the j-th expert (-1: none).
+template <int PER>
+__device__ __forceinline__ int choose(const RouteArgs& a, int64_t t, int lane) {
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = 32 * i + lane < a.n ? key_of(logit(a, t, 32 * i + lane)) : 0u;
+  uint32_t mine = 0, top = 0;
+  int id = -1;
+  float all = 0.0f;
+  for (int j = 0; j < a.k; ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (j == 0) {
+      top = best;
+      if (!a.renorm && best) {
+        const float m = value_of(best);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (key[i]) all = fadd(all, key[i] == best ? 1.0f : expf(fadd(value_of(key[i]), -m)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all = fadd(all, __shfl_xor_sync(0xffffffffu, all, o));
+      }
+    }
+    if (best == 0u) break;
+    uint32_t at = 0xffffffffu;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i)
+      if (key[i] == best) at = 32 * i + lane;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (at == 32u * i + lane) key[i] = 0u;
+    if (lane == j) mine = best, id = static_cast<int>(at);
+  }
+  float p = 0.0f;
+  if (id >= 0) p = mine == top ? 1.0f : expf(fadd(value_of(mine), -value_of(top)));
+  if (a.renorm) {
+    all = p;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all = fadd(all, __shfl_xor_sync(0xffffffffu, all, o));
+  }
+  if (lane < a.k) {
+    a.weights[t * a.k + lane] = id >= 0 ? __fdiv_rn(p, all) : 0.0f;
+    a.experts[t * a.k + lane] = id;
+  }
+  return id;
+}
+
+// Rows of each expert before this CTA's (base) and the offsets, from the counts.
+// An inclusive scan over the experts by all threads; n <= 2 * kThreads.
+__device__ __forceinline__ void scan_counts(const RouteArgs& a, int ctas, int32_t* base, int32_t* sums) {
+  __shared__ int32_t wsum[kThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int carry = 0;
+  for (int e0 = 0; e0 < a.n; e0 += kThreads) {
+    const int e = e0 + threadIdx.x;
+    int before = 0, total = 0;
+    if (e < a.n) {
+      for (int c0 = 0; c0 < ctas; c0 += 8) {
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < ctas ? __ldcg(a.counts + int64_t{c0 + i} * a.n + e) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (c0 + i < static_cast<int>(blockIdx.x)) before += v[i];
+          total += v[i];
+        }
+      }
+    }
+    int inc = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int ahead = carry;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) ahead += wsum[w];
+      carry += wsum[w];
+    }
+    inc += ahead;
+    if (e < a.n) {
+      base[e] = inc - total + before;
+      sums[e] = inc;
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) a.offsets[0] = 0;
+    for (int e = threadIdx.x; e < a.n; e += kThreads) a.offsets[e + 1] = sums[e];
+  }
+}
+
+// The rows of tokens [t0, t1) in order: a thread per expert walks the pairs.
+__device__ __forceinline__ void place(const RouteArgs& a, int64_t t0, int64_t t1, int32_t* base, int16_t* ids,
+                                      int32_t* at) {
+  const int step = kPairs / a.k;  // tokens at a time
+  for (int64_t s = t0; s < t1; s += step) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(step), t1 - s)) * a.k;
+    __syncthreads();
+    for (int i = threadIdx.x; i < (n + 7) / 8 * 8; i += kThreads) {
+      const int id = i < n ? a.experts[s * a.k + i] : -1;
+      ids[i] = static_cast<int16_t>(id);
+      if (i < n && id < 0) at[i] = -1;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.n; e += kThreads) {
+      int next = base[e];
+      for (int i = 0; i < n; i += 8) {  // eight pairs a read
+        const uint4 q = *reinterpret_cast<const uint4*>(ids + i);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (static_cast<int>(w[j >> 1] >> (16 * (j & 1)) & 0xffffu) == e) at[i + j] = next++;
+      }
+      base[e] = next;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int p = at[i];
+      a.places[s * a.k + i] = p;
+      if (p >= 0) a.row_token[p] = static_cast<int32_t>(s + i / a.k);
+    }
+  }
+}
+
+template <int PER, bool ONE>
+__global__ void __launch_bounds__(kThreads) k_route_choose(const RouteArgs a) {
+  __shared__ int32_t hist[kRouteExperts];
+  __shared__ int32_t sums[ONE ? kRouteExperts : 1];
+  __shared__ __align__(16) int16_t ids[ONE ? kPairs : 8];
+  __shared__ int32_t at[ONE ? kPairs : 1];
+  for (int e = threadIdx.x; e < a.n; e += kThreads) hist[e] = 0;
+  __syncthreads();
+  const int64_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tokens);
+  const int lane = threadIdx.x & 31;
+  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += kThreads / 32) {
+    const int id = choose<PER>(a, t, lane);
+    if (id >= 0) atomicAdd(&hist[id], 1);  // (a count: its order does not matter)
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.n; e += kThreads) a.counts[int64_t{blockIdx.x} * a.n + e] = hist[e];
+  if constexpr (ONE) {
+    __syncthreads();
+    scan_counts(a, 1, hist, sums);
+    place(a, t0, t1, hist, ids, at);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) k_route_place(const RouteArgs a) {
+  __shared__ int32_t base[kRouteExperts], sums[kRouteExperts];
+  __shared__ __align__(16) int16_t ids[kPairs];
+  __shared__ int32_t at[kPairs];
+  scan_counts(a, gridDim.x, base, sums);
+  const int64_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tokens);
+  place(a, t0, t1, base, ids, at);
+}
+
+template <int PER>
+int launch_route_per(const RouteArgs& a, int ctas, cudaStream_t st) {
+  if (ctas <= 1) {
+    k_route_choose<PER, true><<<1, kThreads, 0, st>>>(a);
+  } else {
+    k_route_choose<PER, false><<<ctas, kThreads, 0, st>>>(a);
+    k_route_place<<<ctas, kThreads, 0, st>>>(a);
+  }
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+int launch_route(const lp_matrix& logits, float* weights, int32_t* experts, int32_t* offsets, int32_t* row_token,
+                 int32_t* places, int64_t k, int renorm, int32_t* counts, cudaStream_t st) {
+  RouteArgs a{static_cast<const uint8_t*>(logits.data), logits.stride * size_of(logits.dtype), logits.dtype,
+              weights, experts, offsets, row_token, places, counts, logits.rows, 0,
+              static_cast<int>(logits.cols), static_cast<int>(k), renorm};
+  int ctas = 1;
+  if (a.tokens > kOneCta) {
+    // a multiple of the CTA's 16 warps each, on as many CTAs as the counts have room for
+    a.per = (a.tokens + kRouteCtas - 1) / kRouteCtas;
+    a.per = (a.per + 15) / 16 * 16;
+    ctas = static_cast<int>((a.tokens + a.per - 1) / a.per);
+  } else {
+    a.per = a.tokens;
+  }
+  if (a.n <= 32) return launch_route_per<1>(a, ctas, st);
+  if (a.n <= 64) return launch_route_per<2>(a, ctas, st);
+  if (a.n <= 128) return launch_route_per<4>(a, ctas, st);
+  if (a.n <= 256) return launch_route_per<8>(a, ctas, st);
+  return launch_route_per<kMaxPer>(a, ctas, st);
+}
+
+}  // namespace lp

@@ -1,0 +1,316 @@
+// rows8.cu -- 8-bit rows: their codec (quantizeRows, dequantizeRows), the
+// root-mean-square norm that makes them from a residual stream (addRmsNorm), and
+// the sum of a token's experts' rows (combineExperts).
+//
+// Rows are MXFP8 (e4m3 codes, one E8M0 byte per 32 elements) or int8 (one fp32
+// scale per group).  All four stream: bytes bound them for many rows and the
+// launch with its chain of loads for few.
+#include <algorithm>
+
+#include "lp_device.cuh"
+#include "lp_internal.h"
+#include "rows.cuh"
+
+namespace lp {
+namespace {
+
+struct Mat {  // rows of a matrix; p may be null
+  uint8_t* p;
+  int64_t stride;  // bytes
+  int type;
+};
+struct Rows8 {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t code_stride, scale_stride;  // bytes
+  int int8;                           // else MXFP8
+  int lanes;                          // of 8 elements, in a group
+  int group_shift;                    // log2 of the group
+};
+
+// A lane's 8 elements of a row as codes, its group's scale by the group's first
+// lane.  The `lanes` lanes of a group are in one warp; `on`: store.
+template <bool VEC>
+__device__ __forceinline__ void put_rows8(const Rows8& q, int64_t row, int unit, const float* x, bool on) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+  for (int o = 1; o < q.lanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  uint32_t w[2];
+  uint8_t* sp = q.scales + row * q.scale_stride;
+  const bool first = on && (unit & (q.lanes - 1)) == 0;
+  if (q.int8) {
+    const float s = m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+    codes<8>(w, x, s);
+    if (first) reinterpret_cast<float*>(sp)[(unit * 8) >> q.group_shift] = s;
+  } else {
+    const uint32_t c = mx8_scale(m);
+    const float inv = mx8_inverse(c);
+    w[0] = e4m3x4(x, inv);
+    w[1] = e4m3x4(x + 4, inv);
+    if (first) sp[unit >> 2] = static_cast<uint8_t>(c);
+  }
+  if (!on) return;
+  uint8_t* p = q.codes + row * q.code_stride + unit * 8;
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// ---------------------------------------------------------- addRmsNorm
+//
+//   r = x + residual, n = r / sqrt(mean r^2 + eps) * weight;  total = r, y = n,
+//   codes = n in 8 bits
+//
+// One pass: a row's elements stay in its CTA's registers (C pieces of 8 a thread)
+// between the sum of squares and the scaling.  r is rounded to the stream's type
+// before it is squared, so that the norm is that of what the stream carries on.
+struct NormArgs {
+  Mat x, res, total, y;
+  const uint8_t* weight;
+  Rows8 q;
+  int64_t rows;
+  int cols, wtype;
+  float eps;
+};
+
+template <bool VEC, int C>
+__global__ void __launch_bounds__(1024) k_norm(const NormArgs a) {
+  __shared__ float part[2][32];
+  const int units = (a.cols + 7) / 8, warps = blockDim.x >> 5;
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+    float v[C][8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int u = c * blockDim.x + threadIdx.x, n = a.cols - 8 * u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] = 0.0f;
+      if (u >= units) continue;
+      load8_of<VEC>(v[c], a.x.p + row * a.x.stride + int64_t{8} * u * size_of(a.x.type), a.x.type, n);
+      if (a.res.p) {
+        float r[8];
+        load8_of<VEC>(r, a.res.p + row * a.res.stride + int64_t{8} * u * size_of(a.res.type), a.res.type, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = rounded(fadd(v[c][i], r[i]), a.res.type);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = __fmaf_rn(v[c][i], v[c][i], sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum = fadd(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+    if ((threadIdx.x & 31) == 0) part[flip][threadIdx.x >> 5] = sum;
+    __syncthreads();  // (two sets of parts: the next row's writes meet no reads)
+    float t = (threadIdx.x & 31) < warps ? part[flip][threadIdx.x & 31] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = fadd(t, __shfl_xor_sync(0xffffffffu, t, o));
+    const float rs = __fdiv_rn(1.0f, __fsqrt_rn(fadd(__fdiv_rn(t, static_cast<float>(a.cols)), a.eps)));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int u = c * blockDim.x + threadIdx.x, n = a.cols - 8 * u;
+      const bool on = u < units;
+      float w[8] = {}, z[8];
+      if (on) {
+        if (a.total.p)
+          store8_of<VEC>(a.total.p + row * a.total.stride + int64_t{8} * u * size_of(a.total.type), v[c],
+                         a.total.type, n);
+        load8_of<VEC>(w, a.weight + int64_t{8} * u * size_of(a.wtype), a.wtype, n);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = fmul(fmul(v[c][i], rs), w[i]);
+      if (on && a.y.p)
+        store8_of<VEC>(a.y.p + row * a.y.stride + int64_t{8} * u * size_of(a.y.type), z, a.y.type, n);
+      if (a.q.codes) put_rows8<VEC>(a.q, row, u, z, on);
+    }
+  }
+}
+
+// -------------------------------------------- quantizeRows, dequantizeRows
+struct CodecArgs {
+  Mat x;
+  Rows8 q;
+  int64_t rows;
+  int cols;
+};
+constexpr int kCodecThreads = 256;
+
+template <bool VEC>
+__global__ void __launch_bounds__(kCodecThreads) k_quantize_rows(const CodecArgs a) {
+  const int per = a.cols / 8;
+  const int64_t n = a.rows * per, step = static_cast<int64_t>(gridDim.x) * kCodecThreads;
+  // whole warps run the same number of rounds: a group's maximum meets by shuffles
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * kCodecThreads + (threadIdx.x & ~31u); i0 < n; i0 += step) {
+    const int64_t i = i0 + (threadIdx.x & 31);
+    const bool on = i < n;
+    const int64_t row = on ? (n >> 32 ? i / per : static_cast<uint32_t>(i) / static_cast<uint32_t>(per)) : 0;
+    const int u = on ? static_cast<int>(i - row * per) : 0;
+    float x[8] = {};
+    if (on) load8_of<VEC>(x, a.x.p + row * a.x.stride + int64_t{8} * u * size_of(a.x.type), a.x.type, 8);
+    put_rows8<VEC>(a.q, row, u, x, on);
+  }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kCodecThreads) k_dequantize_rows(const CodecArgs a) {
+  const int per = a.cols / 8;
+  const int64_t n = a.rows * per, step = static_cast<int64_t>(gridDim.x) * kCodecThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCodecThreads + threadIdx.x; i < n; i += step) {
+    const int64_t row = n >> 32 ? i / per : static_cast<uint32_t>(i) / static_cast<uint32_t>(per);
+    const int u = static_cast<int>(i - row * per);
+    const uint8_t* p = a.q.codes + row * a.q.code_stride + int64_t{8} * u;
+    const uint8_t* sp = a.q.scales + row * a.q.scale_stride;
+    uint32_t w[2] = {0, 0};
+    if constexpr (VEC) {
+      const uint2 t = *reinterpret_cast<const uint2*>(p);
+      w[0] = t.x, w[1] = t.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j >> 2] |= static_cast<uint32_t>(p[j]) << (8 * (j & 3));
+    }
+    float x[8];
+    if (a.q.int8) {
+      const float s = reinterpret_cast<const float*>(sp)[(u * 8) >> a.q.group_shift];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[j] = fmul(static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3)))), s);
+    } else {
+      const float s = e8m0_value(sp[u >> 2]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = e4m3x2_values(w[j >> 1] >> (16 * (j & 1)) & 0xffffu);
+        x[2 * j] = fmul(v.x, s);
+        x[2 * j + 1] = fmul(v.y, s);
+      }
+    }
+    store8_of<VEC>(a.x.p + row * a.x.stride + int64_t{8} * u * size_of(a.x.type), x, a.x.type, 8);
+  }
+}
+
+// ------------------------------------------------------- combineExperts
+//
+//   out[t] = residual[t] + sum_j weights[t, j] * rows[places[t, j]]
+//
+// in the order of j, in fp32.  A thread holds 8 elements of a token and reads
+// four of its experts' rows at a time.
+struct CombineArgs {
+  Mat rows, res, out;
+  const float* weights;
+  const int32_t* places;
+  int64_t tokens, nrows;
+  int k, cols;
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(kCodecThreads) k_combine(const CombineArgs a) {
+  const int per = (a.cols + 7) / 8;
+  const int64_t n = a.tokens * per, step = static_cast<int64_t>(gridDim.x) * kCodecThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCodecThreads + threadIdx.x; i < n; i += step) {
+    const int64_t t = n >> 32 ? i / per : static_cast<uint32_t>(i) / static_cast<uint32_t>(per);
+    const int u = static_cast<int>(i - t * per), left = a.cols - 8 * u;
+    const uint8_t* col = a.rows.p + int64_t{8} * u * size_of(a.rows.type);
+    float sum[8] = {};
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+      float w[4], x[4][8];
+      int64_t place[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = j0 + j < a.k;
+        place[j] = in ? a.places[t * a.k + j0 + j] : -1;
+        w[j] = in ? a.weights[t * a.k + j0 + j] : 0.0f;
+        if (place[j] >= a.nrows) place[j] = -1;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (place[j] >= 0) load8_of<VEC>(x[j], col + place[j] * a.rows.stride, a.rows.type, left);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (place[j] < 0) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = __fmaf_rn(w[j], x[j][e], sum[e]);
+      }
+    }
+    if (a.res.p) {
+      float r[8];
+      load8_of<VEC>(r, a.res.p + t * a.res.stride + int64_t{8} * u * size_of(a.res.type), a.res.type, left);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = fadd(r[e], sum[e]);
+    }
+    store8_of<VEC>(a.out.p + t * a.out.stride + int64_t{8} * u * size_of(a.out.type), sum, a.out.type, left);
+  }
+}
+
+Mat mat(const lp_matrix* m) {
+  if (!m) return {nullptr, 0, LP_F32};
+  return {static_cast<uint8_t*>(m->data), m->stride * size_of(m->dtype), m->dtype};
+}
+Rows8 rows8(const lp_rows8* r) {
+  if (!r) return {};
+  const int shift = 31 - __builtin_clz(static_cast<unsigned>(r->group));
+  return {static_cast<uint8_t*>(r->codes), static_cast<uint8_t*>(r->scales), r->code_stride,
+          r->scale_stride * (r->dtype == LP_I8 ? 4 : 1), r->dtype == LP_I8, r->group / 8, shift};
+}
+int codec_grid(int64_t threads) {
+  return static_cast<int>(std::min<int64_t>((threads + kCodecThreads - 1) / kCodecThreads,
+                                            device_info().sm_count * 32ll));
+}
+
+}  // namespace
+
+int launch_norm(const lp_matrix& x, const lp_matrix* residual, const void* weight, int weight_type, float eps,
+                const lp_matrix* total, const lp_matrix* y, const lp_rows8* q, bool vec, cudaStream_t st) {
+  NormArgs a{mat(&x), mat(residual), mat(total), mat(y), static_cast<const uint8_t*>(weight), rows8(q),
+             x.rows, static_cast<int>(x.cols), weight_type, eps};
+  const int units = (a.cols + 7) / 8;
+  const int sms = device_info().sm_count;
+  // Few rows: as many threads as there are pieces, whose chains are shortest; many: two
+  // pieces a thread.
+  int c = 1;
+  while ((units + c - 1) / c > 1024) c *= 2;
+  if (c == 1 && units > 64 && x.rows > sms) c = 2;
+  const int threads = ((units + c - 1) / c + 31) / 32 * 32;
+  const int grid = static_cast<int>(std::min<int64_t>(x.rows, sms * 16ll));
+#define LP_NORM(C)                                           \
+  if (c == C) {                                              \
+    if (vec) k_norm<true, C><<<grid, threads, 0, st>>>(a);   \
+    else k_norm<false, C><<<grid, threads, 0, st>>>(a);      \
+    return cuda_status(cudaGetLastError());                  \
+  }
+  LP_NORM(1) LP_NORM(2) LP_NORM(4)
+#undef LP_NORM
+  return LP_ERR_UNSUPPORTED;
+}
+
+int launch_quantize_rows(const lp_matrix& x, const lp_rows8& q, bool vec, cudaStream_t st) {
+  const CodecArgs a{mat(&x), rows8(&q), x.rows, static_cast<int>(x.cols)};
+  const int grid = codec_grid(x.rows * (x.cols / 8));
+  if (vec) k_quantize_rows<true><<<grid, kCodecThreads, 0, st>>>(a);
+  else k_quantize_rows<false><<<grid, kCodecThreads, 0, st>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+int launch_dequantize_rows(const lp_rows8& q, const lp_matrix& x, bool vec, cudaStream_t st) {
+  const CodecArgs a{mat(&x), rows8(&q), x.rows, static_cast<int>(x.cols)};
+  const int grid = codec_grid(x.rows * (x.cols / 8));
+  if (vec) k_dequantize_rows<true><<<grid, kCodecThreads, 0, st>>>(a);
+  else k_dequantize_rows<false><<<grid, kCodecThreads, 0, st>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+int launch_combine(const lp_matrix& rows, const float* weights, const int32_t* places, int64_t k,
+                   const lp_matrix* residual, const lp_matrix& out, bool vec, cudaStream_t st) {
+  const CombineArgs a{mat(&rows), mat(residual), mat(&out), weights, places, out.rows, rows.rows,
+                      static_cast<int>(k), static_cast<int>(out.cols)};
+  const int grid = codec_grid(out.rows * ((out.cols + 7) / 8));
+  if (vec) k_combine<true><<<grid, kCodecThreads, 0, st>>>(a);
+  else k_combine<false><<<grid, kCodecThreads, 0, st>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace lp
