@@ -515,10 +515,12 @@ int lp_add_rms_norm(const lp_matrix *x, const lp_matrix *residual, const void *w
                     int64_t weight_len, int32_t weight_type, float eps, const lp_matrix *total,
                     const lp_matrix *y, const lp_rows8 *q, lp_stream_t stream);
 
-/* Bytes of workspace that lp_route_experts and lp_expert_gemm take on the current device.
- * It is zeroed once, when it is allocated; every call leaves it ready for the next one on
- * the same stream.  Calls that may run at the same time need one each. */
-int lp_experts_workspace(int64_t *bytes);
+/* Bytes of workspace that lp_route_experts and the experts' products take on the current
+ * device: rows and cols are those of the largest product with a row_token (its rows are
+ * gathered there), 0 without one.  It is zeroed once, when it is allocated; every call
+ * leaves it ready for the next one on the same stream.  Calls that may run at the same
+ * time need one each. */
+int lp_experts_workspace(int64_t rows, int64_t cols, int64_t *bytes);
 
 /* Each token's k experts (k at most 32, experts at most 1024) and the order of their rows.
  * logits: tokens x experts.  Out, tokens x k: experts (the k largest logits, largest

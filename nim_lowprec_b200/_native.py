@@ -125,7 +125,7 @@ SIGNATURES = {
     "lp_quantize_rows": "ppp",
     "lp_dequantize_rows": "ppp",
     "lp_add_rms_norm": "pppnifpppp",
-    "lp_experts_workspace": "p",
+    "lp_experts_workspace": "nnp",
     "lp_route_experts": "ppnpnpnpnpnnipnp",
     "lp_expert_weights_bytes": "ppp",
     "lp_expert_weights_pack": "pnpnipp",

@@ -10,7 +10,6 @@ namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
 constexpr int64_t kMaxCols = 32768;  // of a row that is normed
-constexpr int64_t kCountBytes = int64_t{lp::kRouteCtas} * lp::kRouteExperts * 4;
 
 #define LP_REQUIRE(cond)              \
   do {                                \
@@ -94,12 +93,13 @@ int check_product(const lp_expert_weights* w, bool gated, const lp_rows8* x, con
   return aligned16(x) ? LP_OK : LP_ERR_UNSUPPORTED;
 }
 
+int64_t product_workspace(const int32_t* row_token, int64_t rows, int64_t cols) {
+  return lp::experts::fixed_workspace() + (row_token ? lp::experts::gather_workspace(rows, cols) : 0);
+}
 int check_workspace(const void* p, int64_t len, int64_t need) {
   LP_REQUIRE(len >= need);
   return !p || reinterpret_cast<uintptr_t>(p) & 15 ? LP_ERR_ARG : LP_OK;
 }
-
-int64_t workspace_bytes() { return kCountBytes; }
 
 }  // namespace
 
@@ -148,9 +148,10 @@ int lp_add_rms_norm(const lp_matrix* x, const lp_matrix* residual, const void* w
   return lp::launch_norm(*x, residual, weight, weight_type, eps, total, y, q, vec, S(stream));
 }
 
-int lp_experts_workspace(int64_t* bytes) {
+int lp_experts_workspace(int64_t rows, int64_t cols, int64_t* bytes) {
+  LP_REQUIRE(rows >= 0 && rows <= kIntMax && cols >= 0 && cols <= kIntMax);
   if (!bytes) return LP_ERR_ARG;
-  *bytes = workspace_bytes();
+  *bytes = lp::experts::fixed_workspace() + lp::experts::gather_workspace(rows, cols);
   return LP_OK;
 }
 
@@ -166,18 +167,18 @@ int lp_route_experts(const lp_matrix* logits, float* weights, int64_t weights_le
   LP_REQUIRE(weights_len == t * k && experts_len == t * k && row_token_len == t * k && places_len == t * k);
   if (bad(weights, t) || bad(experts, t) || bad(row_token, t) || bad(places, t) || !offsets) return LP_ERR_ARG;
   if (renormalize != 0 && renormalize != 1) return LP_ERR_ARG;
-  if (const int e = check_workspace(workspace, workspace_len, workspace_bytes())) return e;
+  if (const int e = check_workspace(workspace, workspace_len, lp::experts::fixed_workspace())) return e;
   // experts are read again while places are written: nothing that is written may lie on
   // anything else
   const Span s[] = {span(weights, t * k, 4), span(experts, t * k, 4), span(row_token, t * k, 4),
                     span(places, t * k, 4), span(offsets, n + 1, 4),
-                    span(workspace, workspace_bytes(), 1),
+                    span(workspace, lp::experts::fixed_workspace(), 1),
                     span(logits->data, t ? (t - 1) * logits->stride + n : 0, elem_size(logits->dtype))};
   for (const Span& a : s)
     for (const Span& b : s)
       if (&a < &b && meet(a, b)) return LP_ERR_ARG;
   return lp::launch_route(*logits, weights, experts, offsets, row_token, places, k, renormalize,
-                          static_cast<int32_t*>(workspace), S(stream));
+                          reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + lp::experts::kCounterBytes), S(stream));
 }
 
 int lp_expert_weights_bytes(const lp_expert_weights* w, int64_t* tile_bytes, int64_t* scale_bytes) {
@@ -207,7 +208,7 @@ int lp_expert_gemm(const lp_expert_weights* w, const lp_rows8* x, const int32_t*
   if (const int e = check_matrix(out)) return e;
   const int64_t rows = row_token ? row_token_len : x->rows;
   LP_REQUIRE(out->rows == rows && out->cols == w->rows);
-  if (const int e = check_workspace(workspace, workspace_len, workspace_bytes())) return e;
+  if (const int e = check_workspace(workspace, workspace_len, product_workspace(row_token, rows, x->cols))) return e;
   if (rows == 0) return LP_OK;
   LP_REQUIRE(x->rows > 0);
   return lp::launch_experts(*w, *x, offsets, row_token, rows, out, nullptr, workspace, S(stream));
@@ -222,7 +223,7 @@ int lp_expert_gemm_gated(const lp_expert_weights* w, const lp_rows8* x, const in
   const int64_t rows = row_token ? row_token_len : x->rows;
   LP_REQUIRE(out->rows == rows && out->cols == w->rows / 2);
   if (!aligned16(out)) return LP_ERR_UNSUPPORTED;
-  if (const int e = check_workspace(workspace, workspace_len, workspace_bytes())) return e;
+  if (const int e = check_workspace(workspace, workspace_len, product_workspace(row_token, rows, x->cols))) return e;
   if (rows == 0) return LP_OK;
   LP_REQUIRE(x->rows > 0);
   return lp::launch_experts(*w, *x, offsets, row_token, rows, nullptr, out, workspace, S(stream));

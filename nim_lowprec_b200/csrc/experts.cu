@@ -99,45 +99,211 @@ __global__ void __launch_bounds__(256) k_pack_scales(const PackArgs a) {
   }
 }
 
+// --------------------------------------------------------------- gather
+// Rows into the experts' order, scales padded with zeros to whole 16 bytes.  (The
+// products' own loaders gathering row by row was slower: a gather of four rows costs
+// TMA as much as a tile of 128, and copies of 16 bytes by threads made a prompt's
+// gated product 690 us where this and tiles take 420.)
+struct GatherArgs {
+  const uint8_t *codes, *scales;
+  uint8_t *to, *to_scales;
+  int64_t code_stride, scale_stride, to_scale_stride;
+  const int32_t *end, *row_token;  // end: offsets[experts]
+  int64_t rows, tokens;
+  int cols;
+};
+__global__ void __launch_bounds__(256) k_gather(const GatherArgs a) {
+  const int cp = a.cols / 16, sp = static_cast<int>(a.to_scale_stride / 16), per = cp + sp;
+  const int64_t rows = min(a.rows, static_cast<int64_t>(max(__ldg(a.end), 0))), n = rows * per;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t row = n >> 32 ? i / per : static_cast<uint32_t>(i) / static_cast<uint32_t>(per);
+    const int p = static_cast<int>(i - row * per), token = __ldg(a.row_token + row);
+    const bool in = static_cast<uint32_t>(token) < static_cast<uint32_t>(a.tokens);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (p < cp) {
+      if (in) v = __ldg(reinterpret_cast<const uint4*>(a.codes + token * a.code_stride) + p);
+      reinterpret_cast<uint4*>(a.to + row * a.cols)[p] = v;
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+      const uint8_t* from = a.scales + token * a.scale_stride;
+      for (int b = 0; b < 16; ++b) {
+        const int at = 16 * (p - cp) + b;
+        if (in && at < a.cols / 32) w[b >> 2] |= static_cast<uint32_t>(__ldg(from + at)) << (8 * (b & 3));
+      }
+      reinterpret_cast<uint4*>(a.to_scales + row * a.to_scale_stride)[p - cp] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
 // -------------------------------------------------------------- product
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
 constexpr int kMaxN = 240;
+constexpr int kMaxStages = 12;
+constexpr int kSfRing = 3;  // blocks of four chunks' scale factors
 constexpr uint32_t kTmemCols = 512, kSfCol = 480;  // accumulators at 0 and 240
-constexpr int kSfStage = kSfBytes + 1024;          // A's atom, and B's two
 constexpr int kGateTokens = 32, kGatePitch = 65;   // the gated epilogue's transposition
 constexpr int kGateBytes = kGateTokens * kGatePitch * 4;
+constexpr int kBoxes = 5;
 
-__device__ __forceinline__ uint64_t sf_desc(const void* p) {
-  uint64_t d = static_cast<uint64_t>((saddr(p) & 0x3FFFFu) >> 4);
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred P; elect.sync _|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(p));
+  return p != 0;
+}
+
+struct Maps {
+  CUtensorMap a;          // weight tiles
+  CUtensorMap b[kBoxes];  // rows in order, by boxes of 32, 64, 128, 192 and bn
+};
+
+// A block of 32 x 16 bytes at a shared address, as tcgen05.cp reads it.
+__device__ __forceinline__ uint64_t sf_desc(uint32_t at) {
+  uint64_t d = static_cast<uint64_t>((at & 0x3FFFFu) >> 4);
   d |= static_cast<uint64_t>(128 >> 4) << 16;  // core matrices of 8 rows x 16 bytes, one wide
   d |= static_cast<uint64_t>(128 >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
   return d;
 }
-__device__ __forceinline__ void sf_copy(uint32_t taddr, const void* atom) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sf_desc(atom)) : "memory");
+
+// The instructions that differ between one CTA and a pair that shares a tile.
+template <int CG>
+struct Tc;
+#define LP_TC(CG)                                                                                              \
+  template <>                                                                                                  \
+  struct Tc<CG> {                                                                                              \
+    static __device__ __forceinline__ void alloc(uint32_t* dst) {                                              \
+      asm volatile("tcgen05.alloc.cta_group::" #CG ".sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(dst)), \
+                   "r"(kTmemCols)                                                                              \
+                   : "memory");                                                                                \
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::" #CG ".sync.aligned;" ::: "memory");           \
+    }                                                                                                          \
+    static __device__ __forceinline__ void dealloc(uint32_t t) {                                               \
+      asm volatile("tcgen05.dealloc.cta_group::" #CG ".sync.aligned.b32 %0, %1;" ::"r"(t), "r"(kTmemCols)      \
+                   : "memory");                                                                                \
+    }                                                                                                          \
+    static __device__ __forceinline__ void sf_copy(uint32_t t, uint64_t atom) {                                \
+      asm volatile("tcgen05.cp.cta_group::" #CG ".32x128b.warpx4 [%0], %1;" ::"r"(t), "l"(atom)                \
+                   : "memory");                                                                                \
+    }                                                                                                          \
+    static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,             \
+                                               uint32_t sfa, uint32_t sfb, bool add) {                         \
+      asm volatile(                                                                                            \
+          "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::" #CG                                  \
+          ".kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p; }" ::"r"(d),                           \
+          "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(sfa), "r"(sfb)                      \
+          : "memory");                                                                                         \
+    }                                                                                                          \
+  };
+LP_TC(1)
+LP_TC(2)
+#undef LP_TC
+
+// One arrival once every tcgen05 operation issued so far has finished, in each
+// CTA of the pair.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
 }
-__device__ __forceinline__ void mma_mx8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
-                                        uint32_t sfb, bool add) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p; }" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(sfa), "r"(sfb)
-      : "memory");
+// The same in this CTA alone.
+template <int CG>
+__device__ __forceinline__ void commit_own(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    mma_commit(bar);
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar))
+                 : "memory");
+  }
 }
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* tm, int col, const int* row, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(saddr(dst)),
-      "l"(reinterpret_cast<uint64_t>(tm)), "r"(col), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]),
-      "r"(saddr(bar))
-      : "memory");
+// The leading CTA's barrier of the same name.
+template <int CG>
+__device__ __forceinline__ uint32_t lead(uint64_t* bar) {
+  uint32_t a = saddr(bar);
+  if constexpr (CG == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(saddr(bar)));
+  return a;
 }
-__device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   saddr(dst)),
-               "l"(src), "r"(bytes), "r"(saddr(bar))
+template <int CG>
+__device__ __forceinline__ void arrive_lead(uint64_t* bar) {
+  if constexpr (CG == 1) mbar_arrive(bar);
+  else
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead<2>(bar)) : "memory");
+}
+// A converged warp waits for a barrier (its shared address), what the other CTA of a
+// pair wrote before its arrival included.  Bounded as mbar_wait is.
+template <int CG>
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  if constexpr (CG == 1)
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kSuspendHintNs)
+        : "memory");
+  else
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kSuspendHintNs)
+        : "memory");
+  return ok != 0;
+}
+template <int CG>
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort) {
+  const uint64_t t0 = global_ns();
+  while (true) {
+    if (__all_sync(0xffffffffu, try_wait<CG>(bar, parity))) return true;
+    const bool late = global_ns() - t0 > kWaitLimitNs;
+    if (__any_sync(0xffffffffu, late)) {
+      raise_error(LP_ERR_TIMEOUT);
+      *abort = 1;
+      return false;
+    }
+    if (__any_sync(0xffffffffu, *abort != 0)) return false;
+  }
+}
+template <int CG>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (__all_sync(0xffffffffu, try_wait<CG>(bar, parity))) return true;
+  return wait_longer<CG>(bar, parity, abort);
+}
+// A tile of rows into this CTA's shared memory, counted at `bar` (a cluster address).
+template <int CG>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* tm, int c0, int c1, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0)
+               : "memory");
+}
+// One arrival of this thread once the copies that it has issued are there.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(bar)) : "memory");
 }
 
 // The segments, as every CTA reads them from the offsets: an expert's first row,
@@ -146,14 +312,13 @@ __device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t byt
 struct Segments {
   int *row0, *rows, *start;  // start: experts + 1
 };
-__device__ __forceinline__ int tiles_of(int rows, int bn) { return (rows + bn - 1) / bn; }
 // Rows of each tile of a segment: as many tiles as needed, alike, a multiple of 16.
 __device__ __forceinline__ int rows_per(int rows, int bn) {
-  const int nt = max(1, tiles_of(rows, bn));
+  const int nt = (rows + bn - 1) / bn;
   return ((rows + nt - 1) / nt + 15) & ~15;
 }
 
-__device__ __forceinline__ void read_segments(const Args& a, const Segments& s, int lane) {
+__device__ __forceinline__ void read_segments(const Args& a, const Segments& s, int mtiles, int lane) {
   int carry = 0;
   for (int e0 = 0; e0 < a.experts; e0 += 32) {
     const int e = e0 + lane;
@@ -163,7 +328,7 @@ __device__ __forceinline__ void read_segments(const Args& a, const Segments& s, 
       n = max(min(__ldg(a.offsets + e + 1), a.rows) - lo, 0);
       if (n > 0) {
         const int per = rows_per(n, a.bn);
-        tiles = min((n + per - 1) / per * a.mtiles, 1 << 24);
+        tiles = min((n + per - 1) / per * mtiles, 1 << 24);
       }
     }
     int inc = tiles;
@@ -183,17 +348,52 @@ __device__ __forceinline__ void read_segments(const Args& a, const Segments& s, 
   if (lane == 0) s.start[0] = 0;
 }
 
-// A CTA's work, in order.  Every warp walks it by itself.
-struct Tile {
-  int e, mt, row0, n;  // expert, weight tile, first row, rows
+// A CTA's (or pair's) work, in order.  Every warp walks it by itself.  Where there
+// are many tiles, they go round; where there are few, the chunks of all tiles laid
+// end to end are cut into equal shares, and a tile that is cut leaves partial sums.
+struct Item {
+  int e, mt, row0, n;  // expert, weight tile (of the pair), first row, rows
+  int k0, k1;          // chunks of K
+  int first, parts;    // of a cut tile: the first CTA that has some of it, and how many have
 };
 struct Walk {
   const Args& a;
   const Segments& s;
-  int t, e = 0;
-  __device__ Walk(const Args& args, const Segments& seg) : a(args), s(seg), t(blockIdx.x) {}
-  __device__ __forceinline__ bool next(Tile& w) {
-    if (t >= s.start[a.experts]) return false;
+  int ctas, step, total, t, e = 0, mtiles;
+  int64_t pos, end, units;
+  bool split;
+  __device__ Walk(const Args& args, const Segments& seg, int cta, int n, int mt)
+      : a(args), s(seg), ctas(n), step(n), total(seg.start[args.experts]), t(cta), mtiles(mt) {
+    split = a.split && total < a.split * n;
+    if (split) {
+      units = static_cast<int64_t>(total) * a.kchunks;
+      ctas = static_cast<int>(min(static_cast<int64_t>(n), max(units / kLeastUnits, int64_t{1})));
+      pos = units * cta / ctas;
+      end = cta < ctas ? units * (cta + 1) / ctas : 0;
+    }
+  }
+  static constexpr int kLeastUnits = 4;
+  __device__ __forceinline__ int cta_of(int64_t unit) const {
+    return static_cast<int>(((unit + 1) * ctas - 1) / units);
+  }
+  __device__ __forceinline__ bool next(Item& w) {
+    w.k0 = 0;
+    w.k1 = a.kchunks;
+    w.parts = 1;
+    if (split) {
+      if (pos >= end) return false;
+      t = static_cast<int>(pos / a.kchunks);
+      const int64_t base = static_cast<int64_t>(t) * a.kchunks;
+      w.k0 = static_cast<int>(pos - base);
+      w.k1 = static_cast<int>(min(static_cast<int64_t>(a.kchunks), end - base));
+      if (w.k0 > 0 || w.k1 < a.kchunks) {
+        w.first = cta_of(base);
+        w.parts = cta_of(base + a.kchunks - 1) - w.first + 1;
+      }
+      pos += w.k1 - w.k0;
+    } else if (t >= total) {
+      return false;
+    }
     while (t >= s.start[e + 1]) ++e;
     const int rows = s.rows[e], per = rows_per(rows, a.bn), nt = (rows + per - 1) / per;
     const int at = t - s.start[e], j = at % nt;
@@ -201,30 +401,10 @@ struct Walk {
     w.mt = at / nt;
     w.row0 = s.row0[e] + j * per;
     w.n = min(per, rows - j * per);
-    t += gridDim.x;
+    if (!split) t += step;
     return true;
   }
 };
-
-// Four chunks' scale words of one row (nsf scales) from block `blk` of four chunks on.
-__device__ __forceinline__ uint4 load_scales(const Args& a, const uint8_t* p, int blk, int nsf) {
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (p == nullptr) return make_uint4(0, 0, 0, 0);
-  const int b0 = 16 * blk;
-  if (a.xscale_vec == 16 && b0 + 16 <= nsf) return *reinterpret_cast<const uint4*>(p + b0);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int b = b0 + 4 * j;
-    if (a.xscale_vec >= 4) {
-      if (b < nsf) w[j] = *reinterpret_cast<const uint32_t*>(p + b);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (b + i < nsf) w[j] |= static_cast<uint32_t>(p[b + i]) << (8 * i);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 __device__ __forceinline__ float silu_mul(float g, float u) {
   // g / (1 + exp(-g)); the quotient's two units in the last place are far below the
@@ -232,214 +412,247 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return fmul(__fdividef(g, fadd(1.0f, __expf(-g))), u);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release; barrier.cluster.wait.acquire;" ::: "memory");
+}
+// The epilogue's warps agree: true where all have seen true.
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return all != 0;
+}
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <bool GATED>
-__global__ void __launch_bounds__(kThreads, 1)
-    k_experts(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args a) {
-  constexpr int kMaxStages = 12;
+template <int CG, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__ Maps maps, const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ uint64_t full[kMaxStages], sfull[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], done;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sffull[kSfRing], sfempty[kSfRing];
+  __shared__ uint64_t acc_full[2], acc_empty[2], done;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int s_abort;
+  __shared__ int s_last;
 
   uint8_t* smem = smem_raw + ((1024u - (saddr(smem_raw) & 1023u)) & 1023u);
-  const int stage_bytes = kTileM * kChunkK + a.bn * kChunkK;
+  const int stage_bytes = kTileM * kChunkK + a.bn / CG * kChunkK;
   uint8_t* sf_mem = smem + a.stages * stage_bytes;
-  uint8_t* gate_mem = sf_mem + a.stages * kSfStage;
+  uint8_t* gate_mem = sf_mem + kSfRing * a.sf_block;
   int* seg_mem = reinterpret_cast<int*>(gate_mem + (GATED ? kGateBytes : 0));
   const Segments seg{seg_mem, seg_mem + a.experts, seg_mem + 2 * a.experts};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? blockIdx.x & 1 : 0, cta = blockIdx.x / CG, ctas = gridDim.x / CG;
+  const int mtiles = (a.mtiles + CG - 1) / CG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&sfull[s], 2);
+      // (of a pair, the leading CTA's count for both)
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < kSfRing; ++b) {
+      mbar_init(&sffull[b], 1 + 128 + (CG == 2 && rank == 0 ? 1 : 0));
+      mbar_init(&sfempty[b], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], 4 * CG);
     }
     mbar_init(&done, 1);
     s_abort = 0;
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(&tmem_base, kTmemCols);
-  if (warp == 0) read_segments(a, seg, lane);
+  if (warp == 1) Tc<CG>::alloc(&tmem_base);
+  if (warp == 0) read_segments(a, seg, mtiles, lane);
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   fence_after();
   const uint32_t tbase = tmem_base;
-  Walk walk(a, seg);
-  Tile w;
+  const uint32_t stage_at = saddr(smem), sf_at = saddr(sf_mem);
+  const uint32_t full_at = saddr(full), empty_at = saddr(empty), sffull_at = saddr(sffull), sfempty_at = saddr(sfempty);
+  const uint32_t acc_full_at = saddr(acc_full), acc_empty_at = saddr(acc_empty), full_lead = lead<CG>(full);
+  Walk walk(a, seg, cta, ctas, mtiles);
+  Item w;
 
   if (warp == 0) {
-    // ------------------------------------------------------ producer
-    int it = 0, s = 0, phase = 0;
-    bool more = walk.next(w);
-    int idx[2][4], nidx[2][4];
-    auto rows_of = [&](const Tile& t, int (&ix)[2][4]) {
-      // rows past the tile's are row `tokens`, which TMA fills with zeros
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = 4 * (lane + 32 * i) + j;
-          int row = a.tokens;
-          if (c < t.n) {
-            const int v = __ldg(a.row_token + t.row0 + c);
-            if (static_cast<uint32_t>(v) < static_cast<uint32_t>(a.tokens)) row = v;
-          }
-          ix[i][j] = row;
-        }
-      }
-    };
-    if (more && a.row_token) rows_of(w, nidx);
-    while (more) {
-      const int n16 = (w.n + 15) & ~15;
-      const int64_t tile = (static_cast<int64_t>(w.e) * a.mtiles + w.mt) * a.kchunks;
-      const int row0 = w.row0;
-      if (a.row_token) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) idx[i][j] = nidx[i][j];
-      }
-      more = walk.next(w);
-      if (more && a.row_token) rows_of(w, nidx);
-      for (int kc = 0; kc < a.kchunks; ++kc, ++it) {
-        bool ok = true;
-        if (it >= a.stages) ok = mbar_wait(&empty[s], phase ^ 1, &s_abort);
-        ok = __all_sync(0xffffffffu, ok && !s_abort);
+    // ------------------------------------------------------ the weights
+    // (the whole warp walks and waits, and one lane issues: operands then come from the
+    // uniform registers that these instructions take)
+    int it = 0, s = 0, phase = 1, sb = 0, sphase = 1;
+    bool ok = true;
+    while (ok && walk.next(w)) {
+      const int mt = min(w.mt * CG + rank, a.mtiles - 1);  // (a pair's second tile may not exist)
+      const int tile = (w.e * a.mtiles + mt) * a.kchunks;
+      for (int kc = w.k0; kc < w.k1; ++kc, ++it) {
+        ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort);  // (the first round passes)
         if (!ok) break;
-        uint8_t* st = smem + s * stage_bytes;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full[s], a.a_bytes + kSfBytes + n16 * kChunkK);
-          tma_load_2d(st, &tmA, 0, static_cast<int>((tile + kc) * kTileM), &full[s]);
-          bulk_in(sf_mem + s * kSfStage, a.wscales + (tile + kc) * kSfBytes, kSfBytes, &full[s]);
+        if (elect_one()) {
+          if (rank == 0) expect_tx(full_at + 8 * s, CG * a.a_bytes);
+          load_tile<CG>(stage_at + s * stage_bytes, &maps.a, 0, (tile + kc) * kTileM, full_lead + 8 * s);
         }
         __syncwarp();
-        uint8_t* b = st + kTileM * kChunkK;
-        if (a.row_token) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int g = lane + 32 * i;
-            if (4 * g < n16) tma_gather4(b + g * 4 * kChunkK, &tmB, kc * kChunkK, idx[i], &full[s]);
-          }
-        } else if (16 * lane < n16) {
-          tma_load_2d(b + lane * 16 * kChunkK, &tmB, kc * kChunkK, row0 + 16 * lane, &full[s]);
-        }
         if (++s == a.stages) s = 0, phase ^= 1;
+        if (kc != w.k0 && (kc & 3)) continue;
+        // the atoms of the block of four chunks
+        ok = warp_wait<1>(sfempty_at + 8 * sb, sphase, &s_abort);
+        if (!ok) break;
+        if (elect_one()) {
+          const int at = kc & ~3, n = min(4, a.kchunks - at) * kSfBytes;
+          expect_tx(sffull_at + 8 * sb, n);
+          bulk_in(sf_at + sb * a.sf_block, a.wscales + (tile + at) * int64_t{kSfBytes}, n, sffull_at + 8 * sb);
+        }
+        __syncwarp();
+        if (++sb == kSfRing) sb = 0, sphase ^= 1;
       }
-      if (s_abort) break;
     }
-    // copies in flight end before the CTA does
-    for (int u = max(0, it - a.stages); u < it; ++u) mbar_wait(&full[u % a.stages], (u / a.stages) & 1);
+    // What is in flight here, copies and signals, ends before the CTA does: the last stages
+    // are waited for as if they were to be filled again.
+    for (int u = 0; ok && u < min(it, a.stages); ++u) {
+      if (--s < 0) s = a.stages - 1, phase ^= 1;
+      ok = warp_wait<1>(empty_at + 8 * s, phase ^ 1, &s_abort);
+    }
+    if (!ok)
+      for (const uint64_t t0 = global_ns(); global_ns() - t0 < 1000000;) __nanosleep(1000);
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      int s = 0, phase = 0, item = 0, it = 0;
+    if (rank == 0) {
+      int s = 0, phase = 0, item = 0, sb = 0, sphase = 0;
       bool ok = true;
+      const uint32_t a_desc = static_cast<uint32_t>(sw128_desc(smem));  // (the high word is the same everywhere)
+      const uint32_t desc_high = static_cast<uint32_t>(sw128_desc(smem) >> 32);
+      auto desc = [&](uint32_t low) { return static_cast<uint64_t>(desc_high) << 32 | low; };
       while (ok && walk.next(w)) {
         const int buf = item & 1;
-        if (item >= 2) ok = mbar_wait(&acc_empty[buf], ((item >> 1) & 1) ^ 1, &s_abort);
-        fence_after();
+        ok = warp_wait<CG>(acc_empty_at + 8 * buf, ((item >> 1) & 1) ^ 1, &s_abort);
         const int n16 = (w.n + 15) & ~15;
         const uint32_t idesc = a.idesc | static_cast<uint32_t>(n16 >> 3) << 17;
         const uint32_t acc = tbase + buf * kMaxN;
-        for (int kc = 0; ok && kc < a.kchunks; ++kc, ++it) {
-          ok = mbar_wait(&full[s], phase, &s_abort) && mbar_wait(&sfull[s], phase, &s_abort) && !s_abort;
-          if (!ok) break;
-          fence_after();
-          const uint8_t* st = smem + s * stage_bytes;
-          const uint8_t* sf = sf_mem + s * kSfStage;
-          const uint32_t sfa = tbase + kSfCol + (it & 1) * 12, sfb = sfa + 4;
-          sf_copy(sfa, sf);
-          sf_copy(sfb, sf + kSfBytes);
-          if (n16 > 128) sf_copy(sfb + 4, sf + kSfBytes + 512);
-          const uint64_t ad = sw128_desc(st), bd = sw128_desc(st + kTileM * kChunkK);
-          const int blocks = min(4, (a.k - kc * kChunkK) >> 5);
+        const bool wide = n16 > 128;
+        bool add = false;
+        for (int k4 = w.k0 & ~3; ok && k4 < w.k1; k4 += 4) {
+          ok = warp_wait<CG>(sffull_at + 8 * sb, sphase, &s_abort);
+          const uint64_t sf = sf_desc(sf_at + sb * a.sf_block), sfr = sf_desc(sf_at + sb * a.sf_block + 4 * kSfBytes);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j < blocks)
-              mma_mx8(acc, ad + 2 * j, bd + 2 * j, idesc | static_cast<uint32_t>(j) << 4 | static_cast<uint32_t>(j) << 29,
-                      sfa | static_cast<uint32_t>(j) << 30, sfb | static_cast<uint32_t>(j) << 30, kc > 0 || j > 0);
+          for (int c = 0; c < 4; ++c) {
+            const int kc = k4 + c;
+            if (!ok || kc < w.k0 || kc >= w.k1) continue;
+            ok = warp_wait<CG>(full_at + 8 * s, phase, &s_abort);
+            if (!ok) continue;
+            // rows and scale factors came by generic writes, and are read by the asynchronous proxy
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fence_after();
+            const uint32_t low = a_desc + s * (stage_bytes >> 4);
+            const uint32_t sfa = tbase + kSfCol + (c & 1) * 12, sfb = sfa + 4;
+            const int blocks = (a.k - kc * kChunkK) >> 5;
+            const uint32_t sfc = c * (a.sf_rows >> 4);
+            if (elect_one()) {
+              Tc<CG>::sf_copy(sfa, sf + c * (kSfBytes >> 4));
+              Tc<CG>::sf_copy(sfb, sfr + sfc);
+              if (wide) Tc<CG>::sf_copy(sfb + 4, sfr + sfc + (512 >> 4));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (j < blocks)
+                  Tc<CG>::mma(acc, desc(low + 2 * j), desc(low + (kTileM * kChunkK >> 4) + 2 * j),
+                              idesc | static_cast<uint32_t>(j) << 4 | static_cast<uint32_t>(j) << 29,
+                              sfa | static_cast<uint32_t>(j) << 30, sfb | static_cast<uint32_t>(j) << 30, add || j > 0);
+              }
+              commit<CG>(empty_at + 8 * s);
+              if (c == 3 || kc + 1 == w.k1) commit<CG>(sfempty_at + 8 * sb);
+            }
+            __syncwarp();
+            add = true;
+            if (++s == a.stages) s = 0, phase ^= 1;
           }
-          mma_commit(&empty[s]);
-          if (++s == a.stages) s = 0, phase ^= 1;
+          if (++sb == kSfRing) sb = 0, sphase ^= 1;
         }
-        mma_commit(&acc_full[buf]);
+        if (elect_one()) commit<CG>(acc_full_at + 8 * buf);
+        __syncwarp();
         ++item;
       }
       // every MMA issued must be finished before tensor memory is freed
-      mma_commit(&done);
+      if (elect_one()) commit_own<CG>(&done);
+      __syncwarp();
       mbar_wait(&done, 0);
-    }
-  } else if (warp < 4) {
-    // ------------------------------------------- the rows' scale factors
-    const int first = (warp - 2) * 32 + lane, nsf = a.k >> 5, blks = (a.kchunks + 3) / 4;
-    const uint8_t *row[4], *nrow[4];
-    uint4 nxt[4];
-    auto rows_of = [&](const Tile& t, const uint8_t* (&p)[4]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = first + 64 * i;
-        p[i] = nullptr;
-        if (c < t.n) {
-          const int v = a.row_token ? __ldg(a.row_token + t.row0 + c) : t.row0 + c;
-          if (static_cast<uint32_t>(v) < static_cast<uint32_t>(a.tokens)) p[i] = a.xscales + v * a.xscale_stride;
+    } else {
+      // The other CTA of a pair: its scale factors are there, says this warp to the leading
+      // one's barriers.
+      int sb = 0, sphase = 0;
+      bool ok = true;
+      while (ok && walk.next(w)) {
+        for (int k4 = w.k0 & ~3; k4 < w.k1; k4 += 4) {
+          ok = warp_wait<1>(sffull_at + 8 * sb, sphase, &s_abort);
+          if (!ok) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (lane == 0) arrive_lead<CG>(&sffull[sb]);
+          __syncwarp();
+          if (++sb == kSfRing) sb = 0, sphase ^= 1;
         }
       }
-    };
-    int it = 0, s = 0, phase = 0;
-    bool more = walk.next(w), ok = true;
-    if (more) {
-      rows_of(w, nrow);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) nxt[i] = load_scales(a, nrow[i], 0, nsf);
     }
-    while (more && ok) {
-      const int n = w.n;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) row[i] = nrow[i];
-      more = walk.next(w);
-      if (more) rows_of(w, nrow);
-      for (int blk = 0; ok && blk < blks; ++blk) {
-        uint32_t cur[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          cur[i][0] = nxt[i].x, cur[i][1] = nxt[i].y, cur[i][2] = nxt[i].z, cur[i][3] = nxt[i].w;
-        }
-        if (blk + 1 < blks) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nxt[i] = load_scales(a, row[i], blk + 1, nsf);
-        } else if (more) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nxt[i] = load_scales(a, nrow[i], 0, nsf);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (4 * blk + j >= a.kchunks) break;
-          if (it >= a.stages) ok = mbar_wait(&empty[s], phase ^ 1, &s_abort);
-          ok = __all_sync(0xffffffffu, ok && !s_abort);
+  } else if (warp == 2) {
+    // --------------------------------------------------- rows in order
+    {
+      int s = 0, phase = 1;
+      bool ok = true;
+      while (ok && walk.next(w)) {
+        const int half = ((w.n + 15) & ~15) / CG;  // of this CTA
+        const int box = half <= 32 ? 0 : half <= 64 ? 1 : half <= 128 ? 2 : half <= 192 ? 3 : 4;
+        const int rows = min(box == 4 ? 256 : box == 3 ? 192 : 32 << box, a.bn / CG);
+        const CUtensorMap* tm = &maps.b[box];
+        const int row = w.row0 + rank * half;
+        for (int kc = w.k0; kc < w.k1; ++kc) {
+          ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort);
           if (!ok) break;
-          uint8_t* atoms = sf_mem + s * kSfStage + kSfBytes;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = first + 64 * i;
-            if (64 * i < n) *reinterpret_cast<uint32_t*>(atoms + 512 * (c >> 7) + sf_off(c & 127, 0)) = cur[i][j];
+          if (elect_one()) {
+            if (rank == 0) expect_tx(full_at + 8 * s, CG * rows * kChunkK);
+            load_tile<CG>(stage_at + s * stage_bytes + kTileM * kChunkK, tm, kc * kChunkK, row, full_lead + 8 * s);
           }
-          // generic writes, read by tcgen05.cp through the asynchronous proxy
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sfull[s]);
-          ++it;
           if (++s == a.stages) s = 0, phase ^= 1;
         }
       }
     }
-  } else {
+  } else if (warp >= 8) {
+    // ------------------------------------------- the rows' scale factors
+    // (copies that arrive at the barrier by themselves: nothing here waits for memory)
+    const int lt = threadIdx.x - 256, nsf = a.k >> 5;
+    int sb = 0, sphase = 1;
+    bool ok = true;
+    while (ok && walk.next(w)) {
+      for (int k4 = w.k0 & ~3; k4 < w.k1; k4 += 4) {
+        ok = warp_wait<1>(sfempty_at + 8 * sb, sphase, &s_abort);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = lt + 128 * i, row = w.row0 + c;
+          if (128 * i >= w.n) continue;
+          const uint32_t to = sf_at + sb * a.sf_block + 4 * kSfBytes + 512 * i + sf_off(lt, 0);
+          const bool in = c < w.n && row < a.tokens;
+          const uint8_t* p = a.xscales + (in ? row : 0) * a.xscale_stride + 4 * k4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (a.xscale_words) {
+              const bool on = in && 4 * (k4 + j) < nsf;
+              cp_async4(to + j * a.sf_rows, on ? p + 4 * j : a.xscales, on);
+            } else {
+              uint32_t word = 0;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (in && 4 * (k4 + j) + e < nsf) word |= static_cast<uint32_t>(__ldg(p + 4 * j + e)) << (8 * e);
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + j * a.sf_rows), "r"(word) : "memory");
+            }
+          }
+        }
+        if (a.xscale_words) cp_async_arrive(&sffull[sb]);
+        else mbar_arrive(&sffull[sb]);
+        if (++sb == kSfRing) sb = 0, sphase ^= 1;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= 4) {
     // ------------------------------------------------------ epilogue
     const int q = warp & 3;  // the warp's lanes of tensor memory
     const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
@@ -448,19 +661,62 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (walk.next(w)) {
       const int buf = item & 1;
       bool ok = mbar_wait(&acc_full[buf], (item >> 1) & 1, &s_abort);
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-      if (!ok) break;
+      // (warps that gave up and warps that did not must not part at the barriers below)
+      if (!epilogue_all(ok && !s_abort)) break;
       fence_after();
       const uint32_t acc = tbase + lanes + buf * kMaxN;
-      if constexpr (!GATED) {
-        const int m = w.mt * kTileM + 32 * q + lane;
-        uint8_t* out = a.out + w.row0 * a.out_stride + static_cast<int64_t>(m) * size_of(a.out_type);
+      const int mt = w.mt * CG + rank;
+      bool write = mt < a.mtiles;
+      const float* parts = nullptr;
+      if (CG == 1 && w.parts > 1) {
+        // partial sums: column by column, 128 rows each; the last CTA to arrive adds
+        // them in the CTAs' order
+        float* mine = a.partials + (2 * cta + (w.k0 == 0)) * int64_t{kSplitN * kTileM} + 32 * q + lane;
         for (int c0 = 0; c0 < w.n; c0 += 16) {
           uint32_t v[16];
           tmem_ld16(acc + c0, v);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c0 + i < w.n) __stcg(mine + (c0 + i) * kTileM, __uint_as_float(v[i]));
+        }
+        __threadfence();
+        epilogue_sync();
+        if (threadIdx.x == 128) {
+          const int last = atomicAdd(a.counters + w.first, 1u) == static_cast<uint32_t>(w.parts - 1);
+          if (last) a.counters[w.first] = 0;
+          __threadfence();
+          s_last = last;
+        }
+        epilogue_sync();
+        write = s_last;
+        parts = a.partials + 32 * q + lane;
+      }
+      auto part = [&](int p, int c) {
+        return __ldcg(parts + (2 * (w.first + p) + (p == 0)) * int64_t{kSplitN * kTileM} + c * kTileM);
+      };
+      if (!write) {
+      } else if constexpr (!GATED) {
+        const int m = mt * kTileM + 32 * q + lane;
+        uint8_t* out = a.out + w.row0 * a.out_stride + static_cast<int64_t>(m) * size_of(a.out_type);
+        for (int c0 = 0; c0 < w.n; c0 += 16) {
+          uint32_t v[16];
+          if (CG == 1 && parts) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float sum = 0.0f;
+              if (c0 + i < w.n)
+                for (int p = 0; p < w.parts; ++p) sum = fadd(sum, part(p, c0 + i));
+              v[i] = __float_as_uint(sum);
+            }
+          } else {
+            tmem_ld16(acc + c0, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));
+          }
           if (m < a.features) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -470,10 +726,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         for (int c0 = 0; c0 < w.n; c0 += kGateTokens) {
           uint32_t v[32];
-          tmem_ld32(acc + c0, v);  // (past the tile's columns: whatever is there, not stored)
-          tmem_wait_ld();
+          if (CG == 1 && parts) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));
+            for (int i = 0; i < 32; ++i) {
+              float sum = 0.0f;
+              if (c0 + i < w.n)
+                for (int p = 0; p < w.parts; ++p) sum = fadd(sum, part(p, c0 + i));
+              v[i] = __float_as_uint(sum);
+            }
+          } else {
+            tmem_ld32(acc + c0, v);  // (past the tile's columns: whatever is there, not stored)
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));
+          }
           const bool up = lane & 16;  // this lane holds an up row; its partner the gate's
           const int f = 16 * q + (lane & 15);
 #pragma unroll
@@ -484,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           epilogue_sync();
           // 16 features of a token each; two lanes hold a block of 32
-          const int t = 8 * q + (lane >> 2), f0 = 16 * (lane & 3), feature = w.mt * 64 + f0;
+          const int t = 8 * q + (lane >> 2), f0 = 16 * (lane & 3), feature = mt * 64 + f0;
           float x[16], top = 0.0f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -505,15 +771,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) arrive_lead<CG>(&acc_empty[buf]);
       ++item;
     }
   }
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // nobody's shared memory goes while the pair still reads or signals there
   if (warp == 1) {
+    __syncwarp();
     fence_after();
-    tmem_dealloc(tbase, kTmemCols);
+    Tc<CG>::dealloc(tbase);
   }
 }
 
@@ -539,22 +807,41 @@ bool encode_rows(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool GATED>
-int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& a, int smem, cudaStream_t st) {
+template <int CG, bool GATED>
+int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   const DeviceInfo& di = device_info();
-  auto kern = k_experts<GATED>;
-  static int set[kMaxDevices];
+  auto kern = k_experts<CG, GATED>;
+  static int ctas[kMaxDevices];  // of a full grid, 0 before the first launch
   const int slot = di.ordinal % kMaxDevices;
-  if (set[slot] < smem) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, di.max_smem_optin - 1024);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t c{};
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  c.attrs = &attr;
+  c.numAttrs = CG == 2 ? 1 : 0;
+  if (!ctas[slot]) {
+    const int most = di.max_smem_optin - 1024;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return cuda_status(e);
-    set[slot] = di.max_smem_optin - 1024;
+    int n = di.sm_count;
+    if (CG == 2) {  // as many pairs as fit at a time
+      c.gridDim = dim3(di.sm_count / 2 * 2);
+      c.dynamicSmemBytes = most;
+      e = cudaOccupancyMaxActiveClusters(&n, kern, &c);
+      if (e != cudaSuccess) return cuda_status(e);
+      if (n < 1) return LP_ERR_UNSUPPORTED;
+      n *= 2;
+      c.dynamicSmemBytes = smem;
+    }
+    ctas[slot] = n;
   }
-  kern<<<di.sm_count, kThreads, smem, st>>>(ta, tb, a);
-  return cuda_status(cudaGetLastError());
+  c.gridDim = dim3(ctas[slot]);
+  return cuda_status(cudaLaunchKernelEx(&c, kern, maps, a));
 }
-
 }  // namespace
 
 int launch_pack_experts(const void* codes, const void* scales, int scale_type, const lp_expert_weights& w,
@@ -571,18 +858,30 @@ int launch_pack_experts(const void* codes, const void* scales, int scale_type, c
   return cuda_status(cudaGetLastError());
 }
 
-int launch_experts(const lp_expert_weights& w, const lp_rows8& x, const int32_t* offsets, const int32_t* row_token,
+int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int32_t* offsets, const int32_t* row_token,
                    int64_t rows, const lp_matrix* out, const lp_rows8* out8, void* workspace, cudaStream_t st) {
+  uint8_t* space = static_cast<uint8_t*>(workspace);
+  lp_rows8 x = given;
+  if (row_token) {
+    x = gathered_rows(rows, given.cols, space + fixed_workspace());
+    const GatherArgs g{static_cast<const uint8_t*>(given.codes), static_cast<const uint8_t*>(given.scales),
+                       static_cast<uint8_t*>(x.codes), static_cast<uint8_t*>(x.scales), given.code_stride,
+                       given.scale_stride, x.scale_stride, offsets + w.experts, row_token, rows, given.rows,
+                       static_cast<int>(given.cols)};
+    const int64_t pieces = rows * (given.cols / 16 + x.scale_stride / 16);
+    const int grid = static_cast<int>(std::min<int64_t>((pieces + 255) / 256, device_info().sm_count * 16ll));
+    k_gather<<<grid, 256, 0, st>>>(g);
+    if (const int e = cuda_status(cudaGetLastError())) return e;
+  }
   const Layout l = layout(w.experts, w.rows, w.cols, w.dtype, w.gated);
   Args a{};
   a.wscales = static_cast<const uint8_t*>(w.scales);
   a.xscales = static_cast<const uint8_t*>(x.scales);
   a.xscale_stride = x.scale_stride;
-  const uintptr_t al = reinterpret_cast<uintptr_t>(x.scales) | static_cast<uintptr_t>(x.scale_stride);
-  // (a word holds four scales of one row where a row has a multiple of four)
-  a.xscale_vec = x.cols % kChunkK ? 1 : (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 1;
+  // (a word holds four scales of one row where a row has a multiple of four, or zeros behind them)
+  a.xscale_words =
+      (row_token || x.cols % kChunkK == 0) && ((reinterpret_cast<uintptr_t>(x.scales) | static_cast<uintptr_t>(x.scale_stride)) & 3) == 0;
   a.offsets = offsets;
-  a.row_token = row_token;
   a.experts = static_cast<int>(w.experts);
   a.mtiles = static_cast<int>(l.mtiles);
   a.kchunks = static_cast<int>(l.kchunks);
@@ -590,8 +889,8 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& x, const int32_t*
   a.rows = static_cast<int>(rows);
   a.tokens = static_cast<int>(x.rows);
   a.a_bytes = static_cast<uint32_t>(l.tile_bytes);
-  // A e2m1 (5) or e4m3 (0), B e4m3, both K-major, E8M0 scales, M = 128
-  a.idesc = (w.dtype == LP_E2M1 ? 5u << 7 : 0u) | 1u << 23 | static_cast<uint32_t>(128 >> 4) << 24;
+  // A e2m1 (5) or e4m3 (0), B e4m3, both K-major, E8M0 scales
+  a.idesc = (w.dtype == LP_E2M1 ? 5u << 7 : 0u) | 1u << 23;
   if (out) {
     a.out = static_cast<uint8_t*>(out->data);
     a.out_stride = out->stride * size_of(out->dtype);
@@ -604,25 +903,36 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& x, const int32_t*
     a.out_scale_stride = out8->scale_stride;
     a.features = static_cast<int>(out8->cols);
   }
-  a.partials = static_cast<float*>(workspace);
+  a.counters = reinterpret_cast<uint32_t*>(space);
+  a.partials = reinterpret_cast<float*>(space + kCounterBytes);
   // A token has at most one row per expert, so no segment is longer than x.
-  const int64_t most = row_token ? std::min(rows, x.rows) : rows;
+  const int64_t most = row_token ? std::min(rows, given.rows) : rows;
   const int64_t mean = (rows + w.experts - 1) / w.experts;
   int bn = kMaxN;
   if (mean <= 16) bn = 32;
   else if (mean <= 48) bn = 64;
   else if (mean <= 112) bn = 128;
+  int cg = mean > 112 ? 2 : 1;
   a.bn = static_cast<int>(std::min<int64_t>(bn, (most + 15) / 16 * 16));
-  const int fixed = 1024 + (w.gated ? kGateBytes : 0) + static_cast<int>(3 * w.experts + 1) * 4;
-  const int stage = (kTileM + a.bn) * kChunkK + kSfStage;
-  a.stages = std::min(12, (device_info().max_smem_optin - 1024 - fixed) / stage);
+  a.split = a.bn <= kSplitN && cg == 1 ? 8 : 0;
+  a.sf_rows = a.bn > 128 ? 1024 : 512;
+  a.sf_block = 4 * (kSfBytes + a.sf_rows);
+  const int fixed = 1024 + kSfRing * a.sf_block + (w.gated ? kGateBytes : 0)+
+                    static_cast<int>(3 * w.experts + 1) * 4;
+  const int stage = (kTileM + a.bn / cg) * kChunkK;
+  a.stages = std::min(kMaxStages, (device_info().max_smem_optin - 1024 - fixed) / stage);
   if (a.stages < 2) return LP_ERR_UNSUPPORTED;
-  CUtensorMap ta, tb;
-  if (!encode_tiles(&ta, w.tiles, l.tiles, w.dtype == LP_E2M1) ||
-      !encode_rows(&tb, x.codes, x.cols, x.rows, x.code_stride, row_token ? 1 : 16))
-    return LP_ERR_UNSUPPORTED;
+  Maps maps;
+  if (!encode_tiles(&maps.a, w.tiles, l.tiles, w.dtype == LP_E2M1)) return LP_ERR_UNSUPPORTED;
+  const int boxes[kBoxes] = {32, 64, 128, 192, 256};
+  for (int b = 0; b < kBoxes; ++b)
+    if (!encode_rows(&maps.b[b], x.codes, x.cols, x.rows, x.code_stride, std::min(boxes[b], a.bn / cg)))
+      return LP_ERR_UNSUPPORTED;
   const int smem = fixed + a.stages * stage;
-  return w.gated ? launch<true>(ta, tb, a, smem, st) : launch<false>(ta, tb, a, smem, st);
+  // M = 128 of a CTA, or 256 of a pair
+  a.idesc |= static_cast<uint32_t>(cg * 128 >> 4) << 24;
+  if (w.gated) return cg == 2 ? launch<2, true>(maps, a, smem, st) : launch<1, true>(maps, a, smem, st);
+  return cg == 2 ? launch<2, false>(maps, a, smem, st) : launch<1, false>(maps, a, smem, st);
 }
 
 unsigned int take_error_experts() {

@@ -64,27 +64,33 @@ def addRmsNorm(x, residual, weight, eps, total=None, y=None, codes=None, scales=
         N.check(status, "addRmsNorm")
 
 
-def expertsWorkspace(device=None):
-    """A workspace for routeExperts, expertGemm and expertGemmGated, zeroed.  Calls that may run at
-    the same time (on several streams, in several captured graphs) need one each."""
+def expertsWorkspace(device=None, rows=0, columns=0):
+    """A workspace for routeExperts, expertGemm and expertGemmGated, zeroed; rows and columns are
+    those of the largest product with a rowToken.  Calls that may run at the same time (on several
+    streams, in several captured graphs) need one each."""
     with torch.cuda.device(device):
-        size = ctypes.c_int64()
-        N.check(N.lib().lp_experts_workspace(ctypes.byref(size)), "expertsWorkspace")
-        return torch.zeros(size.value, dtype=torch.uint8, device="cuda")
+        return torch.zeros(_workspace_bytes(rows, columns), dtype=torch.uint8, device="cuda")
+
+
+def _workspace_bytes(rows, columns):
+    size = ctypes.c_int64()
+    N.check(N.lib().lp_experts_workspace(rows, columns, ctypes.byref(size)), "expertsWorkspace")
+    return size.value
 
 
 _workspaces = {}  # (device, stream) -> the workspace of calls that bring none
 
 
-def _workspace(t, name):
+def _workspace(t, name, gather=None):
     fast, index = _fast(), _cuda(t, name).device.index
     if fast.capturing(index):
         raise RuntimeError(f"{name}: a captured call needs a workspace of its own "
                            "(expertsWorkspace(), made before the capture)")
     key = (index, fast.current_stream(index))
     workspace = _workspaces.get(key)
-    if workspace is None:
-        workspace = _workspaces[key] = expertsWorkspace(t.device)
+    rows, columns = (gather.numel(), t.shape[-1]) if gather is not None else (0, 0)
+    if workspace is None or (rows and workspace.numel() < _workspace_bytes(rows, columns)):
+        workspace = _workspaces[key] = expertsWorkspace(t.device, rows, columns)
     return workspace
 
 
@@ -176,7 +182,7 @@ def expertGemm(w, codes, scales, offsets, out, rowToken=None, workspace=None):
     rows of no expert are left alone.  Products are exact, sums fp32, results rounded once.
     Workspace as in routeExperts."""
     if workspace is None:
-        workspace = _workspace(codes, "expertGemm")
+        workspace = _workspace(codes, "expertGemm", rowToken)
     status = _fast().expert_gemm(w._ref, w._index, codes, scales, offsets, rowToken, out, workspace)
     if status:
         N.check(status, "expertGemm")
@@ -187,7 +193,7 @@ def expertGemmGated(w, codes, scales, offsets, outCodes, outScales, rowToken=Non
     expertGemm's rows (lp_expert_gemm_gated): the rows of the down projection's expertGemm.
     `w` is laid out with gated=True."""
     if workspace is None:
-        workspace = _workspace(codes, "expertGemmGated")
+        workspace = _workspace(codes, "expertGemmGated", rowToken)
     status = _fast().expert_gemm_gated(w._ref, w._index, codes, scales, offsets, rowToken, outCodes,
                                        outScales, workspace)
     if status:
