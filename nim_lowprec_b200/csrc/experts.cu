@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "experts.cuh"
 #include "rows.cuh"
@@ -136,13 +137,13 @@ __global__ void __launch_bounds__(256) k_gather(const GatherArgs a) {
 }
 
 // -------------------------------------------------------------- product
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kMaxN = 240;
 constexpr int kMaxStages = 12;
 constexpr int kSfRing = 3;  // blocks of four chunks' scale factors
 constexpr uint32_t kTmemCols = 512, kSfCol = 480;  // accumulators at 0 and 240
 constexpr int kGateTokens = 32, kGatePitch = 65;   // the gated epilogue's transposition
-constexpr int kGateBytes = kGateTokens * kGatePitch * 4;
+constexpr int kGateBytes = 2 * kGateTokens * kGatePitch * 4;  // of two groups of warps
 constexpr int kBoxes = 5;
 
 __device__ __forceinline__ bool elect_one() {
@@ -268,8 +269,28 @@ __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile
     if (__any_sync(0xffffffffu, *abort != 0)) return false;
   }
 }
+// Whether a barrier's phase is over, without waiting.  Asked one step ahead, so that the
+// answer is there when it is needed: a wait that finds its barrier ready takes about 100
+// cycles all the same, half of what a chunk of few rows may take.
 template <int CG>
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool peek(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  if constexpr (CG == 1)
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+  else
+    asm volatile(
+        "{ .reg .pred p; mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  return ok != 0;
+}
+template <int CG>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, bool ready = false) {
+  if (__all_sync(0xffffffffu, ready)) return true;
   if (__all_sync(0xffffffffu, try_wait<CG>(bar, parity))) return true;
   return wait_longer<CG>(bar, parity, abort);
 }
@@ -306,11 +327,12 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(saddr(bar)) : "memory");
 }
 
-// The segments, as every CTA reads them from the offsets: an expert's first row,
-// its rows, and the tiles of the experts before it.  Offsets are clamped to the
-// rows there are, so that no value in them leads out of range.
+// The segments that have rows, as every CTA reads them from the offsets: the expert, its
+// first row, its rows, and the tiles of those before it.  Offsets are clamped to the rows
+// there are, so that no value in them leads out of range.
 struct Segments {
-  int *row0, *rows, *start;  // start: experts + 1
+  int *id, *row0, *rows, *tiles, *start;  // tiles: along the rows; start: one more
+  int* count;
 };
 // Rows of each tile of a segment: as many tiles as needed, alike, a multiple of 16.
 __device__ __forceinline__ int rows_per(int rows, int bn) {
@@ -318,19 +340,23 @@ __device__ __forceinline__ int rows_per(int rows, int bn) {
   return ((rows + nt - 1) / nt + 15) & ~15;
 }
 
+// One warp; the offsets lie in s.start.
 __device__ __forceinline__ void read_segments(const Args& a, const Segments& s, int mtiles, int lane) {
-  int carry = 0;
+  int carry = 0, kept = 0;
+  int next = lane < a.experts ? s.start[lane] : 0;
   for (int e0 = 0; e0 < a.experts; e0 += 32) {
     const int e = e0 + lane;
-    int lo = 0, n = 0, tiles = 0;
+    int lo = 0, n = 0, along = 0, tiles = 0;
     if (e < a.experts) {
-      lo = min(max(__ldg(a.offsets + e), 0), a.rows);
-      n = max(min(__ldg(a.offsets + e + 1), a.rows) - lo, 0);
+      lo = min(max(next, 0), a.rows);
+      n = max(min(s.start[e + 1], a.rows) - lo, 0);
       if (n > 0) {
         const int per = rows_per(n, a.bn);
-        tiles = min((n + per - 1) / per * mtiles, 1 << 24);
+        along = (n + per - 1) / per;
+        tiles = min(along * mtiles, 1 << 24);
       }
     }
+    next = e + 32 < a.experts ? s.start[e + 32] : 0;
     int inc = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -338,14 +364,24 @@ __device__ __forceinline__ void read_segments(const Args& a, const Segments& s, 
       if (lane >= o) inc += up;
     }
     inc = min(inc + carry, 1 << 30);  // (more than any segments in order come to)
-    if (e < a.experts) {
-      s.row0[e] = lo;
-      s.rows[e] = n;
-      s.start[e + 1] = inc;
+    const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
+    __syncwarp();  // (what is written below has been read: at most as many as went by)
+    if (n > 0) {
+      const int at = kept + __popc(some & ((1u << lane) - 1));
+      s.id[at] = e;
+      s.row0[at] = lo;
+      s.rows[at] = n;
+      s.tiles[at] = along;
+      s.start[at + 1] = inc;
     }
+    kept += __popc(some);
     carry = __shfl_sync(0xffffffffu, inc, 31);
+    __syncwarp();
   }
-  if (lane == 0) s.start[0] = 0;
+  if (lane == 0) {
+    s.start[0] = 0;
+    *s.count = kept;
+  }
 }
 
 // A CTA's (or pair's) work, in order.  Every warp walks it by itself.  Where there
@@ -359,49 +395,70 @@ struct Item {
 struct Walk {
   const Args& a;
   const Segments& s;
-  int ctas, step, total, t, e = 0, mtiles;
-  int64_t pos, end, units;
+  int ctas, step, total, t, e = 0, g, steps;  // steps: of g chunks, of a tile
+  int at = 0, left = 0, share = 0, more = 0;  // steps: into the tile, of this CTA; `more` CTAs have one more than the share
   bool split;
-  __device__ Walk(const Args& args, const Segments& seg, int cta, int n, int mt)
-      : a(args), s(seg), ctas(n), step(n), total(seg.start[args.experts]), t(cta), mtiles(mt) {
-    split = a.split && total < a.split * n;
+  __device__ Walk(const Args& args, const Segments& seg, int cta, int n, int chunks)
+      : a(args), s(seg), ctas(n), step(n), total(seg.start[*seg.count]), t(cta), g(chunks),
+        steps((args.kchunks + chunks - 1) / chunks) {
+    split = a.split && total < a.split * n && static_cast<int64_t>(total) * steps < (1 << 30);
     if (split) {
-      units = static_cast<int64_t>(total) * a.kchunks;
-      ctas = static_cast<int>(min(static_cast<int64_t>(n), max(units / kLeastUnits, int64_t{1})));
-      pos = units * cta / ctas;
-      end = cta < ctas ? units * (cta + 1) / ctas : 0;
+      const int units = total * steps;
+      ctas = min(n, max(units * g / kLeastChunks, 1));
+      share = units / ctas;
+      more = units - share * ctas;
+      const int first = cta * share + min(cta, more);
+      left = cta < ctas ? share + (cta < more ? 1 : 0) : 0;
+      t = first / steps;
+      at = first - t * steps;
     }
   }
-  static constexpr int kLeastUnits = 4;
-  __device__ __forceinline__ int cta_of(int64_t unit) const {
-    return static_cast<int>(((unit + 1) * ctas - 1) / units);
+  static constexpr int kLeastChunks = 4;
+  __device__ __forceinline__ int cta_of(int unit) const {
+    const int big = more * (share + 1);
+    return unit < big ? unit / (share + 1) : more + (unit - big) / share;
   }
   __device__ __forceinline__ bool next(Item& w) {
     w.k0 = 0;
     w.k1 = a.kchunks;
     w.parts = 1;
-    if (split) {
-      if (pos >= end) return false;
-      t = static_cast<int>(pos / a.kchunks);
-      const int64_t base = static_cast<int64_t>(t) * a.kchunks;
-      w.k0 = static_cast<int>(pos - base);
-      w.k1 = static_cast<int>(min(static_cast<int64_t>(a.kchunks), end - base));
-      if (w.k0 > 0 || w.k1 < a.kchunks) {
-        w.first = cta_of(base);
-        w.parts = cta_of(base + a.kchunks - 1) - w.first + 1;
+    if (split ? left == 0 : t >= total) return false;
+    if (t >= s.start[e + 1]) {  // the last segment that starts at t or before
+      int lo = e + 1, hi = *s.count - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t >= s.start[mid]) lo = mid;
+        else hi = mid - 1;
       }
-      pos += w.k1 - w.k0;
-    } else if (t >= total) {
-      return false;
+      e = lo;
     }
-    while (t >= s.start[e + 1]) ++e;
-    const int rows = s.rows[e], per = rows_per(rows, a.bn), nt = (rows + per - 1) / per;
-    const int at = t - s.start[e], j = at % nt;
-    w.e = e;
-    w.mt = at / nt;
-    w.row0 = s.row0[e] + j * per;
-    w.n = min(per, rows - j * per);
-    if (!split) t += step;
+    const int along = s.tiles[e], in = t - s.start[e];
+    w.e = s.id[e];
+    if (along == 1) {
+      w.mt = in;
+      w.row0 = s.row0[e];
+      w.n = s.rows[e];
+    } else {
+      const int rows = s.rows[e], per = rows_per(rows, a.bn);
+      w.mt = in / along;
+      const int j = in - w.mt * along;
+      w.row0 = s.row0[e] + j * per;
+      w.n = min(per, rows - j * per);
+    }
+    if (!split) {
+      t += step;
+      return true;
+    }
+    const int n = min(steps - at, left);
+    if (n < steps) {
+      w.k0 = at * g;
+      w.k1 = min(a.kchunks, (at + n) * g);
+      w.first = cta_of(t * steps);
+      w.parts = cta_of(t * steps + steps - 1) - w.first + 1;
+    }
+    left -= n;
+    at = 0;
+    ++t;
     return true;
   }
 };
@@ -415,33 +472,47 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release; barrier.cluster.wait.acquire;" ::: "memory");
 }
-// The epilogue's warps agree: true where all have seen true.
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+// The warps of a group agree: true where all have seen true.
+__device__ __forceinline__ bool epilogue_all(bool ok, int group) {
   uint32_t all;
   asm volatile(
-      "{ .reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
+      "{ .reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, %2, 128, p; selp.u32 %0, 1, 0, q; }"
       : "=r"(all)
-      : "r"(static_cast<uint32_t>(ok))
+      : "r"(static_cast<uint32_t>(ok)), "r"(1 + group)
       : "memory");
   return all != 0;
 }
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void epilogue_sync(int group) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+}
+template <class T>
+__device__ __forceinline__ T to(float x) {
+  if constexpr (sizeof(T) == 4) return x;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
 
-template <int CG, bool GATED>
+template <int CG, int G, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__ Maps maps, const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sffull[kSfRing], sfempty[kSfRing];
   __shared__ uint64_t acc_full[2], acc_empty[2], done;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int s_abort;
-  __shared__ int s_last;
+  __shared__ int s_last[2];
 
   uint8_t* smem = smem_raw + ((1024u - (saddr(smem_raw) & 1023u)) & 1023u);
-  const int stage_bytes = kTileM * kChunkK + a.bn / CG * kChunkK;
+  constexpr int kABytes = G * kTileM * kChunkK;  // (of shared memory: 8 bits an element)
+  const int b_bytes = a.bn / CG * kChunkK, stage_bytes = kABytes + G * b_bytes;
   uint8_t* sf_mem = smem + a.stages * stage_bytes;
   uint8_t* gate_mem = sf_mem + kSfRing * a.sf_block;
   int* seg_mem = reinterpret_cast<int*>(gate_mem + (GATED ? kGateBytes : 0));
-  const Segments seg{seg_mem, seg_mem + a.experts, seg_mem + 2 * a.experts};
+  const Segments seg{seg_mem + 1,
+                     seg_mem + 1 + a.experts,
+                     seg_mem + 1 + 2 * a.experts,
+                     seg_mem + 1 + 3 * a.experts,
+                     seg_mem + 1 + 4 * a.experts,
+                     seg_mem};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? blockIdx.x & 1 : 0, cta = blockIdx.x / CG, ctas = gridDim.x / CG;
   const int mtiles = (a.mtiles + CG - 1) / CG;
@@ -465,6 +536,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     mbar_fence_init();
   }
   if (warp == 1) Tc<CG>::alloc(&tmem_base);
+  if (warp == 2 && lane <= kBoxes)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &maps.b[lane - 1] : &maps.a)) : "memory");
+  // What the kernels before this one write is not read before here.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldg(a.offsets + e);
+  __syncthreads();
   if (warp == 0) read_segments(a, seg, mtiles, lane);
   fence_before();
   __syncthreads();
@@ -474,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   const uint32_t stage_at = saddr(smem), sf_at = saddr(sf_mem);
   const uint32_t full_at = saddr(full), empty_at = saddr(empty), sffull_at = saddr(sffull), sfempty_at = saddr(sfempty);
   const uint32_t acc_full_at = saddr(acc_full), acc_empty_at = saddr(acc_empty), full_lead = lead<CG>(full);
-  Walk walk(a, seg, cta, ctas, mtiles);
+  Walk walk(a, seg, cta, ctas, G);
   Item w;
 
   if (warp == 0) {
@@ -482,15 +559,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     // (the whole warp walks and waits, and one lane issues: operands then come from the
     // uniform registers that these instructions take)
     int it = 0, s = 0, phase = 1, sb = 0, sphase = 1;
-    bool ok = true;
+    bool ok = true, ready = true;
     while (ok && walk.next(w)) {
       const int mt = min(w.mt * CG + rank, a.mtiles - 1);  // (a pair's second tile may not exist)
       const int tile = (w.e * a.mtiles + mt) * a.kchunks;
-      for (int kc = w.k0; kc < w.k1; ++kc, ++it) {
-        ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort);  // (the first round passes)
+      for (int kc = w.k0; kc < w.k1; kc += G, ++it) {
+        ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort, ready);  // (the first round passes)
         if (!ok) break;
+        const int s1 = s + 1 == a.stages ? 0 : s + 1;
+        ready = peek<1>(empty_at + 8 * s1, s1 ? phase : phase ^ 1);
         if (elect_one()) {
-          if (rank == 0) expect_tx(full_at + 8 * s, CG * a.a_bytes);
+          if (rank == 0) expect_tx(full_at + 8 * s, CG * G * a.a_bytes);
           load_tile<CG>(stage_at + s * stage_bytes, &maps.a, 0, (tile + kc) * kTileM, full_lead + 8 * s);
         }
         __syncwarp();
@@ -520,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     // --------------------------------------------------- MMA issuer
     if (rank == 0) {
       int s = 0, phase = 0, item = 0, sb = 0, sphase = 0;
-      bool ok = true;
+      bool ok = true, ready = false, sf_ready = false;
       const uint32_t a_desc = static_cast<uint32_t>(sw128_desc(smem));  // (the high word is the same everywhere)
       const uint32_t desc_high = static_cast<uint32_t>(sw128_desc(smem) >> 32);
       auto desc = [&](uint32_t low) { return static_cast<uint64_t>(desc_high) << 32 | low; };
@@ -531,36 +610,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
         const uint32_t idesc = a.idesc | static_cast<uint32_t>(n16 >> 3) << 17;
         const uint32_t acc = tbase + buf * kMaxN;
         const bool wide = n16 > 128;
+        fence_after();
         bool add = false;
         for (int k4 = w.k0 & ~3; ok && k4 < w.k1; k4 += 4) {
-          ok = warp_wait<CG>(sffull_at + 8 * sb, sphase, &s_abort);
+          ok = warp_wait<CG>(sffull_at + 8 * sb, sphase, &s_abort, sf_ready);
+          // the rows' factors came by generic writes, and are read by the asynchronous proxy
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           const uint64_t sf = sf_desc(sf_at + sb * a.sf_block), sfr = sf_desc(sf_at + sb * a.sf_block + 4 * kSfBytes);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 4; c += G) {
             const int kc = k4 + c;
             if (!ok || kc < w.k0 || kc >= w.k1) continue;
-            ok = warp_wait<CG>(full_at + 8 * s, phase, &s_abort);
+            ok = warp_wait<CG>(full_at + 8 * s, phase, &s_abort, ready);
             if (!ok) continue;
-            // rows and scale factors came by generic writes, and are read by the asynchronous proxy
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            fence_after();
+            const int s1 = s + 1 == a.stages ? 0 : s + 1, sb1 = sb + 1 == kSfRing ? 0 : sb + 1;
+            const bool last = c + G == 4 || kc + G >= w.k1;  // of its block of scale factors
+            ready = peek<CG>(full_at + 8 * s1, s1 ? phase : phase ^ 1);
+            if (last) sf_ready = peek<CG>(sffull_at + 8 * sb1, sb1 ? sphase : sphase ^ 1);
             const uint32_t low = a_desc + s * (stage_bytes >> 4);
-            const uint32_t sfa = tbase + kSfCol + (c & 1) * 12, sfb = sfa + 4;
-            const int blocks = (a.k - kc * kChunkK) >> 5;
-            const uint32_t sfc = c * (a.sf_rows >> 4);
             if (elect_one()) {
-              Tc<CG>::sf_copy(sfa, sf + c * (kSfBytes >> 4));
-              Tc<CG>::sf_copy(sfb, sfr + sfc);
-              if (wide) Tc<CG>::sf_copy(sfb + 4, sfr + sfc + (512 >> 4));
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (j < blocks)
-                  Tc<CG>::mma(acc, desc(low + 2 * j), desc(low + (kTileM * kChunkK >> 4) + 2 * j),
-                              idesc | static_cast<uint32_t>(j) << 4 | static_cast<uint32_t>(j) << 29,
-                              sfa | static_cast<uint32_t>(j) << 30, sfb | static_cast<uint32_t>(j) << 30, add || j > 0);
+              for (int g = 0; g < G; ++g) {
+                const int blocks = (a.k - (kc + g) * kChunkK) >> 5;  // (none: a last step's second chunk)
+                const uint32_t sfa = tbase + kSfCol + ((c + g) & 1) * 12, sfb = sfa + 4;
+                const uint32_t al = low + g * (kTileM * kChunkK >> 4), bl = low + (kABytes >> 4) + g * (b_bytes >> 4);
+                const uint64_t rows_at = sfr + (c + g) * (a.sf_rows >> 4);
+                Tc<CG>::sf_copy(sfa, sf + (c + g) * (kSfBytes >> 4));
+                Tc<CG>::sf_copy(sfb, rows_at);
+                if (wide) Tc<CG>::sf_copy(sfb + 4, rows_at + (512 >> 4));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  if (j < blocks)
+                    Tc<CG>::mma(acc, desc(al + 2 * j), desc(bl + 2 * j),
+                                idesc | static_cast<uint32_t>(j) << 4 | static_cast<uint32_t>(j) << 29,
+                                sfa | static_cast<uint32_t>(j) << 30, sfb | static_cast<uint32_t>(j) << 30,
+                                add || g > 0 || j > 0);
+                }
               }
               commit<CG>(empty_at + 8 * s);
-              if (c == 3 || kc + 1 == w.k1) commit<CG>(sfempty_at + 8 * sb);
+              if (last) commit<CG>(sfempty_at + 8 * sb);
             }
             __syncwarp();
             add = true;
@@ -596,26 +684,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     // --------------------------------------------------- rows in order
     {
       int s = 0, phase = 1;
-      bool ok = true;
+      bool ok = true, ready = true;
       while (ok && walk.next(w)) {
         const int half = ((w.n + 15) & ~15) / CG;  // of this CTA
         const int box = half <= 32 ? 0 : half <= 64 ? 1 : half <= 128 ? 2 : half <= 192 ? 3 : 4;
         const int rows = min(box == 4 ? 256 : box == 3 ? 192 : 32 << box, a.bn / CG);
         const CUtensorMap* tm = &maps.b[box];
         const int row = w.row0 + rank * half;
-        for (int kc = w.k0; kc < w.k1; ++kc) {
-          ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort);
+        for (int kc = w.k0; kc < w.k1; kc += G) {
+          ok = warp_wait<1>(empty_at + 8 * s, phase, &s_abort, ready);
           if (!ok) break;
+          const int s1 = s + 1 == a.stages ? 0 : s + 1;
+          ready = peek<1>(empty_at + 8 * s1, s1 ? phase : phase ^ 1);
           if (elect_one()) {
-            if (rank == 0) expect_tx(full_at + 8 * s, CG * rows * kChunkK);
-            load_tile<CG>(stage_at + s * stage_bytes + kTileM * kChunkK, tm, kc * kChunkK, row, full_lead + 8 * s);
+            if (rank == 0) expect_tx(full_at + 8 * s, CG * G * rows * kChunkK);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              load_tile<CG>(stage_at + s * stage_bytes + kABytes + g * b_bytes, tm, (kc + g) * kChunkK, row,
+                            full_lead + 8 * s);
           }
           __syncwarp();
           if (++s == a.stages) s = 0, phase ^= 1;
         }
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 8 && warp < 12) {
     // ------------------------------------------- the rows' scale factors
     // (copies that arrive at the barrier by themselves: nothing here waits for memory)
     const int lt = threadIdx.x - 256, nsf = a.k >> 5;
@@ -654,17 +747,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= 4) {
     // ------------------------------------------------------ epilogue
-    const int q = warp & 3;  // the warp's lanes of tensor memory
-    const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
-    float* gate = reinterpret_cast<float*>(gate_mem);
-    int item = 0;
-    while (walk.next(w)) {
-      const int buf = item & 1;
-      bool ok = mbar_wait(&acc_full[buf], (item >> 1) & 1, &s_abort);
+    // Two groups of four warps take turns: each has an accumulator.
+    const int q = warp & 3, group = warp >> 3;  // the warp's lanes of tensor memory, and its group
+    const uint32_t acc = tbase + (static_cast<uint32_t>(32 * q) << 16) + group * kMaxN;
+    float* gate = reinterpret_cast<float*>(gate_mem) + group * (kGateTokens * kGatePitch);
+    for (int item = 0; walk.next(w); ++item) {
+      if ((item & 1) != group) continue;
+      bool ok = mbar_wait(&acc_full[group], (item >> 1) & 1, &s_abort);
       // (warps that gave up and warps that did not must not part at the barriers below)
-      if (!epilogue_all(ok && !s_abort)) break;
+      if (!epilogue_all(ok && !s_abort, group)) break;
       fence_after();
-      const uint32_t acc = tbase + lanes + buf * kMaxN;
       const int mt = w.mt * CG + rank;
       bool write = mt < a.mtiles;
       const float* parts = nullptr;
@@ -683,72 +775,75 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
             if (c0 + i < w.n) __stcg(mine + (c0 + i) * kTileM, __uint_as_float(v[i]));
         }
         __threadfence();
-        epilogue_sync();
-        if (threadIdx.x == 128) {
+        epilogue_sync(group);
+        if (q == 0 && lane == 0) {
           const int last = atomicAdd(a.counters + w.first, 1u) == static_cast<uint32_t>(w.parts - 1);
           if (last) a.counters[w.first] = 0;
           __threadfence();
-          s_last = last;
+          s_last[group] = last;
         }
-        epilogue_sync();
-        write = s_last;
+        epilogue_sync(group);
+        write = s_last[group];
         parts = a.partials + 32 * q + lane;
       }
-      auto part = [&](int p, int c) {
-        return __ldcg(parts + (2 * (w.first + p) + (p == 0)) * int64_t{kSplitN * kTileM} + c * kTileM);
+      // NC accumulators of this thread's row from column c0 on, or the sums of their parts,
+      // a part's reads all at once.
+      auto columns = [&](auto& v, int c0) {
+        constexpr int NC = sizeof(v) / 4;
+        if (CG == 1 && parts) {
+          const float* at = parts + c0 * kTileM + (2 * w.first + 1) * int64_t{kSplitN * kTileM};
+          for (int p = 0; p < w.parts; ++p) {  // (the first CTA's second place, the others' first)
+            float x[NC];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) x[i] = c0 + i < w.n ? __ldcg(at + i * kTileM) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+              v[i] = p ? __float_as_uint(fadd(__uint_as_float(v[i]), x[i])) : __float_as_uint(x[i]);
+            at += (p ? 2 : 1) * int64_t{kSplitN * kTileM};
+          }
+        } else {
+          if constexpr (NC == 16) tmem_ld16(acc + c0, v);
+          else tmem_ld32(acc + c0, v);  // (past the tile's columns: whatever is there, not stored)
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < NC; ++i) asm volatile("" : "+r"(v[i]));
+        }
       };
       if (!write) {
       } else if constexpr (!GATED) {
         const int m = mt * kTileM + 32 * q + lane;
-        uint8_t* out = a.out + w.row0 * a.out_stride + static_cast<int64_t>(m) * size_of(a.out_type);
-        for (int c0 = 0; c0 < w.n; c0 += 16) {
-          uint32_t v[16];
-          if (CG == 1 && parts) {
+        const bool on = m < a.features;
+        auto rows_out = [&](auto type) {
+          using T = decltype(type);
+          uint8_t* out = a.out + w.row0 * a.out_stride + static_cast<int64_t>(m) * sizeof(T);
+          for (int c0 = 0; c0 < w.n; c0 += 16) {
+            uint32_t v[16];
+            columns(v, c0);
+            const int n = on ? w.n - c0 : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              float sum = 0.0f;
-              if (c0 + i < w.n)
-                for (int p = 0; p < w.parts; ++p) sum = fadd(sum, part(p, c0 + i));
-              v[i] = __float_as_uint(sum);
+              if (i < n) *reinterpret_cast<T*>(out) = to<T>(__uint_as_float(v[i]));
+              out += a.out_stride;
             }
-          } else {
-            tmem_ld16(acc + c0, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));
           }
-          if (m < a.features) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c0 + i < w.n) store1_of(out + (c0 + i) * a.out_stride, __uint_as_float(v[i]), a.out_type);
-          }
-        }
+        };
+        if (a.out_type == LP_F32) rows_out(float{});
+        else if (a.out_type == LP_F16) rows_out(__half{});
+        else rows_out(__nv_bfloat16{});
       } else {
         for (int c0 = 0; c0 < w.n; c0 += kGateTokens) {
           uint32_t v[32];
-          if (CG == 1 && parts) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float sum = 0.0f;
-              if (c0 + i < w.n)
-                for (int p = 0; p < w.parts; ++p) sum = fadd(sum, part(p, c0 + i));
-              v[i] = __float_as_uint(sum);
-            }
-          } else {
-            tmem_ld32(acc + c0, v);  // (past the tile's columns: whatever is there, not stored)
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));
-          }
+          columns(v, c0);
           const bool up = lane & 16;  // this lane holds an up row; its partner the gate's
           const int f = 16 * q + (lane & 15);
+          float* to = gate + (up ? 16 * kGatePitch : 0) + f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint32_t other = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[16 + i], 16);
             const float g = __uint_as_float(up ? other : v[i]), u = __uint_as_float(up ? v[16 + i] : other);
-            gate[(i + (up ? 16 : 0)) * kGatePitch + f] = silu_mul(g, u);
+            to[i * kGatePitch] = silu_mul(g, u);
           }
-          epilogue_sync();
+          epilogue_sync(group);
           // 16 features of a token each; two lanes hold a block of 32
           const int t = 8 * q + (lane >> 2), f0 = 16 * (lane & 3), feature = mt * 64 + f0;
           float x[16], top = 0.0f;
@@ -766,13 +861,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
                 make_uint4(e4m3x4(x, inv), e4m3x4(x + 4, inv), e4m3x4(x + 8, inv), e4m3x4(x + 12, inv));
             if (!(lane & 1)) a.out_scales[row * a.out_scale_stride + (feature >> 5)] = static_cast<uint8_t>(code);
           }
-          epilogue_sync();
+          epilogue_sync(group);
         }
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) arrive_lead<CG>(&acc_empty[buf]);
-      ++item;
+      if (lane == 0) arrive_lead<CG>(&acc_empty[group]);
     }
   }
   fence_before();
@@ -785,12 +879,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   }
 }
 
-bool encode_tiles(CUtensorMap* tm, const void* base, int64_t tiles, bool fp4) {
+bool encode_tiles(CUtensorMap* tm, const void* base, int64_t tiles, int chunks, bool fp4) {
   EncodeFn fn = encoder();
   if (!fn) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kChunkK), static_cast<cuuint64_t>(tiles * kTileM)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(fp4 ? kChunkK / 2 : kChunkK)};
-  const cuuint32_t box[2] = {kChunkK, kTileM}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {kChunkK, static_cast<cuuint32_t>(chunks * kTileM)}, one[2] = {1, 1};
   return fn(tm, fp4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -807,22 +901,24 @@ bool encode_rows(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int CG, bool GATED>
+template <int CG, int G, bool GATED>
 int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   const DeviceInfo& di = device_info();
-  auto kern = k_experts<CG, GATED>;
+  auto kern = k_experts<CG, G, GATED>;
   static int ctas[kMaxDevices];  // of a full grid, 0 before the first launch
   const int slot = di.ordinal % kMaxDevices;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = CG;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t c{};
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = smem;
   c.stream = st;
-  c.attrs = &attr;
-  c.numAttrs = CG == 2 ? 1 : 0;
+  c.attrs = attr;
+  c.numAttrs = CG;
   if (!ctas[slot]) {
     const int most = di.max_smem_optin - 1024;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
@@ -842,6 +938,12 @@ int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   c.gridDim = dim3(ctas[slot]);
   return cuda_status(cudaLaunchKernelEx(&c, kern, maps, a));
 }
+template <int CG>
+int launch_g(int g, bool gated, const Maps& maps, const Args& a, int smem, cudaStream_t st) {
+  if (g == 2) return gated ? launch<CG, 2, true>(maps, a, smem, st) : launch<CG, 2, false>(maps, a, smem, st);
+  return gated ? launch<CG, 1, true>(maps, a, smem, st) : launch<CG, 1, false>(maps, a, smem, st);
+}
+
 }  // namespace
 
 int launch_pack_experts(const void* codes, const void* scales, int scale_type, const lp_expert_weights& w,
@@ -913,17 +1015,18 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   else if (mean <= 48) bn = 64;
   else if (mean <= 112) bn = 128;
   int cg = mean > 112 ? 2 : 1;
+  int g = cg == 2 ? 1 : 2;
   a.bn = static_cast<int>(std::min<int64_t>(bn, (most + 15) / 16 * 16));
-  a.split = a.bn <= kSplitN && cg == 1 ? 8 : 0;
+  a.split = a.bn <= kSplitN && cg == 1 ? 32 : 0;
   a.sf_rows = a.bn > 128 ? 1024 : 512;
   a.sf_block = 4 * (kSfBytes + a.sf_rows);
   const int fixed = 1024 + kSfRing * a.sf_block + (w.gated ? kGateBytes : 0)+
-                    static_cast<int>(3 * w.experts + 1) * 4;
-  const int stage = (kTileM + a.bn / cg) * kChunkK;
+                    static_cast<int>(5 * w.experts + 2) * 4;
+  const int stage = g * (kTileM + a.bn / cg) * kChunkK;
   a.stages = std::min(kMaxStages, (device_info().max_smem_optin - 1024 - fixed) / stage);
   if (a.stages < 2) return LP_ERR_UNSUPPORTED;
   Maps maps;
-  if (!encode_tiles(&maps.a, w.tiles, l.tiles, w.dtype == LP_E2M1)) return LP_ERR_UNSUPPORTED;
+  if (!encode_tiles(&maps.a, w.tiles, l.tiles, g, w.dtype == LP_E2M1)) return LP_ERR_UNSUPPORTED;
   const int boxes[kBoxes] = {32, 64, 128, 192, 256};
   for (int b = 0; b < kBoxes; ++b)
     if (!encode_rows(&maps.b[b], x.codes, x.cols, x.rows, x.code_stride, std::min(boxes[b], a.bn / cg)))
@@ -931,8 +1034,7 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   const int smem = fixed + a.stages * stage;
   // M = 128 of a CTA, or 256 of a pair
   a.idesc |= static_cast<uint32_t>(cg * 128 >> 4) << 24;
-  if (w.gated) return cg == 2 ? launch<2, true>(maps, a, smem, st) : launch<1, true>(maps, a, smem, st);
-  return cg == 2 ? launch<2, false>(maps, a, smem, st) : launch<1, false>(maps, a, smem, st);
+  return cg == 2 ? launch_g<2>(g, w.gated, maps, a, smem, st) : launch_g<1>(g, w.gated, maps, a, smem, st);
 }
 
 unsigned int take_error_experts() {
