@@ -114,24 +114,31 @@ struct GatherArgs {
   int cols;
 };
 __global__ void __launch_bounds__(256) k_gather(const GatherArgs a) {
-  const int cp = a.cols / 16, sp = static_cast<int>(a.to_scale_stride / 16), per = cp + sp;
-  const int64_t rows = min(a.rows, static_cast<int64_t>(max(__ldg(a.end), 0))), n = rows * per;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t row = n >> 32 ? i / per : static_cast<uint32_t>(i) / static_cast<uint32_t>(per);
-    const int p = static_cast<int>(i - row * per), token = __ldg(a.row_token + row);
+  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, cp = a.cols / 16, nsf = a.cols / 32;
+  const int64_t rows = min(a.rows, static_cast<int64_t>(max(__ldg(a.end), 0)));
+  // a warp a row, 16 bytes a lane, four at a time
+  for (int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
+    const int token = __ldg(a.row_token + row);
     const bool in = static_cast<uint32_t>(token) < static_cast<uint32_t>(a.tokens);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (p < cp) {
-      if (in) v = __ldg(reinterpret_cast<const uint4*>(a.codes + token * a.code_stride) + p);
-      reinterpret_cast<uint4*>(a.to + row * a.cols)[p] = v;
-    } else {
-      uint32_t w[4] = {0, 0, 0, 0};
-      const uint8_t* from = a.scales + token * a.scale_stride;
-      for (int b = 0; b < 16; ++b) {
-        const int at = 16 * (p - cp) + b;
-        if (in && at < a.cols / 32) w[b >> 2] |= static_cast<uint32_t>(__ldg(from + at)) << (8 * (b & 3));
-      }
-      reinterpret_cast<uint4*>(a.to_scales + row * a.to_scale_stride)[p - cp] = make_uint4(w[0], w[1], w[2], w[3]);
+    const uint4* from = reinterpret_cast<const uint4*>(a.codes + (in ? token : 0) * a.code_stride);
+    const uint8_t* sf = a.scales + (in ? token : 0) * a.scale_stride;
+    uint4* to = reinterpret_cast<uint4*>(a.to + row * a.cols);
+    for (int p0 = lane; p0 < cp; p0 += 128) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = in && p0 + 32 * i < cp ? __ldg(from + p0 + 32 * i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p0 + 32 * i < cp) to[p0 + 32 * i] = v[i];
+    }
+    for (int w = lane; w < a.to_scale_stride / 4; w += 32) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (in && 4 * w + b < nsf) word |= static_cast<uint32_t>(__ldg(sf + 4 * w + b)) << (8 * b);
+      reinterpret_cast<uint32_t*>(a.to_scales + row * a.to_scale_stride)[w] = word;
     }
   }
 }
@@ -539,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   if (warp == 2 && lane <= kBoxes)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &maps.b[lane - 1] : &maps.a)) : "memory");
   // What the kernels before this one write is not read before here.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
   for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldg(a.offsets + e);
   __syncthreads();
   if (warp == 0) read_segments(a, seg, mtiles, lane);
@@ -970,10 +977,8 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
                        static_cast<uint8_t*>(x.codes), static_cast<uint8_t*>(x.scales), given.code_stride,
                        given.scale_stride, x.scale_stride, offsets + w.experts, row_token, rows, given.rows,
                        static_cast<int>(given.cols)};
-    const int64_t pieces = rows * (given.cols / 16 + x.scale_stride / 16);
-    const int grid = static_cast<int>(std::min<int64_t>((pieces + 255) / 256, device_info().sm_count * 16ll));
-    k_gather<<<grid, 256, 0, st>>>(g);
-    if (const int e = cuda_status(cudaGetLastError())) return e;
+    const int grid = static_cast<int>(std::min<int64_t>((rows + 7) / 8, device_info().sm_count * 16ll));
+    if (const int e = launch_early(k_gather, grid, 256, st, g)) return e;
   }
   const Layout l = layout(w.experts, w.rows, w.cols, w.dtype, w.gated);
   Args a{};

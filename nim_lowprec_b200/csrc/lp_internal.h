@@ -151,7 +151,7 @@ int launch_attn_chunk(const attn::Args& a, int cache_type, int dim, cudaStream_t
 
 // 8-bit rows (rows8.cu), the router (route.cu) and the experts' products (experts.cu)
 constexpr int kRouteExperts = 1024;  // most experts
-constexpr int kRouteCtas = 128;      // most CTAs that count
+constexpr int kRouteCtas = 128;      // most CTAs that count: four to a lane
 int launch_norm(const lp_matrix& x, const lp_matrix* residual, const void* weight, int weight_type, float eps,
                 const lp_matrix* total, const lp_matrix* y, const lp_rows8* q, bool vec, cudaStream_t st);
 int launch_quantize_rows(const lp_matrix& x, const lp_rows8& q, bool vec, cudaStream_t st);
@@ -185,6 +185,22 @@ inline int cuda_status(cudaError_t e) {
   if (e == cudaSuccess) return LP_OK;
   note_cuda_error(e);
   return LP_ERR_CUDA;
+}
+
+// A launch that may begin while the kernel before it in the stream ends (programmatic
+// stream serialization): the kernel waits (griddepcontrol.wait) before it touches memory.
+template <class Args>
+inline int launch_early(void (*kernel)(Args), int grid, int threads, cudaStream_t st, const Args& args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(static_cast<unsigned>(grid));
+  c.blockDim = dim3(static_cast<unsigned>(threads));
+  c.stream = st;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&c, kernel, args));
 }
 
 }  // namespace lp

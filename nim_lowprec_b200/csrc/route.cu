@@ -20,7 +20,6 @@ namespace lp {
 namespace {
 
 constexpr int kMaxPer = kRouteExperts / 32;  // logits a lane holds
-constexpr int kPairs = 2048;                 // (token, choice) pairs placed at a time
 constexpr int kThreads = 512;
 constexpr int kOneCta = 64;                  // tokens that one CTA takes
 
@@ -30,7 +29,7 @@ struct RouteArgs {
   int type;
   float* weights;
   int32_t *experts, *offsets, *row_token, *places;
-  int32_t* counts;  // [CTAs][experts]
+  int32_t* counts;  // [experts][kRouteCtas]
   int64_t tokens, per;  // of a CTA
   int n, k, renorm;
 };
@@ -102,27 +101,41 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t t, int lane) {
   return id;
 }
 
-// Rows of each expert before this CTA's (base) and the offsets, from the counts.
-// An inclusive scan over the experts by all threads; n <= 2 * kThreads.
+// Rows of each expert before this CTA's (base) and the offsets, from the counts: a warp
+// reads an expert's counts of all CTAs at once, then a scan over the experts.
 __device__ __forceinline__ void scan_counts(const RouteArgs& a, int ctas, int32_t* base, int32_t* sums) {
   __shared__ int32_t wsum[kThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int carry = 0;
-  for (int e0 = 0; e0 < a.n; e0 += kThreads) {
-    const int e = e0 + threadIdx.x;
-    int before = 0, total = 0;
-    if (e < a.n) {
-      for (int c0 = 0; c0 < ctas; c0 += 8) {
-        int v[8];
+  static_assert(kRouteCtas == 128, "");
+  for (int e0 = warp; e0 < a.n; e0 += 4 * (kThreads / 32)) {
+    int4 c[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c0 + i < ctas ? __ldcg(a.counts + int64_t{c0 + i} * a.n + e) : 0;
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + i * (kThreads / 32);
+      c[i] = e < a.n && 4 * lane < ctas ? __ldcg(reinterpret_cast<const int4*>(a.counts + int64_t{e} * kRouteCtas) + lane)
+                                        : make_int4(0, 0, 0, 0);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (c0 + i < static_cast<int>(blockIdx.x)) before += v[i];
-          total += v[i];
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + i * (kThreads / 32), v[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+      int before = 0, total = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (4 * lane + j < static_cast<int>(blockIdx.x)) before += v[j];
+        if (4 * lane + j < ctas) total += v[j];
+      }
+      before = __reduce_add_sync(0xffffffffu, before);
+      total = __reduce_add_sync(0xffffffffu, total);
+      if (lane == 0 && e < a.n) {
+        base[e] = before;
+        sums[e] = total;
       }
     }
+  }
+  __syncthreads();
+  int carry = 0;
+  for (int e0 = 0; e0 < a.n; e0 += kThreads) {
+    const int e = e0 + threadIdx.x, total = e < a.n ? sums[e] : 0;
     int inc = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -136,49 +149,48 @@ __device__ __forceinline__ void scan_counts(const RouteArgs& a, int ctas, int32_
       if (w < warp) ahead += wsum[w];
       carry += wsum[w];
     }
-    inc += ahead;
     if (e < a.n) {
-      base[e] = inc - total + before;
-      sums[e] = inc;
+      base[e] += ahead + inc - total;
+      if (blockIdx.x == 0) a.offsets[e + 1] = ahead + inc;
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) a.offsets[0] = 0;
-    for (int e = threadIdx.x; e < a.n; e += kThreads) a.offsets[e + 1] = sums[e];
-  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[0] = 0;
 }
 
-// The rows of tokens [t0, t1) in order: a thread per expert walks the pairs.
-__device__ __forceinline__ void place(const RouteArgs& a, int64_t t0, int64_t t1, int32_t* base, int16_t* ids,
-                                      int32_t* at) {
-  const int step = kPairs / a.k;  // tokens at a time
-  for (int64_t s = t0; s < t1; s += step) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(step), t1 - s)) * a.k;
+// The rows of tokens [t0, t1) in order, a pair a thread: its place is the expert's base,
+// plus the pairs of that expert in warps before, plus those in lanes before.
+__device__ __forceinline__ void place(const RouteArgs& a, int64_t t0, int64_t t1, int32_t* base, int32_t* sums,
+                                      uint16_t* ahead) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t end = t1 * a.k;
+  for (int64_t p0 = t0 * a.k; p0 < end; p0 += kThreads) {
+    for (int i = threadIdx.x; i < (kThreads / 32) * a.n; i += kThreads) ahead[i] = 0;
+    const int64_t p = p0 + threadIdx.x;
+    const int id = p < end ? a.experts[p] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    const int rank = __popc(same & ((1u << lane) - 1));
     __syncthreads();
-    for (int i = threadIdx.x; i < (n + 7) / 8 * 8; i += kThreads) {
-      const int id = i < n ? a.experts[s * a.k + i] : -1;
-      ids[i] = static_cast<int16_t>(id);
-      if (i < n && id < 0) at[i] = -1;
-    }
+    if (id >= 0 && rank == 0) ahead[warp * a.n + id] = static_cast<uint16_t>(__popc(same));
     __syncthreads();
     for (int e = threadIdx.x; e < a.n; e += kThreads) {
-      int next = base[e];
-      for (int i = 0; i < n; i += 8) {  // eight pairs a read
-        const uint4 q = *reinterpret_cast<const uint4*>(ids + i);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      int run = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (static_cast<int>(w[j >> 1] >> (16 * (j & 1)) & 0xffffu) == e) at[i + j] = next++;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        const int c = ahead[w * a.n + e];
+        ahead[w * a.n + e] = static_cast<uint16_t>(run);
+        run += c;
       }
-      base[e] = next;
+      sums[e] = run;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int p = at[i];
-      a.places[s * a.k + i] = p;
-      if (p >= 0) a.row_token[p] = static_cast<int32_t>(s + i / a.k);
+    if (p < end) {
+      const int at = id >= 0 ? base[id] + ahead[warp * a.n + id] + rank : -1;
+      a.places[p] = at;
+      if (id >= 0) a.row_token[at] = static_cast<int32_t>(p / a.k);
     }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.n; e += kThreads) base[e] += sums[e];
   }
 }
 
@@ -186,43 +198,40 @@ template <int PER, bool ONE>
 __global__ void __launch_bounds__(kThreads) k_route_choose(const RouteArgs a) {
   __shared__ int32_t hist[kRouteExperts];
   __shared__ int32_t sums[ONE ? kRouteExperts : 1];
-  __shared__ __align__(16) int16_t ids[ONE ? kPairs : 8];
-  __shared__ int32_t at[ONE ? kPairs : 1];
+  __shared__ uint16_t ahead[ONE ? kThreads / 32 * kRouteExperts : 1];
   for (int e = threadIdx.x; e < a.n; e += kThreads) hist[e] = 0;
   __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tokens);
   const int lane = threadIdx.x & 31;
   for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += kThreads / 32) {
     const int id = choose<PER>(a, t, lane);
     if (id >= 0) atomicAdd(&hist[id], 1);  // (a count: its order does not matter)
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
-  for (int e = threadIdx.x; e < a.n; e += kThreads) a.counts[int64_t{blockIdx.x} * a.n + e] = hist[e];
+  for (int e = threadIdx.x; e < a.n; e += kThreads) a.counts[int64_t{e} * kRouteCtas + blockIdx.x] = hist[e];
   if constexpr (ONE) {
     __syncthreads();
     scan_counts(a, 1, hist, sums);
-    place(a, t0, t1, hist, ids, at);
+    place(a, t0, t1, hist, sums, ahead);
   }
 }
 
 __global__ void __launch_bounds__(kThreads) k_route_place(const RouteArgs a) {
   __shared__ int32_t base[kRouteExperts], sums[kRouteExperts];
-  __shared__ __align__(16) int16_t ids[kPairs];
-  __shared__ int32_t at[kPairs];
+  __shared__ uint16_t ahead[kThreads / 32 * kRouteExperts];
+  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
   scan_counts(a, gridDim.x, base, sums);
   const int64_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tokens);
-  place(a, t0, t1, base, ids, at);
+  place(a, t0, t1, base, sums, ahead);
 }
 
 template <int PER>
 int launch_route_per(const RouteArgs& a, int ctas, cudaStream_t st) {
-  if (ctas <= 1) {
-    k_route_choose<PER, true><<<1, kThreads, 0, st>>>(a);
-  } else {
-    k_route_choose<PER, false><<<ctas, kThreads, 0, st>>>(a);
-    k_route_place<<<ctas, kThreads, 0, st>>>(a);
-  }
-  return cuda_status(cudaGetLastError());
+  if (ctas <= 1) return launch_early(k_route_choose<PER, true>, 1, kThreads, st, a);
+  if (const int e = launch_early(k_route_choose<PER, false>, ctas, kThreads, st, a)) return e;
+  return launch_early(k_route_place, ctas, kThreads, st, a);
 }
 
 }  // namespace

@@ -148,6 +148,26 @@ __device__ __forceinline__ void load8_of(float* x, const uint8_t* p, int type, i
     }
   }
 }
+// Eight elements of type T as they lie in memory, 16-byte aligned: loads that are issued
+// together, before the first is converted.  Plain loads, as above.
+template <int T>
+struct Raw8 {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    a = *reinterpret_cast<const uint4*>(p);
+    if constexpr (T == LP_F32) b = reinterpret_cast<const uint4*>(p)[1];
+  }
+  __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float* x) const {
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (T == LP_F32) x[i] = __uint_as_float(w[i]);
+      else if constexpr (T == LP_F16) x[i] = h2f(w[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+      else x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+  }
+};
 __device__ __forceinline__ void store1_of(uint8_t* p, float x, int type) {
   if (type == LP_F32) *reinterpret_cast<float*>(p) = x;
   else if (type == LP_F16) *reinterpret_cast<__half*>(p) = __float2half_rn(x);
