@@ -65,15 +65,19 @@ class Decoder:
     def forward(self, x, caches, step, window=0, sinks=0):
         """x [tokens, width]: the new tokens' hidden states, request after request."""
         t, h, g = x.shape[0], self.heads, self.kvHeads
-        for (proj, outp), cache in zip(self.layers, caches):
+        for i, ((proj, outp), cache) in enumerate(zip(self.layers, caches)):
             norm = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
             rows = proj(norm).view(t, h + 2 * g, self.dim)
             L.storeKV(cache, rows[:, h:h + g], rows[:, h + g:], step.slots)
             out = torch.empty(t, h, self.dim, device="cuda")
             L.pagedAttention(cache, step.tables, step.qStart, step.seqLens, rows[:, :h], out,
                              window=window, sinks=sinks)
-            x = x + outp(out.view(t, self.width))
+            x = self.after(i, x, outp(out.view(t, self.width)))
         return x
+
+    def after(self, layer, x, delta):
+        """What follows a layer's attention, which adds delta to the stream."""
+        return x + delta
 
 
 class Step:
@@ -109,12 +113,13 @@ class Batch:
         return self.step
 
 
-def run(cache="int8", steps=16, lens=(37, 5, 120), window=0, sinks=0, seed=0, one_chunk=False):
+def run(cache="int8", steps=16, lens=(37, 5, 120), window=0, sinks=0, seed=0, one_chunk=False,
+        model=None):
     """Hidden states of the prompts and the decoded tokens, [requests][tokens, width].  The next
     token's hidden state is the last one's, normed.  one_chunk: all tokens again as one chunk
     (the decoded ones given), which must give the same states."""
     dtype = {"int8": torch.int8, "fp16": torch.float16, "bf16": torch.bfloat16}[cache]
-    model, page = Decoder(seed=seed), 16
+    model, page = model or Decoder(seed=seed), 16
     gen = torch.Generator(device="cuda")
     gen.manual_seed(seed + 1)
     prompts = [torch.randn(n, model.width, generator=gen, device="cuda") for n in lens]
