@@ -21,12 +21,21 @@
 // stage is one contiguous read of 8 (16) KB and one of 512 bytes, and odd sizes of
 // M and K end in tiles of zeros instead of in the kernel.
 //
-// One persistent CTA per SM, 8 warps:
-//   warp 0     producer: per stage the tile's codes and scales, and the rows' codes
-//              by tile (rows in order) or by gather of four rows (row_token)
-//   warp 1     copies scale factors to tensor memory and issues the MMAs
-//   warps 2-3  the rows' scale factors, gathered, into atoms
-//   warps 4-7  epilogue, while the next tile's MMAs fill the other accumulator
+// One persistent CTA per SM (or pair of CTAs, whose MMAs take 256 weight rows and the
+// rows' halves from both), 16 warps:
+//   warp 0       the weights' tiles and, a block of four chunks at a time, their scales
+//   warp 1       copies scale factors to tensor memory and issues the MMAs (of a pair, in the
+//                leading CTA; in the other it passes on that scale factors are there)
+//   warp 2       the rows, a box of up to 240 of them
+//   warps 8-11   the rows' scale factors, word by word into atoms (cp.async)
+//   warps 4-7, 12-15  epilogue, taking turns with the two accumulators
+// Rows named by row_token are gathered by a kernel of their own first.
+//
+// What bounds it (B200).  Few rows: the weights' bytes, 57 tokens over 8 experts of 28672 x
+// 4096 in e2m1 105 us (4.7 TB/s, 5.5 between start and join); the smallest calls the chain of
+// offsets, first loads and joins (one token over 8 of 64 experts, 23 MB: 12 us, of which 5
+// stream).  Many rows: the products, 64 experts x 1024 rows gated 1.9 to 2.0 PFLOP/s back to
+// back; a step of two chunks takes about 1000 cycles where its MMAs take 800 to 960.
 // Every wait is bounded, and tensor memory is freed on every path.
 #include <cuda.h>
 
@@ -104,7 +113,7 @@ __global__ void __launch_bounds__(256) k_pack_scales(const PackArgs a) {
 // Rows into the experts' order, scales padded with zeros to whole 16 bytes.  (The
 // products' own loaders gathering row by row was slower: a gather of four rows costs
 // TMA as much as a tile of 128, and copies of 16 bytes by threads made a prompt's
-// gated product 690 us where this and tiles take 420.)
+// gated product 690 us where this and tiles take 390.)
 struct GatherArgs {
   const uint8_t *codes, *scales;
   uint8_t *to, *to_scales;
@@ -114,7 +123,9 @@ struct GatherArgs {
   int cols;
 };
 __global__ void __launch_bounds__(256) k_gather(const GatherArgs a) {
-  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
+  // The product after this one begins once every CTA here has passed the wait: whatever came
+  // before the gather is there then, and the product waits for the gathered rows alone.
+  asm volatile("griddepcontrol.wait; griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, cp = a.cols / 16, nsf = a.cols / 32;
   const int64_t rows = min(a.rows, static_cast<int64_t>(max(__ldg(a.end), 0)));
   // a warp a row, 16 bytes a lane, four at a time
@@ -146,6 +157,12 @@ __global__ void __launch_bounds__(256) k_gather(const GatherArgs a) {
 // -------------------------------------------------------------- product
 constexpr int kThreads = 512;
 constexpr int kMaxN = 240;
+// Chunks of K to a stage.  A step through the pipeline has fixed costs beside its products
+// (a wait, an issue by one lane: about 300 cycles, where a chunk of 16 rows takes 180 and one
+// of 240 rows 480), so two chunks share one: 57 tokens over 8 experts 141 -> 107 us.
+constexpr int G = 2;
+constexpr int kPairRows = 200;   // mean rows per expert above which two CTAs share a tile
+constexpr int kSplitTiles = 32;  // tiles per CTA below which they are cut along K
 constexpr int kMaxStages = 12;
 constexpr int kSfRing = 3;  // blocks of four chunks' scale factors
 constexpr uint32_t kTmemCols = 512, kSfCol = 480;  // accumulators at 0 and 240
@@ -402,16 +419,16 @@ struct Item {
 struct Walk {
   const Args& a;
   const Segments& s;
-  int ctas, step, total, t, e = 0, g, steps;  // steps: of g chunks, of a tile
+  int ctas, step, total, t, e = 0, steps;  // steps: of a tile
   int at = 0, left = 0, share = 0, more = 0;  // steps: into the tile, of this CTA; `more` CTAs have one more than the share
   bool split;
-  __device__ Walk(const Args& args, const Segments& seg, int cta, int n, int chunks)
-      : a(args), s(seg), ctas(n), step(n), total(seg.start[*seg.count]), t(cta), g(chunks),
-        steps((args.kchunks + chunks - 1) / chunks) {
+  __device__ Walk(const Args& args, const Segments& seg, int cta, int n)
+      : a(args), s(seg), ctas(n), step(n), total(seg.start[*seg.count]), t(cta),
+        steps((args.kchunks + G - 1) / G) {
     split = a.split && total < a.split * n && static_cast<int64_t>(total) * steps < (1 << 30);
     if (split) {
       const int units = total * steps;
-      ctas = min(n, max(units * g / kLeastChunks, 1));
+      ctas = min(n, max(units * G / kLeastChunks, 1));
       share = units / ctas;
       more = units - share * ctas;
       const int first = cta * share + min(cta, more);
@@ -458,8 +475,8 @@ struct Walk {
     }
     const int n = min(steps - at, left);
     if (n < steps) {
-      w.k0 = at * g;
-      w.k1 = min(a.kchunks, (at + n) * g);
+      w.k0 = at * G;
+      w.k1 = min(a.kchunks, (at + n) * G);
       w.first = cta_of(t * steps);
       w.parts = cta_of(t * steps + steps - 1) - w.first + 1;
     }
@@ -499,7 +516,7 @@ __device__ __forceinline__ T to(float x) {
   else return __float2bfloat16_rn(x);
 }
 
-template <int CG, int G, bool GATED>
+template <int CG, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__ Maps maps, const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], sffull[kSfRing], sfempty[kSfRing];
@@ -546,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   if (warp == 2 && lane <= kBoxes)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &maps.b[lane - 1] : &maps.a)) : "memory");
   // What the kernels before this one write is not read before here.
-  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!a.gathered) asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldg(a.offsets + e);
   __syncthreads();
   if (warp == 0) read_segments(a, seg, mtiles, lane);
@@ -558,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   const uint32_t stage_at = saddr(smem), sf_at = saddr(sf_mem);
   const uint32_t full_at = saddr(full), empty_at = saddr(empty), sffull_at = saddr(sffull), sfempty_at = saddr(sfempty);
   const uint32_t acc_full_at = saddr(acc_full), acc_empty_at = saddr(acc_empty), full_lead = lead<CG>(full);
-  Walk walk(a, seg, cta, ctas, G);
+  Walk walk(a, seg, cta, ctas);
   Item w;
 
   if (warp == 0) {
@@ -690,6 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   } else if (warp == 2) {
     // --------------------------------------------------- rows in order
     {
+      if (a.gathered) asm volatile("griddepcontrol.wait;" ::: "memory");
       int s = 0, phase = 1;
       bool ok = true, ready = true;
       while (ok && walk.next(w)) {
@@ -718,6 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   } else if (warp >= 8 && warp < 12) {
     // ------------------------------------------- the rows' scale factors
     // (copies that arrive at the barrier by themselves: nothing here waits for memory)
+    if (a.gathered) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lt = threadIdx.x - 256, nsf = a.k >> 5;
     int sb = 0, sphase = 1;
     bool ok = true;
@@ -886,12 +906,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   }
 }
 
-bool encode_tiles(CUtensorMap* tm, const void* base, int64_t tiles, int chunks, bool fp4) {
+bool encode_tiles(CUtensorMap* tm, const void* base, int64_t tiles, bool fp4) {
   EncodeFn fn = encoder();
   if (!fn) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kChunkK), static_cast<cuuint64_t>(tiles * kTileM)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(fp4 ? kChunkK / 2 : kChunkK)};
-  const cuuint32_t box[2] = {kChunkK, static_cast<cuuint32_t>(chunks * kTileM)}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {kChunkK, G * kTileM}, one[2] = {1, 1};
   return fn(tm, fp4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -908,10 +928,10 @@ bool encode_rows(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int CG, int G, bool GATED>
+template <int CG, bool GATED>
 int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   const DeviceInfo& di = device_info();
-  auto kern = k_experts<CG, G, GATED>;
+  auto kern = k_experts<CG, GATED>;
   static int ctas[kMaxDevices];  // of a full grid, 0 before the first launch
   const int slot = di.ordinal % kMaxDevices;
   cudaLaunchAttribute attr[2];
@@ -945,12 +965,6 @@ int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   c.gridDim = dim3(ctas[slot]);
   return cuda_status(cudaLaunchKernelEx(&c, kern, maps, a));
 }
-template <int CG>
-int launch_g(int g, bool gated, const Maps& maps, const Args& a, int smem, cudaStream_t st) {
-  if (g == 2) return gated ? launch<CG, 2, true>(maps, a, smem, st) : launch<CG, 2, false>(maps, a, smem, st);
-  return gated ? launch<CG, 1, true>(maps, a, smem, st) : launch<CG, 1, false>(maps, a, smem, st);
-}
-
 }  // namespace
 
 int launch_pack_experts(const void* codes, const void* scales, int scale_type, const lp_expert_weights& w,
@@ -989,6 +1003,7 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   a.xscale_words =
       (row_token || x.cols % kChunkK == 0) && ((reinterpret_cast<uintptr_t>(x.scales) | static_cast<uintptr_t>(x.scale_stride)) & 3) == 0;
   a.offsets = offsets;
+  a.gathered = row_token != nullptr;
   a.experts = static_cast<int>(w.experts);
   a.mtiles = static_cast<int>(l.mtiles);
   a.kchunks = static_cast<int>(l.kchunks);
@@ -1015,23 +1030,23 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   // A token has at most one row per expert, so no segment is longer than x.
   const int64_t most = row_token ? std::min(rows, given.rows) : rows;
   const int64_t mean = (rows + w.experts - 1) / w.experts;
-  int bn = kMaxN;
-  if (mean <= 16) bn = 32;
-  else if (mean <= 48) bn = 64;
-  else if (mean <= 112) bn = 128;
-  int cg = mean > 112 ? 2 : 1;
-  int g = cg == 2 ? 1 : 2;
+  // Few rows per expert: tiles of at most 128 rows, one CTA each; many: of 240, two CTAs
+  // each.  One CTA / two, us: 32 experts of 2880 x 1440 in e2m1 with 25 rows each 25 / 36,
+  // 75 rows 34 / 39, 150 rows 48 / 51; one of 4096 x 4096 with 400 rows 15 / 20; 64 gated of
+  // 2816 x 2048 with 1024 rows each 450 / 390, 8 of 4096 x 14336 in e4m3 550 / 470.  (Tiles
+  // of at most 64 rows cost the same time as ones of 128 and are more.)
+  const int cg = mean > kPairRows ? 2 : 1, bn = cg == 2 ? kMaxN : 128;
   a.bn = static_cast<int>(std::min<int64_t>(bn, (most + 15) / 16 * 16));
-  a.split = a.bn <= kSplitN && cg == 1 ? 32 : 0;
+  a.split = a.bn <= kSplitN ? kSplitTiles : 0;
   a.sf_rows = a.bn > 128 ? 1024 : 512;
   a.sf_block = 4 * (kSfBytes + a.sf_rows);
   const int fixed = 1024 + kSfRing * a.sf_block + (w.gated ? kGateBytes : 0)+
                     static_cast<int>(5 * w.experts + 2) * 4;
-  const int stage = g * (kTileM + a.bn / cg) * kChunkK;
+  const int stage = G * (kTileM + a.bn / cg) * kChunkK;
   a.stages = std::min(kMaxStages, (device_info().max_smem_optin - 1024 - fixed) / stage);
   if (a.stages < 2) return LP_ERR_UNSUPPORTED;
   Maps maps;
-  if (!encode_tiles(&maps.a, w.tiles, l.tiles, g, w.dtype == LP_E2M1)) return LP_ERR_UNSUPPORTED;
+  if (!encode_tiles(&maps.a, w.tiles, l.tiles, w.dtype == LP_E2M1)) return LP_ERR_UNSUPPORTED;
   const int boxes[kBoxes] = {32, 64, 128, 192, 256};
   for (int b = 0; b < kBoxes; ++b)
     if (!encode_rows(&maps.b[b], x.codes, x.cols, x.rows, x.code_stride, std::min(boxes[b], a.bn / cg)))
@@ -1039,7 +1054,8 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   const int smem = fixed + a.stages * stage;
   // M = 128 of a CTA, or 256 of a pair
   a.idesc |= static_cast<uint32_t>(cg * 128 >> 4) << 24;
-  return cg == 2 ? launch_g<2>(g, w.gated, maps, a, smem, st) : launch_g<1>(g, w.gated, maps, a, smem, st);
+  if (w.gated) return cg == 2 ? launch<2, true>(maps, a, smem, st) : launch<1, true>(maps, a, smem, st);
+  return cg == 2 ? launch<2, false>(maps, a, smem, st) : launch<1, false>(maps, a, smem, st);
 }
 
 unsigned int take_error_experts() {

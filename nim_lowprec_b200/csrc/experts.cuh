@@ -60,9 +60,10 @@ struct Args {
   const int32_t* offsets;
   int experts, mtiles, kchunks, k;
   int rows, tokens;           // rows of the result, rows of x
+  int gathered;               // the rows come from the kernel before
   int bn;                     // most rows of a tile, a multiple of 16
   int stages;
-  int split;                  // tiles per CTA below which they are cut (0: never)
+  int split;                  // tiles per CTA below which they are cut along K (0: never)
   uint32_t a_bytes;           // of a tile's codes
   uint32_t idesc;             // without N and the scale factors' ids
   uint8_t* out;               // rows (bytes between them: out_stride) or codes
