@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   // What the kernels before this one write is not read before here.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!a.gathered) asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldg(a.offsets + e);
+  for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldcg(a.offsets + e);
   __syncthreads();
   if (warp == 0) read_segments(a, seg, mtiles, lane);
   fence_before();
@@ -965,6 +965,7 @@ int launch(const Maps& maps, const Args& a, int smem, cudaStream_t st) {
   c.gridDim = dim3(ctas[slot]);
   return cuda_status(cudaLaunchKernelEx(&c, kern, maps, a));
 }
+
 }  // namespace
 
 int launch_pack_experts(const void* codes, const void* scales, int scale_type, const lp_expert_weights& w,
@@ -1000,8 +1001,8 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   a.xscales = static_cast<const uint8_t*>(x.scales);
   a.xscale_stride = x.scale_stride;
   // (a word holds four scales of one row where a row has a multiple of four, or zeros behind them)
-  a.xscale_words =
-      (row_token || x.cols % kChunkK == 0) && ((reinterpret_cast<uintptr_t>(x.scales) | static_cast<uintptr_t>(x.scale_stride)) & 3) == 0;
+  a.xscale_words = (row_token || x.cols % kChunkK == 0) &&
+                   ((reinterpret_cast<uintptr_t>(x.scales) | static_cast<uintptr_t>(x.scale_stride)) & 3) == 0;
   a.offsets = offsets;
   a.gathered = row_token != nullptr;
   a.experts = static_cast<int>(w.experts);
@@ -1037,7 +1038,7 @@ int launch_experts(const lp_expert_weights& w, const lp_rows8& given, const int3
   // of at most 64 rows cost the same time as ones of 128 and are more.)
   const int cg = mean > kPairRows ? 2 : 1, bn = cg == 2 ? kMaxN : 128;
   a.bn = static_cast<int>(std::min<int64_t>(bn, (most + 15) / 16 * 16));
-  a.split = a.bn <= kSplitN ? kSplitTiles : 0;
+  a.split = cg == 1 && a.bn <= kSplitN ? kSplitTiles : 0;  // (pairs do not join parts)
   a.sf_rows = a.bn > 128 ? 1024 : 512;
   a.sf_block = 4 * (kSfBytes + a.sf_rows);
   const int fixed = 1024 + kSfRing * a.sf_block + (w.gated ? kGateBytes : 0)+

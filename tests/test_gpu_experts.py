@@ -86,6 +86,14 @@ def test_segments(counts, kind):
     run(5, counts, len(counts) + 2, 256, 352, kind, "bf16", gather=max(counts))
 
 
+@pytest.mark.parametrize("counts", [[700], [500, 0, 300]])
+@pytest.mark.parametrize("tokens", [1, 20, 60, 100])
+def test_a_token_many_times(counts, tokens):
+    """More rows than tokens: the same few rows of x, again and again, for one expert."""
+    run(17, counts, len(counts), 300, 1024, "mx4", "fp32", gather=tokens)
+    run(17, counts, len(counts), 256, 1024, "mx8", gated=True, gather=tokens)
+
+
 @pytest.mark.parametrize("experts", [1, 31, 32, 33, 100, 1024])
 def test_experts(experts):
     counts = [(i * 7) % 5 if i % 3 else 0 for i in range(experts)]
