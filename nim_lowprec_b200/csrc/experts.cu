@@ -563,7 +563,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_experts(const __grid_constant__
   if (warp == 2 && lane <= kBoxes)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &maps.b[lane - 1] : &maps.a)) : "memory");
   // What the kernels before this one write is not read before here.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!a.gathered) asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int e = threadIdx.x; e <= a.experts; e += kThreads) seg.start[e] = __ldcg(a.offsets + e);
   __syncthreads();

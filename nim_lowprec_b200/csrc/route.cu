@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kThreads) k_route_choose(const RouteArgs a) {
     const int id = choose<PER>(a, t, lane);
     if (id >= 0) atomicAdd(&hist[id], 1);  // (a count: its order does not matter)
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // (the launch that places the rows, which waits before it reads anything)
+  if constexpr (!ONE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
   for (int e = threadIdx.x; e < a.n; e += kThreads) a.counts[int64_t{e} * kRouteCtas + blockIdx.x] = hist[e];
   if constexpr (ONE) {
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kThreads) k_route_choose(const RouteArgs a) {
 __global__ void __launch_bounds__(kThreads) k_route_place(const RouteArgs a) {
   __shared__ int32_t base[kRouteExperts], sums[kRouteExperts];
   __shared__ uint16_t ahead[kThreads / 32 * kRouteExperts];
-  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   scan_counts(a, gridDim.x, base, sums);
   const int64_t t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tokens);
   place(a, t0, t1, base, sums, ahead);

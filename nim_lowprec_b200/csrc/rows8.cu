@@ -14,11 +14,10 @@
 namespace lp {
 namespace {
 
-// Launched early (launch_early), a kernel lets the next one begin and waits for the one
-// before it: few rows are bound by launches, each of which then hides behind the last.
-__device__ __forceinline__ void begin() {
-  asm volatile("griddepcontrol.launch_dependents; griddepcontrol.wait;" ::: "memory");
-}
+// Launched early (launch_early), a kernel waits for the one before it.  It does not let the
+// next one begin early: what it writes may be the next GEMV's weights, which that reads
+// before its own wait.
+__device__ __forceinline__ void begin() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct Mat {  // rows of a matrix; p may be null
   uint8_t* p;

@@ -189,6 +189,24 @@ def test_int8_rows_feed_the_int8_product():
     assert bool(((y.view(m, t).double() - want).abs() <= a * 12 * 2.0 ** -24).all())
 
 
+def test_rows_may_be_the_next_product_s_weights():
+    """A GEMV reads its weights before it waits for the kernel before it, so that kernel must not let
+    it begin early: each call's product is that of the weights just written."""
+    g, m, k = R.gen(14), 8192, 2048
+    codes, scales = R.empty_rows8(m, k, "int8", 32)
+    xq = torch.randint(-127, 128, (k,), generator=g, device="cuda", dtype=torch.int8)
+    xs = torch.rand(k // 32, generator=g, device="cuda")
+    a, b = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    for _ in range(6):
+        w = R.randn(g, m, k)
+        torch.cuda.synchronize()
+        L.quantizeRows(w, codes, scales)
+        L.dequantGemvQ8(codes.reshape(-1), scales.reshape(-1), 32, xq, xs, a)
+        torch.cuda.synchronize()
+        L.dequantGemvQ8(codes.reshape(-1), scales.reshape(-1), 32, xq, xs, b)
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("rows", list(R.DT))
 @pytest.mark.parametrize("out", list(R.DT))
 @pytest.mark.parametrize("t,k,cols", [(1, 8, 4096), (37, 3, 96), (300, 1, 1000), (5, 9, 33)])
