@@ -8,7 +8,7 @@ Every .cu under csrc/ is compiled for `sm_100a` only (the library uses
 tcgen05/TMA-era PTX: bulk copies, mbarrier waits, f32x2 arithmetic) and
 linked into one shared object next to this file, with the CUDA runtime linked
 statically.  Where torch is installed, csrc/torch_binding.cpp becomes the
-CPython module _torch_binding beside it (the paged cache's entry points for
+CPython module _torch_binding beside it (the entry points of the cache and the experts for
 torch tensors).  The result travels with the repository snapshot; nothing is
 installed into site-packages.
 """
